@@ -420,6 +420,88 @@ int llamd_hip_be_rope(float *x, int rows, int row_len, const uint32_t *positions
 int llamd_hip_be_get_rows(const float *table, int table_rows, int row_len, const uint32_t *ids,
                           int n_ids, float *out);
 
+/* ---- paged KV cache: prompts, and batches that share prefixes -------------- */
+/* Not in the reference (its cache is one f32 slice per sequence, and a prompt
+ * goes through the decode step token by token). Keys and values lie in pages
+ * of f32, f16 or bf16; a table gives each sequence its pages, so sequences
+ * grow without a slice of max_kv each and may share pages. paged_store puts
+ * new tokens into the cache, paged_prompt attends for any number of new tokens
+ * per sequence, paged_decode for one token per sequence.
+ *
+ * All three are device-pointer calls, asynchronous on the library stream, 0 or
+ * -1. They read lengths, starts, tables and groups on the device, so a captured
+ * call follows them; what lies there never makes a call touch memory outside
+ * the buffers described:
+ *   a position whose page id is outside [0, n_page), or past the table's end,
+ *     is not stored, and attended to by no row;
+ *   a row that attends to nothing (an empty sequence) gives 0;
+ *   tokens before start[0] or from start[n_seq] on belong to no sequence:
+ *     their rows of q_out and out are left as they were.
+ * A masked position has no part in a row whatever it holds (infinities and NaN
+ * included). Two tokens stored at the same position of the same page in one
+ * call leave one of them there.
+ *
+ * Scores, softmax statistics and sums are f32; weights are rounded to the
+ * cache's type for their product with V, the result once at the end. With an
+ * f32 cache every product and sum is f32. Results do not depend on timing.
+ * Pointers are 16-byte aligned (the integer arrays 4). */
+#define LLAMD_HIP_F32 0 /* ggml's type numbers */
+#define LLAMD_HIP_F16 1
+#define LLAMD_HIP_BF16 30
+typedef struct {
+    void *k;       /* [n_page][n_head_kv][page][hd] */
+    void *v;       /* [n_page][n_head_kv][hd][page]: a dimension's positions together */
+    int type;      /* LLAMD_HIP_F32, _F16 or _BF16 */
+    int n_page;
+    int page;      /* positions per page: 16, 32, 64, 128 or 256 */
+    int n_head_kv;
+    int hd;        /* 64, 128 or 256 */
+} llamd_hip_pages;
+typedef struct {
+    const int32_t *start; /* [n_seq + 1], ascending: sequence s has the tokens
+                           * [start[s], start[s+1]) of the packed rows, none or
+                           * more; NULL: sequence s has token s */
+    const int32_t *len;   /* [n_seq] positions in the cache, these tokens
+                           * included: the last token is at position len - 1 */
+    const int32_t *table; /* [n_seq][max_page] page of positions i * page ... */
+    int n_seq;
+    int n_tok;            /* rows of q, k, v and out */
+    int max_page;
+} llamd_hip_batch;
+/* Host only: the rotary frequencies (radians per position) of n_rot / 2 pairs,
+ * base^(-2i/n_rot), for positions stretched by factor. orig_ctx 0: all of them
+ * divided by factor, *mscale 1. orig_ctx > 0 (the trained context): by parts,
+ * pairs that turn beta_slow times or less over orig_ctx are divided, those that
+ * turn beta_fast times or more are not, a linear ramp between; *mscale =
+ * 0.1 ln(factor) + 1 (the YaRN paper's, arXiv 2309.00071; usual beta 32 and 1). */
+int llamd_hip_rope_freqs(int n_rot, double base, double factor, int orig_ctx, double beta_fast,
+                         double beta_slow, double *freqs, float *mscale);
+/* New tokens' q (may be NULL, with q_out), k, v: f32 rows ld_* floats apart
+ * (multiples of 4; one matrix may hold all three) of n_head (n_head_kv) heads.
+ * Per head: x / sqrt(mean(x^2) + eps) * norm (norm NULL: not), then the
+ * rotation by position * freqs[i] (device, n_rot / 2 doubles; angles in 64
+ * bits) times mscale of pairs (i, i + n_rot/2), or (2i, 2i + 1) when
+ * interleaved; dimensions from n_rot on pass. k and v go to their pages, q to
+ * q_out [n_tok][n_head * hd] in the cache's type. */
+int llamd_hip_paged_store(const llamd_hip_pages *c, const llamd_hip_batch *b, const float *q, int ld_q,
+                          const float *k, int ld_k, const float *v, int ld_v, const float *q_norm,
+                          const float *k_norm, float eps, const double *freqs, int n_rot,
+                          int interleaved, float mscale, int n_head, void *q_out);
+/* out[t] = softmax over positions 0 .. the token's own of (scale q . k) v, per
+ * head (n_head / n_head_kv query heads share a kv head). q [n_tok][n_head * hd]
+ * in the cache's type; out the same shape, of the cache's type or f32. */
+int llamd_hip_paged_prompt(const llamd_hip_pages *c, const llamd_hip_batch *b, const void *q, int n_head,
+                           float scale, int out_type, void *out);
+/* The same for one token per sequence, row s of q and out (b->start is not
+ * read), attending to all len[s] positions. Groups of consecutive sequences
+ * (group [n_group + 1] ascending first sequences; n_group 0: none) share their
+ * first shared[g] positions: the pages that these fill (shared[g] / page) are
+ * read once for the group, through the table row of its first sequence; the
+ * page that they end in is each sequence's own. */
+int llamd_hip_paged_decode(const llamd_hip_pages *c, const llamd_hip_batch *b, const int32_t *group,
+                           const int32_t *shared, int n_group, const void *q, int n_head, float scale,
+                           int out_type, void *out);
+
 /* ---- one MoE decode layer (R8 router -> R9 route -> R11 moe_ffn -> R12) ---- */
 /* Not in the reference as one call: DeviceModel::queue_token's MoE phases
  * (crates/llamd-runtime/src/device.rs:486-655) behind a handle.

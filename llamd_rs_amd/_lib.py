@@ -195,6 +195,10 @@ SIGNATURES = {
     "llamd_hip_be_matmul": (i32, [vp, vp, vp, i32, i32, i32]),
     "llamd_hip_be_rope": (i32, [vp, i32, i32, vp, i32, f, f]),
     "llamd_hip_be_get_rows": (i32, [vp, i32, i32, vp, i32, vp]),
+    "llamd_hip_rope_freqs": (i32, [i32, C.c_double, C.c_double, i32, C.c_double, C.c_double, vp, f32p]),
+    "llamd_hip_paged_store": (i32, [vp, vp, vp, i32, vp, i32, vp, i32, vp, vp, f, vp, i32, i32, f, i32, vp]),
+    "llamd_hip_paged_prompt": (i32, [vp, vp, vp, i32, f, i32, vp]),
+    "llamd_hip_paged_decode": (i32, [vp, vp, vp, vp, i32, vp, i32, f, i32, vp]),
     # host-side synthetic data (llamd_rs_amd/csrc/host/synth.cpp)
     "llamd_synth_normal": (None, [u64, f, vp, sz]),
     "llamd_synth_f32_to_f16": (u16, [f]),

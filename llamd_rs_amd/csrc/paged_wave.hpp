@@ -1,0 +1,177 @@
+// paged_wave.hpp -- attention of one wave: 32 query rows that share a kv head against 32 cached positions at a time, with
+// the running maximum and sum of the softmax.
+//
+// A row is a query head of a token. The wave forms S^T = K Q^T and O^T += V^T P^T with 32x32 matrix instructions, so
+// that a lane holds values of one row (lane & 31) throughout: the maximum and the sum are the lane's own but for one
+// exchange with its other half (lane ^ 32), and P^T leaves the softmax in the registers that the second product reads as
+// its right operand. That operand wants a run of RUN positions per half; the rows of K are read in the order that
+// makes the first product leave them so (kv_row). Both left operands are 16-byte runs of memory: K pages hold a
+// position's dimensions together, V pages a dimension's positions.
+//
+// Exponentials are powers of two: x = s * (scale * log2 e) - m. Scores, maxima, sums and O are f32. P is rounded to the
+// cache's type for the second product (half a unit in the last place of values in [0, 1], independent per position, of
+// the size of V's own rounding); the sum l adds the unrounded values.
+#pragma once
+
+#include "paged_util.hpp"
+
+namespace llamd {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t run4 __attribute__((ext_vector_type(4)));  // a 16-byte run of elements
+
+template <class E> struct Mma;
+template <> struct Mma<ElemF16> {
+    typedef _Float16 V __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ v16f mul(run4 a, run4 b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t EXP = 0x7C007C00u;
+};
+template <> struct Mma<ElemBF16> {
+    typedef __bf16 V __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ v16f mul(run4 a, run4 b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t EXP = 0x7F807F80u;
+};
+template <> struct Mma<ElemF32> {
+    static __device__ __forceinline__ v16f mul(run4 a, run4 b, v16f c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+        return c;
+    }
+    static constexpr uint32_t EXP = 0x7F800000u;
+};
+
+constexpr float NEG_INF = -INFINITY;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, WAVE); }
+
+// The maximum that x is taken against: an empty row's is 0, so that its terms are exp2(-inf) = 0 and not NaN.
+__device__ __forceinline__ float against(float m) { return m == NEG_INF ? 0.0f : m; }
+
+// Position (0..31) that row m of the first product's left operand holds, and the one that a lane's score register i is of.
+template <class E> __device__ __forceinline__ int kv_row(int m) {
+    const int i = 4 * (m >> 3) + (m & 3), h = (m >> 2) & 1;
+    return 2 * E::RUN * (i / E::RUN) + E::RUN * h + i % E::RUN;
+}
+template <class E> __device__ __forceinline__ int kv_reg(int i, int h) {
+    return 2 * E::RUN * (i / E::RUN) + E::RUN * h + i % E::RUN;
+}
+
+// A run's elements whose bits are set in `keep` as they are, the others zero.
+template <class E> __device__ __forceinline__ run4 keep_elements(run4 r, uint32_t keep) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (E::RUN == 4) {
+            r[j] &= (keep >> j & 1) ? 0xFFFFFFFFu : 0u;
+        } else {
+            r[j] &= ((keep >> (2 * j) & 1) ? 0xFFFFu : 0u) | ((keep >> (2 * j + 1) & 1) ? 0xFFFF0000u : 0u);
+        }
+    }
+    return r;
+}
+// Bit e: element e is an infinity or NaN.
+template <class E> __device__ __forceinline__ uint32_t not_finite(run4 r) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (E::RUN == 4) {
+            bits |= (uint32_t)((r[j] & Mma<E>::EXP) == Mma<E>::EXP) << j;
+        } else {
+            const uint32_t lo = Mma<E>::EXP & 0xFFFFu, hi = Mma<E>::EXP & 0xFFFF0000u;
+            bits |= (uint32_t)((r[j] & lo) == lo) << (2 * j) | (uint32_t)((r[j] & hi) == hi) << (2 * j + 1);
+        }
+    }
+    return bits;
+}
+
+template <class E> __device__ __forceinline__ run4 to_run(const float *x) {
+    run4 r;
+    if constexpr (E::RUN == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = __float_as_uint(x[j]);
+    } else {
+        typedef typename E::T V __attribute__((ext_vector_type(8)));
+        V v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = E::put(x[j]);
+        r = __builtin_bit_cast(run4, v);
+    }
+    return r;
+}
+
+// The state of 32 rows.
+template <class E, int HD> struct RowState {
+    static constexpr int DB = HD / 32;             // blocks of 32 dimensions
+    static constexpr int QS = HD / (2 * E::RUN);   // steps of the first product
+    static constexpr int PS = 32 / (2 * E::RUN);   // steps of the second
+    v16f o[DB];
+    float m, l;  // the maximum of x, and this half's part of the sum
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+        m = NEG_INF;
+        l = 0.0f;
+    }
+
+    // One step of the second product where some of V is not to be read as it stands: of the runs v(d) of the dimension
+    // blocks, the elements of `keep` are positions that a row attends to, the others may hold anything. An infinity or
+    // NaN at a position that only some rows attend to gives the others nothing, not 0 * inf: such elements are left
+    // out of the product and added one position at a time (pos0 + e) to the rows that see it.
+    template <class Load>
+    __device__ __forceinline__ void add_masked(Load v, uint32_t keep, run4 p, int pos0, int limit) {
+        const int h = (threadIdx.x >> 5) & 1;
+        uint32_t any = 0;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            const run4 x = keep_elements<E>(v(d), keep);
+            const uint32_t bad = not_finite<E>(x);
+            any |= bad;
+            o[d] = Mma<E>::mul(keep_elements<E>(x, ~bad), p, o[d]);
+        }
+        if (!__any(any != 0)) return;
+        for (int e = 0; e < 2 * E::RUN; ++e) {
+            const uint32_t one = (e / E::RUN == h) ? 1u << (e % E::RUN) : 0u;
+            if (!__any((any & one) != 0)) continue;
+            const bool seen = pos0 + e < limit;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const run4 x = keep_elements<E>(v(d), keep & one);
+                const v16f t = Mma<E>::mul(keep_elements<E>(x, not_finite<E>(x)), keep_elements<E>(p, one), o[d]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] = seen ? t[i] : o[d][i];
+            }
+        }
+    }
+
+    // Scores of 32 positions (kv_reg's order) to P, the statistics and O's scale brought up to date.
+    __device__ __forceinline__ void softmax(v16f &s, float scale) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top = fmaxf(top, other_half(top)) * scale;
+        const float m1 = fmaxf(m, top), ref = against(m1);
+        const float shrink = exp2_fast(m - ref);
+        m = m1;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = exp2_fast(__builtin_fmaf(s[i], scale, -ref));
+            sum += s[i];
+        }
+        l = __builtin_fmaf(l, shrink, sum);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
+    }
+};
+
+}  // namespace llamd

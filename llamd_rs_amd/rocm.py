@@ -493,7 +493,158 @@ class LmHead:
             pass
 
 
+class Pages(C.Structure):
+    """llamd_hip_pages: a paged cache's memory. k [n_page][n_head_kv][page][hd],
+    v [n_page][n_head_kv][hd][page]; type is ggml's number (PAGE_TYPES)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("n_page", C.c_int),
+                ("page", C.c_int), ("n_head_kv", C.c_int), ("hd", C.c_int)]
+
+
+class Batch(C.Structure):
+    """llamd_hip_batch: the packed tokens of a call (device pointers)."""
+    _fields_ = [("start", C.c_void_p), ("len", C.c_void_p), ("table", C.c_void_p),
+                ("n_seq", C.c_int), ("n_tok", C.c_int), ("max_page", C.c_int)]
+
+
+PAGE_TYPES = {"f32": 0, "f16": 1, "bf16": 30}
+
+
+def to_bf16(x) -> np.ndarray:
+    """f32 -> bf16 bits (uint16), rounded to nearest even."""
+    u = _f32(x).view(np.uint32)
+    nan = np.isnan(_f32(x))
+    r = ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(nan, np.uint16(0x7FC0), r)
+
+
+def from_bf16(b) -> np.ndarray:
+    return (np.ascontiguousarray(b, np.uint16).astype(np.uint32) << 16).view(np.float32)
+
+
+def rope_freqs(n_rot: int, base: float, factor: float = 1.0, orig_ctx: int = 0, beta_fast: float = 32.0,
+               beta_slow: float = 1.0) -> tuple[np.ndarray, float]:
+    """(radians per position [n_rot / 2] f64, magnitude): llamd_hip_rope_freqs."""
+    f = np.empty(max(n_rot, 2) // 2, np.float64)
+    m = C.c_float()
+    check(lib().llamd_hip_rope_freqs(n_rot, base, factor, orig_ctx, beta_fast, beta_slow, _ptr(f), C.byref(m)),
+          "rope_freqs")
+    return f, m.value
+
+
+class PagedCache:
+    """One layer's paged KV cache (llamd_hip_paged_*) with host arrays in and
+    out. A batch is (table [n_seq, max_page], length [n_seq], start [n_seq + 1]
+    or None for one token each); q and results cross as f32. A program that
+    keeps its data on the device fills Pages and Batch and calls the C ABI."""
+
+    def __init__(self, type: str, n_page: int, page: int, n_head: int, n_head_kv: int, hd: int):
+        if type not in PAGE_TYPES:
+            raise ValueError(f"type {type!r}: f32, f16 or bf16")
+        if min(n_page, page, n_head_kv, hd) <= 0:
+            raise ValueError("n_page, page, n_head_kv and hd must be positive")
+        self.type, self.n_head = type, n_head
+        self.dtype = {"f32": np.float32, "f16": np.float16, "bf16": np.uint16}[type]
+        self.shape_k, self.shape_v = (n_page, n_head_kv, page, hd), (n_page, n_head_kv, hd, page)
+        zero = np.zeros(self.shape_k, self.dtype)
+        self._k, self._v = DeviceBuffer.from_array(zero), DeviceBuffer.from_array(zero)
+        self.pages = Pages(self._k.ptr, self._v.ptr, PAGE_TYPES[type], n_page, page, n_head_kv, hd)
+
+    def encode(self, x) -> np.ndarray:
+        return to_bf16(x) if self.type == "bf16" else _f32(x).astype(self.dtype)
+
+    def decode_values(self, x) -> np.ndarray:
+        return from_bf16(x) if self.type == "bf16" else x.astype(np.float32)
+
+    def read(self) -> tuple[np.ndarray, np.ndarray]:
+        """(K, V) pages as f32."""
+        k = self._k.download(np.empty(self.shape_k, self.dtype))
+        v = self._v.download(np.empty(self.shape_v, self.dtype))
+        return self.decode_values(k), self.decode_values(v)
+
+    def write(self, k, v):
+        k, v = self.encode(k), self.encode(v)
+        if k.shape != self.shape_k or v.shape != self.shape_v:
+            raise ValueError(f"pages are {self.shape_k} and {self.shape_v}")
+        self._k.upload(k)
+        self._v.upload(v)
+
+    def _batch(self, table, length, start, n_tok):
+        table = np.ascontiguousarray(np.atleast_2d(table), np.int32)
+        length = np.ascontiguousarray(length, np.int32)
+        if table.shape[0] != length.size or (start is not None and len(start) != length.size + 1):
+            raise ValueError("one table row, length and start per sequence")
+        keep = [DeviceBuffer.from_array(length), DeviceBuffer.from_array(table)]
+        if start is not None:
+            keep.append(DeviceBuffer.from_array(np.ascontiguousarray(start, np.int32)))
+        b = Batch(keep[2].ptr if start is not None else None, keep[0].ptr, keep[1].ptr, length.size, n_tok,
+                  table.shape[1])
+        return b, keep
+
+    def store(self, q, k, v, table, length, start=None, q_norm=None, k_norm=None, eps: float = 1e-6, freqs=None,
+              interleaved: bool = False, mscale: float = 1.0) -> np.ndarray:
+        """q [n_tok, n_head * hd], k, v [n_tok, n_head_kv * hd]; the rotated q
+        (f32 values of the cache's type), k and v in the pages."""
+        n, _, page, hd = self.shape_k
+        kvh = self.shape_k[1]
+        q, k, v = _f32(q), _f32(k), _f32(v)
+        if q.shape[1:] != (self.n_head * hd,) or k.shape != (q.shape[0], kvh * hd) or v.shape != k.shape:
+            raise ValueError("q must be [n_tok, n_head * hd], k and v [n_tok, n_head_kv * hd]")
+        for w in (q_norm, k_norm):
+            if w is not None and np.size(w) != hd:
+                raise ValueError("norm weights must be [hd]")
+        b, keep = self._batch(table, length, start, q.shape[0])
+        dev = [DeviceBuffer.from_array(x) for x in (q, k, v)]
+        norms = [None if w is None else DeviceBuffer.from_array(_f32(w)) for w in (q_norm, k_norm)]
+        fr = None if freqs is None else DeviceBuffer.from_array(np.ascontiguousarray(freqs, np.float64))
+        out = DeviceBuffer.from_array(np.zeros(q.shape, self.dtype))
+        check(lib().llamd_hip_paged_store(
+            C.byref(self.pages), C.byref(b), dev[0].ptr, self.n_head * hd, dev[1].ptr, kvh * hd, dev[2].ptr, kvh * hd,
+            *(None if w is None else w.ptr for w in norms), eps, fr and fr.ptr,
+            0 if freqs is None else 2 * len(freqs), int(interleaved), mscale, self.n_head, out.ptr), "paged_store")
+        return self.decode_values(out.download(np.empty(q.shape, self.dtype)))
+
+    def _attend(self, call, q, table, length, start, scale, f32_out):
+        hd = self.shape_k[3]
+        q = self.encode(q)
+        if q.ndim != 2 or q.shape[1] != self.n_head * hd:
+            raise ValueError("q must be [n_tok, n_head * hd]")
+        b, keep = self._batch(table, length, start, q.shape[0])
+        dq = DeviceBuffer.from_array(q)
+        dtype = np.float32 if f32_out else self.dtype
+        out = DeviceBuffer.from_array(np.zeros(q.shape, dtype))
+        call(b, dq, hd ** -0.5 if scale is None else scale, 0 if f32_out else PAGE_TYPES[self.type], out)
+        got = out.download(np.empty(q.shape, dtype))
+        return got if f32_out else self.decode_values(got)
+
+    def prompt(self, q, table, length, start, scale: float | None = None, f32_out: bool = False) -> np.ndarray:
+        """Causal attention of the packed tokens q [n_tok, n_head * hd]."""
+        def call(b, dq, scale, number, out):
+            check(lib().llamd_hip_paged_prompt(C.byref(self.pages), C.byref(b), dq.ptr, self.n_head, scale, number,
+                                               out.ptr), "paged_prompt")
+        return self._attend(call, q, table, length, start, scale, f32_out)
+
+    def decode(self, q, table, length, group=None, shared=None, scale: float | None = None,
+               f32_out: bool = False) -> np.ndarray:
+        """One token per sequence; group [n_group + 1] first sequences and
+        shared [n_group] positions where sequences share a prefix."""
+        if (group is None) != (shared is None) or (group is not None and len(group) != len(shared) + 1):
+            raise ValueError("group and shared go together, one more first sequence than groups")
+        g = None if group is None else [DeviceBuffer.from_array(np.ascontiguousarray(x, np.int32))
+                                        for x in (group, shared)]
+
+        def call(b, dq, scale, number, out):
+            check(lib().llamd_hip_paged_decode(C.byref(self.pages), C.byref(b), g and g[0].ptr, g and g[1].ptr,
+                                               0 if g is None else len(shared), dq.ptr, self.n_head, scale, number,
+                                               out.ptr), "paged_decode")
+        return self._attend(call, q, table, length, None, scale, f32_out)
+
+    def close(self):
+        self._k.close()
+        self._v.close()
+
+
 __all__ = [
+    "Pages", "Batch", "PagedCache", "PAGE_TYPES", "rope_freqs", "to_bf16", "from_bf16",
     "BlockQ8K", "DeviceInfo", "DeviceWeights", "Q8_0Weights", "MoeLayer", "LmHead", "Routing",
     "DeviceBuffer", "available", "device_count", "device_info", "quantize_q8k_on_device",
     "swiglu_q8k_on_device", "matvec_q6k", "route", "argmax", "HipError", "HipUnavailable",
