@@ -587,6 +587,9 @@ int llamd::shadow_q6k(const void *w, const size_t *off, int rows, int blocks, co
     return 0;
 }
 
+void *llamd::lib_scratch(size_t bytes) { return scratch(bytes); }
+std::mutex &llamd::lib_scratch_mutex() { return g_smu; }
+
 extern "C" {
 
 // ---- memory ----------------------------------------------------------------

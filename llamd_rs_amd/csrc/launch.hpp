@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace llamd {
 
 // The byte of weight e of token n within its (chunk, block)'s 4 KiB of the
@@ -358,6 +360,11 @@ int launch_matmul_f32_seq(const float *w, const float *x, float *out, int m, int
 // ---- shared by the C ABI's host files ----
 // The library's stream (capi.cpp).
 hipStream_t lib_stream();
+// Library scratch of at least `bytes`, reused call by call in stream order (null: no memory, the error set); hold the
+// mutex from the call to the last launch that uses it. A buffer that a larger one replaces stays for graphs that
+// captured it.
+void *lib_scratch(size_t bytes);
+std::mutex &lib_scratch_mutex();
 // A void device-pointer entry point refused its arguments (the text is in
 // llamd_hip_last_error); llamd_fwd_last_error reports it once (capi.cpp).
 void fwd_refused();

@@ -1,5 +1,5 @@
 // paged.cpp -- the C entry points of the paged cache (include/llamd_hip.h): argument checks and descriptors for the
-// kernels of paged_store.hip and paged_attend.hip. Lengths, starts, tables and groups are device arrays that the host
+// kernels of paged_store.hip and paged_attend.hpp. Lengths, starts, tables and groups are device arrays that the host
 // does not read, so that a captured call follows them; the kernels keep them inside the buffers given here.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -74,6 +74,12 @@ int describe_attend(const char *what, const llamd_hip_pages *c, const llamd_hip_
     a->out_f32 = out_type == PT_F32;
     a->scale = (float)(scale * 1.4426950408889634074);
     return 0;
+}
+
+int attend(const char *what, const PagedAttendArgs &a, int type, bool decode) {
+    const auto launch = type == PT_F32 ? launch_paged_attend_f32
+                        : type == PT_F16 ? launch_paged_attend_f16 : launch_paged_attend_bf16;
+    return launch(a, decode, lib_stream()) ? set_error("%s: launch", what) : 0;
 }
 
 }  // namespace
@@ -153,7 +159,7 @@ int llamd_hip_paged_prompt(const llamd_hip_pages *c, const llamd_hip_batch *b, c
     PagedAttendArgs a{};
     if (describe_attend("paged_prompt", c, b, q, n_head, scale, out_type, out, &a)) return -1;
     if (!b->n_seq || !b->n_tok) return 0;
-    return launch_paged_prompt(a, c->type, lib_stream()) ? set_error("paged_prompt: launch") : 0;
+    return attend("paged_prompt", a, c->type, false);
 }
 
 int llamd_hip_paged_decode(const llamd_hip_pages *c, const llamd_hip_batch *b, const int32_t *group,
@@ -169,7 +175,7 @@ int llamd_hip_paged_decode(const llamd_hip_pages *c, const llamd_hip_batch *b, c
     a.group_at = group;
     a.shared = shared;
     a.n_groups = n_group;
-    return launch_paged_decode(a, c->type, lib_stream()) ? set_error("paged_decode: launch") : 0;
+    return attend("paged_decode", a, c->type, true);
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-// paged.hpp -- arguments of the paged-cache kernels (paged_store.hip, paged_attend.hip) and their launchers. The entry
+// paged.hpp -- arguments of the paged-cache kernels (paged_store.hip, paged_attend.hpp) and their launchers. The entry
 // points (paged.cpp) check everything that the host can see; the kernels check what lies on the device (sequence starts,
 // lengths, page ids) before it becomes an address.
 #pragma once
@@ -47,8 +47,9 @@ struct PagedAttendArgs {
 
 // paged_store.hip
 int launch_paged_store(const PagedStoreArgs &a, int type, hipStream_t st);
-// paged_attend.hip
-int launch_paged_prompt(const PagedAttendArgs &a, int type, hipStream_t st);
-int launch_paged_decode(const PagedAttendArgs &a, int type, hipStream_t st);
+// paged_attend_*.hip: a prompt batch or a decode batch
+int launch_paged_attend_f32(const PagedAttendArgs &a, bool decode, hipStream_t st);
+int launch_paged_attend_f16(const PagedAttendArgs &a, bool decode, hipStream_t st);
+int launch_paged_attend_bf16(const PagedAttendArgs &a, bool decode, hipStream_t st);
 
 }  // namespace llamd

@@ -47,6 +47,13 @@ template <> struct Mma<ElemF32> {
 
 constexpr float NEG_INF = -INFINITY;
 
+// Four values at an element of `out`, rounded to the type, or f32.
+template <class E> __device__ __forceinline__ void put4(void *out, size_t at, float4 x) {
+    typedef typename E::T V __attribute__((ext_vector_type(4)));
+    const V v = {E::put(x.x), E::put(x.y), E::put(x.z), E::put(x.w)};
+    *(V *)((typename E::T *)out + at) = v;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, WAVE); }
 
@@ -104,13 +111,17 @@ template <class E> __device__ __forceinline__ run4 to_run(const float *x) {
     return r;
 }
 
-// The state of 32 rows.
+// Scores this much above the running maximum (as powers of two) are taken against it without a new one: weights stay below
+// 2^LAZY, and O is rescaled only where a row's maximum climbs further, which after the first few tiles it hardly does.
+constexpr float LAZY = 8.0f;
+
+// 32 rows' running softmax and O, over tiles of 32 * SUB positions.
 template <class E, int HD> struct RowState {
     static constexpr int DB = HD / 32;             // blocks of 32 dimensions
     static constexpr int QS = HD / (2 * E::RUN);   // steps of the first product
-    static constexpr int PS = 32 / (2 * E::RUN);   // steps of the second
+    static constexpr int PS = 32 / (2 * E::RUN);   // steps of the second, per 32 positions
     v16f o[DB];
-    float m, l;  // the maximum of x, and this half's part of the sum
+    float m, l;  // what x is taken against, and this half's part of the sum
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -119,6 +130,43 @@ template <class E, int HD> struct RowState {
             for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
         m = NEG_INF;
         l = 0.0f;
+    }
+
+    // Scores (kv_reg's order) to weights, the statistics and O's scale brought up to date.
+    template <int SUB> __device__ __forceinline__ void softmax(v16f (&s)[SUB], float scale) {
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < SUB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+        top = fmaxf(top, other_half(top)) * scale;
+        if (__any(top > m + LAZY)) {
+            const float m1 = fmaxf(m, top), shrink = exp2_fast(m - against(m1));
+            m = m1;
+            l *= shrink;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
+        }
+        const float ref = against(m);
+        float sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < SUB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = exp2_fast(__builtin_fmaf(s[b][i], scale, -ref));
+                sum += s[b][i];
+            }
+        l += sum;
+    }
+
+    // The right operand of step c of the second product.
+    static __device__ __forceinline__ run4 weights(const v16f &s, int c) {
+        float x[E::RUN];
+#pragma unroll
+        for (int j = 0; j < E::RUN; ++j) x[j] = s[c * E::RUN + j];
+        return to_run<E>(x);
     }
 
     // One step of the second product where some of V is not to be read as it stands: of the runs v(d) of the dimension
@@ -137,6 +185,7 @@ template <class E, int HD> struct RowState {
             o[d] = Mma<E>::mul(keep_elements<E>(x, ~bad), p, o[d]);
         }
         if (!__any(any != 0)) return;
+#pragma unroll 1
         for (int e = 0; e < 2 * E::RUN; ++e) {
             const uint32_t one = (e / E::RUN == h) ? 1u << (e % E::RUN) : 0u;
             if (!__any((any & one) != 0)) continue;
@@ -151,26 +200,19 @@ template <class E, int HD> struct RowState {
         }
     }
 
-    // Scores of 32 positions (kv_reg's order) to P, the statistics and O's scale brought up to date.
-    __device__ __forceinline__ void softmax(v16f &s, float scale) {
-        float top = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        top = fmaxf(top, other_half(top)) * scale;
-        const float m1 = fmaxf(m, top), ref = against(m1);
-        const float shrink = exp2_fast(m - ref);
-        m = m1;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[i] = exp2_fast(__builtin_fmaf(s[i], scale, -ref));
-            sum += s[i];
-        }
-        l = __builtin_fmaf(l, shrink, sum);
+    // O to a row of HD values, of the type or f32.
+    template <class W> __device__ __forceinline__ void write_as(void *out, size_t row) const {
+        const int h = (threadIdx.x >> 5) & 1;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
+            for (int i = 0; i < 16; i += 4)
+                put4<W>(out, row * HD + 32 * d + 2 * i + 4 * h,
+                        make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]));
+    }
+    __device__ __forceinline__ void write(void *out, bool f32, size_t row) const {
+        if (f32) write_as<ElemF32>(out, row);
+        else write_as<E>(out, row);
     }
 };
 
