@@ -228,55 +228,105 @@ __device__ __forceinline__ void attend_pages(const PagedArgs &p, const Pages<E> 
 
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
+// x, as something that the compiler cannot keep the results of between tiles: addresses are cheaper made again than held
+// in registers.
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// Asks the scheduler for N reads of a block's operands 6 ahead of their products (left alone it places each right before
+// its product, which then waits for LDS every time).
+template <class E, int N> __device__ __forceinline__ void order_reads() {
+    constexpr int MFMA = E::RUN == 8 ? 1 : 4, AHEAD = N < 6 ? N : 6;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, MFMA, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * MFMA, 0);
+}
+
 // Least steps of a part.
 constexpr int TILE_STEPS = 4;
 
-template <class E, int HD, int NQ, bool PREFIX>
-__global__ __launch_bounds__(256, NQ == 1 && HD * sizeof(typename E::T) <= 256 ? 2 : 1) void paged_tiles(PagedAttendArgs a, Split sp) {
+// O over the sum, to this lane's row (at < 0: none).
+template <class E, int HD>
+__device__ __forceinline__ void write_rows(void *out, bool f32, long long at, RowState<E, HD> &st, float l) {
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
+    if (at >= 0) st.write(out, f32, (size_t)at);
+}
+
+// A wave's rows once more, straight from the pages, every infinity or NaN in V added only where it belongs. A function of
+// its own: its registers would cost paged_tiles some of the reads that it keeps in flight.
+struct Again {
+    PagedArgs p;
+    Split sp;
+    Tile t;
+    int kvh, begin, end;
+    const void *q;
+    void *out;  // null: a part, to `slot`
+    bool out_f32;
+    float scale;
+    size_t slot;
+};
+template <class E, int HD>
+__device__ __attribute__((noinline)) void attend_again(const Again &x, int limit, long long at) {
+    run4 q[HD / (2 * E::RUN)];
+    load_rows<E, HD>(q, x.q, at);
+    RowState<E, HD> st;
+    st.clear();
+    attend_pages<E, HD, 32>(x.p, pages_of<E, HD>(x.p, x.t.seq, x.kvh), x.t, limit, x.begin, x.end, q, x.scale, st);
+    const float l = add_halves(st.l);
+    if (x.out) write_rows<E, HD>(x.out, x.out_f32, at, st, l);
+    else write_part<E, HD>(x.sp, x.slot, st, l);
+}
+
+// W waves of 32 rows each.
+template <class E, int HD, int W, bool PREFIX>
+__global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256 ? 2 : 1) void paged_tiles(PagedAttendArgs a, Split sp) {
     typedef typename E::T T;
     typedef RowState<E, HD> S;
-    constexpr int RUN = E::RUN, R = 128 * NQ;
+    constexpr int RUN = E::RUN, R = 32 * W, THREADS = 64 * W;
     constexpr int KT = HD * sizeof(T) * 256 <= 131072 ? 64 : 32;  // positions per tile: two buffers of K and V in 128 KB
     constexpr int SUB = KT / 32;
     constexpr int KCH = HD / RUN, VCH = KT / RUN;                 // 16-byte runs per row of a tile
-    constexpr int N = KT * KCH / 256;                             // loads of each thread per K (V) tile
+    constexpr int N = KT * KCH / THREADS;                             // loads of each thread per K (V) tile
     __shared__ __align__(16) run4 lds[2][2][KT * KCH];
     const PagedArgs &p = a.p;
-    const int lane = threadIdx.x & 63, h = lane >> 5, m = lane & 31;
+    const int lane = threadIdx.x & 63, m = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // the last tiles, which have the most positions, go first
     const int unit = gridDim.x / p.n_kv_head - 1 - blockIdx.x / p.n_kv_head, kvh = blockIdx.x % p.n_kv_head;
     int tile = unit, rows_end;
     Tile t;
-    Row row[NQ];
+    Row row;
     if constexpr (PREFIX) {
         Group g;
         if (!prefix_tile<R>(a, tile, t, rows_end, g)) return;
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) row[n] = prefix_row<R>(a, tile, t, rows_end, g, kvh, 32 * (NQ * wave + n) + m);
+        row = prefix_row<R>(a, tile, t, rows_end, g, kvh, 32 * wave + m);
     } else {
         TokenSpan span;
         if (!prompt_tile<R>(p, tile, t, rows_end, span)) return;
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) row[n] = prompt_row<R>(p, tile, t, rows_end, span, kvh, 32 * (NQ * wave + n) + m);
+        row = prompt_row<R>(p, tile, t, rows_end, span, kvh, 32 * wave + m);
     }
     const int steps = (t.top + KT - 1) / KT, parts = parts_of(steps, sp.parts, TILE_STEPS);
     if ((int)blockIdx.y >= parts) return;
     const int2 range = part_steps(steps, parts, blockIdx.y);
     // positions that all rows of this wave attend to, and that any does
-    int all = row[0].limit, any = row[0].limit;
-#pragma unroll
-    for (int n = 1; n < NQ; ++n) all = min(all, row[n].limit), any = max(any, row[n].limit);
-    all = wave_reduce(all, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
-    any = wave_reduce(any, 0, [](int x, int y) { return max(x, y); });
+    const int all = wave_reduce(row.limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
+    const int any = wave_reduce(row.limit, 0, [](int x, int y) { return max(x, y); });
 
-    run4 q[NQ][S::QS];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) load_rows<E, HD>(q[n], a.q, row[n].at);
-    S st[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) st[n].clear();
+    run4 q[S::QS];
+    load_rows<E, HD>(q, a.q, row.at);
+    S st;
+    st.clear();
     const Pages<E> g = pages_of<E, HD>(p, t.seq, kvh);
 
     // runs of a tile's row are exchanged by the row's number, so that 16 lanes that read the same run of consecutive
@@ -285,128 +335,168 @@ __global__ __launch_bounds__(256, NQ == 1 && HD * sizeof(typename E::T) <= 256 ?
     const auto v_swap = [](int r) { return VCH >= 16 ? r & 15 : (r >> 1) & 7; };
     // the table's entry for position step * KT + lane, looked at a step later (a use at once would wait for it)
     const auto entry = [&](int step) { return g.table[min(step * KT + (lane & (KT - 1)), t.n_kv - 1) >> p.page_log]; };
-    // this thread's runs of a K and V tile: at = base + lane, into row at / KCH (at / VCH), place at % KCH (at % VCH)
-    const auto stage = [&](int step, int id) {
-        const int t0 = step * KT, page = (unsigned)id < (unsigned)p.n_page ? id : 0;
-        run4 *kd = lds[step & 1][0], *vd = lds[step & 1][1];
+    // This thread's runs of a K and V tile: number at = 256 i + thread, in row at / KCH (at / VCH). A tile inside one page
+    // is a uniform address and a lane's offset; with smaller pages every run asks for its page. They pass through
+    // registers: loads straight into LDS return a quarter as much per cycle.
+    const bool one_page = 1 << p.page_log >= KT;
+    // (step's page: the table's entry for its position of this lane)
+    const auto page_or_0 = [&](int id) { return (unsigned)id < (unsigned)p.n_page ? id : 0; };
+    const auto load_k = [&](run4 (&x)[N], int step, int id) {
+        const int t0 = step * KT;
+        const uint32_t tid = fresh(threadIdx.x);
+        if (one_page) {
+            const int page = page_or_0(__builtin_amdgcn_readfirstlane(id));
+            const char *k = (const char *)(g.k + (size_t)page * g.step + (size_t)(t0 & g.mask) * HD);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int base = (i * 4 + wave) * 64, at = base + lane, r = at / KCH, c = (at % KCH) ^ k_swap(r);
-            const T *src = g.k + (size_t)__shfl(page, r, WAVE) * g.step + (size_t)((t0 + r) & g.mask) * HD + c * RUN;
-            __builtin_amdgcn_global_load_lds((const void *)src, (lds_ptr)(kd + base), 16, 0, 0);
-        }
+            for (int i = 0; i < N; ++i) x[i] = *(const run4 *)(k + i * (THREADS * 16) + tid * 16);
+        } else {
+            const int page = page_or_0(id);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int base = (i * 4 + wave) * 64, at = base + lane, r = at / VCH, c = (at % VCH) ^ v_swap(r);
-            const T *src = g.v + (size_t)__shfl(page, c * RUN, WAVE) * g.step + ((size_t)r << p.page_log) +
-                           ((t0 + c * RUN) & g.mask);
-            __builtin_amdgcn_global_load_lds((const void *)src, (lds_ptr)(vd + base), 16, 0, 0);
+            for (int i = 0; i < N; ++i) {
+                const uint32_t r = (THREADS * i + tid) / KCH, c = tid % KCH;
+                x[i] = *(const run4 *)(g.k + (size_t)__shfl(page, r, WAVE) * g.step +
+                                       (size_t)((t0 + r) & g.mask) * HD + c * RUN);
+            }
         }
     };
-    // V at positions that cannot be read may be anything: 0 in its place
-    const auto clean = [&](int step, unsigned long long valid) {
-        run4 *vd = lds[step & 1][1];
+    const auto load_v = [&](run4 (&x)[N], int step, int id) {
+        const int t0 = step * KT;
+        const uint32_t tid = fresh(threadIdx.x);
+        if (one_page) {
+            const int page = page_or_0(__builtin_amdgcn_readfirstlane(id));
+            const char *v = (const char *)(g.v + (size_t)page * g.step + (t0 & g.mask));
+            const uint32_t v_lane = (uint32_t)(((tid / VCH) << p.page_log) + (tid % VCH) * RUN) * (uint32_t)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                x[i] = *(const run4 *)(v + (size_t)i * ((THREADS / VCH * sizeof(T)) << p.page_log) + v_lane);
+        } else {
+            const int page = page_or_0(id);
+            const uint32_t c = tid % VCH;
+            const T *v = g.v + (size_t)__shfl(page, c * RUN, WAVE) * g.step + ((t0 + c * RUN) & g.mask);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = *(const run4 *)(v + ((size_t)((THREADS * i + tid) / VCH) << p.page_log));
+        }
+    };
+    // positions of a step that can be read
+    const auto readable = [&](int step, int id) {
+        return __ballot((unsigned)id < (unsigned)p.n_page && step * KT + (lane & (KT - 1)) < t.n_kv);
+    };
+    // the loaded runs into their buffer; V at positions that cannot be read may be anything: 0 in its place
+    const auto put_k = [&](const run4 (&x)[N], int step) {
+        run4 *to = lds[step & 1][0];
+        const uint32_t tid = fresh(threadIdx.x);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int at = (i * 4 + wave) * 64 + lane, c = (at % VCH) ^ v_swap(at / VCH);
-            vd[at] = keep_elements<E>(vd[at], (uint32_t)(valid >> (c * RUN)));
+            const uint32_t r = (THREADS * i + tid) / KCH;
+            to[r * KCH + ((tid % KCH) ^ k_swap(r))] = x[i];
+        }
+    };
+    const auto put_v = [&](run4 (&x)[N], int step, unsigned long long valid) {
+        run4 *to = lds[step & 1][1];
+        const uint32_t tid = fresh(threadIdx.x);
+        if (valid != ~0ull) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = keep_elements<E>(x[i], (uint32_t)(valid >> (tid % VCH * RUN)));
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t r = (THREADS * i + tid) / VCH;
+            to[r * VCH + ((tid % VCH) ^ v_swap(r))] = x[i];
         }
     };
 
-    bool careful = false;  // a V that only some of the wave's rows attend to is not finite
+    bool again = false;
     if (range.x < range.y) {
-        int now = entry(range.x), next = range.x + 1 < range.y ? entry(range.x + 1) : 0;
-        stage(range.x, now);
+        const int last = range.y - 1;
+        run4 kr[N], vr[N];
+        int next = entry(range.x);
+        load_k(kr, range.x, next);
+        load_v(vr, range.x, next);
+        unsigned long long valid = readable(range.x, next);
+        put_k(kr, range.x);
+        put_v(vr, range.x, valid);
+        next = entry(min(range.x + 1, last));
         for (int step = range.x; step < range.y; ++step) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            const int t0 = step * KT;
-            const unsigned long long valid = __ballot((unsigned)now < (unsigned)p.n_page && t0 + (lane & (KT - 1)) < t.n_kv);
-            if (valid != ~0ull) clean(step, valid);
             __syncthreads();  // the step's tile is there, and the other buffer is read
-            const int after = step + 2 < range.y ? entry(step + 2) : 0;
-            if (step + 1 < range.y) stage(step + 1, next);
-            now = next;
-            next = after;
-            if (t0 >= any) continue;
-            const run4 *kt = lds[step & 1][0], *vt = lds[step & 1][1];
-            v16f s[NQ][SUB];
-#pragma unroll
-            for (int b = 0; b < SUB; ++b) {
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[n][b][i] = 0.0f;
-                const int r = 32 * b + kv_row<E>(m);
-#pragma unroll
-                for (int c = 0; c < S::QS; ++c) {
-                    const run4 x = kt[r * KCH + ((2 * c + h) ^ k_swap(r))];
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) s[n][b] = Mma<E>::mul(x, q[n][c], s[n][b]);
-                }
+            const int t0 = step * KT;
+            if (step < last) {
+                load_k(kr, step + 1, next);
+                load_v(vr, step + 1, next);
             }
-            if (t0 + KT > all || valid != ~0ull) {
+            const int after = entry(min(step + 2, last));
+            if (t0 < any) {
+                const run4 *kt = lds[step & 1][0], *vt = lds[step & 1][1];
+                // this lane's first run of a K and V tile's block; the others by exchanging bits of its place
+                const uint32_t x = fresh(threadIdx.x);
+                const int h = x >> 5 & 1, m = x & 31;
+                const int k_first = kv_row<E>(m) * KCH + (h ^ k_swap(kv_row<E>(m))), v_first = m * VCH + (h ^ v_swap(m));
+                // (the wave that has products to issue goes first: the other one of its SIMD has exponentials, more often
+                // than not, and both pipes are busy; 8192 tokens 575 -> 568 us)
+                __builtin_amdgcn_s_setprio(1);
+                v16f s[SUB];
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
+                for (int b = 0; b < SUB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < S::QS; ++c)
+#pragma unroll
+                    for (int b = 0; b < SUB; ++b) s[b] = Mma<E>::mul(kt[32 * b * KCH + (k_first ^ (2 * c))], q[c], s[b]);
+                order_reads<E, SUB * S::QS>();
+                __builtin_amdgcn_s_setprio(0);
+                if (t0 + KT > all || valid != ~0ull) {
+                    // a position that a row does not attend to weighs nothing, whatever lies there; but nothing times an
+                    // infinity or NaN is NaN: where V has one, these rows are done again (attend_again)
 #pragma unroll
                     for (int b = 0; b < SUB; ++b)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int at = 32 * b + kv_reg<E>(i, h);
-                            s[n][b][i] = t0 + at < row[n].limit && (valid >> at & 1) ? s[n][b][i] : NEG_INF;
+                            s[b][i] = t0 + at < row.limit && (valid >> at & 1) ? s[b][i] : NEG_INF;
                         }
-                uint32_t bad = 0;
+                    uint32_t bad = 0;
 #pragma unroll 4
-                for (int i = 0; i < KT * KCH / 64; ++i) bad |= not_finite<E>(vt[i * 64 + lane]);
-                careful |= __any(bad != 0);
-            }
-            run4 w[NQ][SUB * S::PS];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                st[n].template softmax<SUB>(s[n], a.scale);
-#pragma unroll
-                for (int c = 0; c < SUB * S::PS; ++c) w[n][c] = S::weights(s[n][c / S::PS], c % S::PS);
-            }
-#pragma unroll
-            for (int c = 0; c < SUB * S::PS; ++c)
-#pragma unroll
-                for (int d = 0; d < S::DB; ++d) {
-                    const int r = 32 * d + m;
-                    const run4 x = vt[r * VCH + ((2 * c + h) ^ v_swap(r))];
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) st[n].o[d] = Mma<E>::mul(x, w[n][c], st[n].o[d]);
+                    for (int i = 0; i < KT * KCH / 64; ++i) bad |= not_finite<E>(vt[i * 64 + (x & 63)]);
+                    again |= __any(bad != 0);
                 }
+                st.template softmax<SUB>(s, a.scale);
+#pragma unroll
+                for (int c = 0; c < SUB * S::PS; ++c) {
+                    const run4 w = S::weights(s[c / S::PS], c % S::PS);
+#pragma unroll
+                    for (int d = 0; d < S::DB; ++d)
+                        st.o[d] = Mma<E>::mul(vt[32 * d * VCH + (v_first ^ (2 * c))], w, st.o[d]);
+                }
+                order_reads<E, SUB * S::PS * S::DB>();
+            }
+            if (step < last) {
+                valid = readable(step + 1, next);
+                put_k(kr, step + 1);
+                put_v(vr, step + 1, valid);
+                next = after;
+            }
         }
     }
-    const auto finish = [&](S &x, const Row &r, int n) {
-        const float l = x.l + other_half(x.l);
-        if (PREFIX || parts > 1) {
-            write_part<E, HD>(sp, ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y) * (4 * NQ) + NQ * wave + n, x, l);
-        } else {
-            const float f = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-            for (int d = 0; d < S::DB; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x.o[d][i] *= f;
-            if (r.at >= 0) x.write(a.out, a.out_f32, (size_t)r.at);
-        }
-    };
-    if (!careful) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) finish(st[n], row[n], n);
+    const size_t slot = ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y) * W + wave;
+    if (again) {
+        Again x;
+        x.p = p;
+        x.sp = sp;
+        x.t = t;
+        x.kvh = kvh;
+        x.begin = range.x * KT;
+        x.end = min(range.y * KT, any);
+        x.q = a.q;
+        x.out = PREFIX || parts > 1 ? nullptr : a.out;
+        x.out_f32 = a.out_f32;
+        x.scale = a.scale;
+        x.slot = slot;
+        attend_again<E, HD>(x, row.limit, row.at);
         return;
     }
-    // a weight of 0 times an infinity or NaN has spoilt rows that do not attend to it: these rows once more, each such
-    // value added where it belongs
-#pragma unroll 1
-    for (int n = 0; n < NQ; ++n) {
-        Row r = row[0];
-        if constexpr (NQ == 2) r = n ? row[1] : r;
-        load_rows<E, HD>(q[0], a.q, r.at);
-        S x;
-        x.clear();
-        attend_pages<E, HD, 32>(p, g, t, r.limit, range.x * KT, min(range.y * KT, any), q[0], a.scale, x);
-        finish(x, r, n);
-    }
+    const float l = add_halves(st.l);
+    if (PREFIX || parts > 1) write_part<E, HD>(sp, slot, st, l);
+    else write_rows<E, HD>(a.out, a.out_f32, row.at, st, l);
 }
 
 // ---- up to 32 rows ---------------------------------------------------------------
@@ -488,7 +578,7 @@ __global__ __launch_bounds__(256) void paged_rows(PagedAttendArgs a, Split sp) {
     attend_pages<E, HD, ROWS_STEP>(p, pages_of<E, HD>(p, t.seq, kvh), t, r.limit, begin + 32 * wave, end, q, a.scale, st);
 
     // the four waves' positions together
-    st.l += other_half(st.l);
+    st.l = add_halves(st.l);
     if (h == 0) {
         stats[0][wave][lane] = st.m;
         stats[1][wave][lane] = st.l;
@@ -665,22 +755,19 @@ bool room(Split &sp, size_t slots, int hd) {
 
 int queued() { return hipGetLastError() == hipSuccess ? 0 : -1; }
 
-// A 16-bit cache's long tiles have two blocks of 32 rows per wave; f32 products are bound by the matrix cores either way.
-template <class E, int HD> constexpr int wide() { return E::RUN == 8 && HD <= 128 ? 2 : 1; }
-
-template <class E, int HD, int NQ>
+template <class E, int HD, int W>
 int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
-    constexpr int R = 128 * NQ, KT = HD * sizeof(typename E::T) * 256 <= 131072 ? 64 : 32;
+    constexpr int R = 32 * W, KT = HD * sizeof(typename E::T) * 256 <= 131072 ? 64 : 32;
     const long long rows = (long long)p.n_tok * p.group, tiles = rows / R + p.n_seq;
-    const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * (3 - NQ);
+    const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
     const long long most = ((long long)p.max_page << p.page_log) / (KT * TILE_STEPS);
     Split sp{};
     sp.parts = (int)std::max(1LL, std::min({(want + busy - 1) / busy, most, 64LL}));
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 256) return -1;
     if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * (R / 32), HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
-    hipLaunchKernelGGL((paged_tiles<E, HD, NQ, false>), grid, dim3(256), 0, st, a, sp);
+    hipLaunchKernelGGL((paged_tiles<E, HD, W, false>), grid, dim3(64 * W), 0, st, a, sp);
     if (sp.parts > 1)
         hipLaunchKernelGGL((paged_join<E, HD, R>), dim3(grid.x, R / 32), dim3(256), 0, st, a, sp);
     return queued();
@@ -706,14 +793,13 @@ template <class E, int HD>
 int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
     const long long rows = (long long)a.p.n_tok * a.p.group / a.p.n_seq;  // of a sequence, on average
     if (rows <= 96) return prompt_rows<E, HD>(a, st);
-    if (rows >= 512) return prompt_tiles<E, HD, wide<E, HD>()>(a, st);
-    return prompt_tiles<E, HD, 1>(a, st);
+    return rows >= 1024 ? prompt_tiles<E, HD, 8>(a, st) : prompt_tiles<E, HD, 4>(a, st);
 }
 
-template <class E, int HD, int NQ>
+template <class E, int HD, int W>
 int decode_with(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
-    constexpr int R = 128 * NQ, KT = HD * sizeof(typename E::T) * 256 <= 131072 ? 64 : 32;
+    constexpr int R = 32 * W, KT = HD * sizeof(typename E::T) * 256 <= 131072 ? 64 : 32;
     const int per = (p.group + 31) / 32, cols = p.n_kv_head * per;
     const long long top = (long long)p.max_page << p.page_log;
     Split sp{};
@@ -725,7 +811,7 @@ int decode_with(const PagedAttendArgs &a, hipStream_t st) {
     if (a.n_groups) {
         const long long rows = (long long)p.n_seq * p.group;
         tiles = rows / R + a.n_groups;
-        const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * (3 - NQ);
+        const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
         sp.parts = (int)std::max(1LL, std::min({(want + busy - 1) / busy, top / (KT * TILE_STEPS), 64LL}));
         const long long slots = tiles * p.n_kv_head * sp.parts * (R / 32);
         if (slots > 0x7FFFFFFF / 256) return -1;
@@ -735,7 +821,7 @@ int decode_with(const PagedAttendArgs &a, hipStream_t st) {
     const bool join = a.n_groups || top > ROWS_STEP;
     if (join && !room(sp, sp.prefix_slots + (size_t)items * cols, HD)) return -1;
     if (a.n_groups)
-        hipLaunchKernelGGL((paged_tiles<E, HD, NQ, true>), dim3((unsigned)(tiles * p.n_kv_head), sp.parts), dim3(256),
+        hipLaunchKernelGGL((paged_tiles<E, HD, W, true>), dim3((unsigned)(tiles * p.n_kv_head), sp.parts), dim3(64 * W),
                            0, st, a, sp);
     hipLaunchKernelGGL((paged_rows<E, HD, true>), dim3((unsigned)items, cols), dim3(256), 0, st, a, sp);
     if (join) hipLaunchKernelGGL((paged_join_decode<E, HD, R>), dim3(p.n_seq, cols), dim3(256), 0, st, a, sp);
@@ -745,7 +831,7 @@ int decode_with(const PagedAttendArgs &a, hipStream_t st) {
 template <class E, int HD>
 int decode_as(const PagedAttendArgs &a, hipStream_t st) {
     const long long rows = a.n_groups ? (long long)a.p.n_seq * a.p.group / a.n_groups : 0;  // of a group, on average
-    return rows >= 256 ? decode_with<E, HD, wide<E, HD>()>(a, st) : decode_with<E, HD, 1>(a, st);
+    return rows >= 1024 ? decode_with<E, HD, 8>(a, st) : decode_with<E, HD, 4>(a, st);
 }
 
 template <class E>

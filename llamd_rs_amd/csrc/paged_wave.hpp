@@ -55,7 +55,22 @@ template <class E> __device__ __forceinline__ void put4(void *out, size_t at, fl
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, WAVE); }
+// The maximum (sum) of a lane's value and that of its other half.
+struct Halves {
+    float lo, hi;
+};
+__device__ __forceinline__ Halves halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ float max_halves(float x) {
+    const Halves v = halves(x);
+    return fmaxf(v.lo, v.hi);
+}
+__device__ __forceinline__ float add_halves(float x) {
+    const Halves v = halves(x);
+    return v.lo + v.hi;
+}
 
 // The maximum that x is taken against: an empty row's is 0, so that its terms are exp2(-inf) = 0 and not NaN.
 __device__ __forceinline__ float against(float m) { return m == NEG_INF ? 0.0f : m; }
@@ -132,14 +147,14 @@ template <class E, int HD> struct RowState {
         l = 0.0f;
     }
 
-    // Scores (kv_reg's order) to weights, the statistics and O's scale brought up to date.
-    template <int SUB> __device__ __forceinline__ void softmax(v16f (&s)[SUB], float scale) {
+    // The running maximum brought up to date with scores, and O and l with it.
+    template <int SUB> __device__ __forceinline__ void raise(const v16f (&s)[SUB], float scale) {
         float top = s[0][0];
 #pragma unroll
         for (int b = 0; b < SUB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-        top = fmaxf(top, other_half(top)) * scale;
+        top = max_halves(top) * scale;
         if (__any(top > m + LAZY)) {
             const float m1 = fmaxf(m, top), shrink = exp2_fast(m - against(m1));
             m = m1;
@@ -149,6 +164,10 @@ template <class E, int HD> struct RowState {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
         }
+    }
+
+    // Scores (kv_reg's order) to weights, added to l.
+    template <int SUB> __device__ __forceinline__ void weigh(v16f (&s)[SUB], float scale) {
         const float ref = against(m);
         float sum = 0.0f;
 #pragma unroll
@@ -159,6 +178,11 @@ template <class E, int HD> struct RowState {
                 sum += s[b][i];
             }
         l += sum;
+    }
+
+    template <int SUB> __device__ __forceinline__ void softmax(v16f (&s)[SUB], float scale) {
+        raise<SUB>(s, scale);
+        weigh<SUB>(s, scale);
     }
 
     // The right operand of step c of the second product.
