@@ -39,6 +39,8 @@ int describe(const char *what, const llamd_hip_pages *c, const llamd_hip_batch *
         return set_error("%s: n_head %d, n_head_kv %d", what, n_head, c->n_head_kv);
     if (b->n_seq < 0 || b->n_tok < 0 || b->max_page <= 0)
         return set_error("%s: n_seq %d, n_tok %d, max_page %d", what, b->n_seq, b->n_tok, b->max_page);
+    if ((long long)b->max_page * c->page > 1 << 30)
+        return set_error("%s: tables of %d pages of %d (2^30 positions at most)", what, b->max_page, c->page);
     if (b->n_seq && (!b->len || !b->table)) return set_error("%s: null lengths or table", what);
     if (!b->start && b->n_tok < b->n_seq)
         return set_error("%s: %d tokens for %d sequences of one token", what, b->n_tok, b->n_seq);

@@ -7,10 +7,10 @@
 // takes consecutive ones: with 8 query heads per kv head, a tile of 256 rows is 32 tokens, whose keys and values are
 // read once for all 8.
 //
-// Two kernels form O. paged_tiles: many rows; the waves of a workgroup have rows of their own and share K and V tiles in
-// LDS. paged_rows: up to 32 rows; the waves share the rows and have positions of their own, read straight into the
+// Two kernels form O. paged_tiles: many rows; the waves of a workgroup have 32 rows of their own each and share K and V
+// tiles in LDS. paged_few: up to 16 rows; the waves share the rows and have positions of their own, read straight into the
 // matrix operands. Either may have a part of a row's positions only; then O (unnormalised), the maximum and the sum
-// go to scratch and paged_join puts the parts together.
+// go to scratch and paged_join or paged_join_decode puts the parts together.
 #pragma once
 
 #include <algorithm>
@@ -22,57 +22,90 @@
 namespace llamd {
 namespace {
 
-// What prompt and decode calls of this batch are split into (host), and where parts lie.
+// Parts of rows: a slot has the statistics (maximum, sum) of `rows` rows and their O, four dimensions at a time:
+// o[slot][HD / 4][rows].
+struct Parts {
+    float4 *o;
+    float2 *ml;
+    int rows;
+};
+
+// How a call is split (host).
 struct Split {
-    float4 *part_o;   // [slot][HD / 8][64] a 32-row block's O: 4 dimensions of a row per lane
-    float2 *part_ml;  // [slot][32] maximum and sum
-    int parts;        // most parts of a row tile (prompt, prefix)
-    int prefix_slots; // decode: slots [0, prefix_slots) are the prefix's
-    int target;       // decode: workgroups wanted per kv head and block of 32 heads
+    Parts many, few;     // of paged_tiles (blocks of 32 rows) and of paged_few
+    int parts;           // most parts of a row tile (prompt, prefix)
+    double per_item;     // decode: 1 / (positions' steps per workgroup wanted)
 };
 
 // ---- rows ------------------------------------------------------------------------
 
-// A tile's rows, and this lane's of them.
+// What a tile of rows belongs to.
 struct Tile {
     int seq;              // the sequence whose table is read
     int n_kv;             // its positions that can be read
     int top;              // positions that the tile's last row attends to
+    int first, end, len;  // prompt: the sequence's tokens and length; prefix: the group's sequences
+    int rows;             // rows in the tile
 };
+// A row of it.
 struct Row {
     long long at;         // token * n_head + head, -1: no row
     int limit;            // positions that it attends to
 };
 
-// Tile number `tile` (R rows) of a prompt batch; false past the last. rows_end: rows in it.
+// Positions of a sequence of length n that the table can hold.
+__device__ __forceinline__ int readable_of(const PagedArgs &p, int n) {
+    return (int)min((long long)max(n, 0), min((long long)p.max_page << p.page_log, 0x7FFFFFFFLL));
+}
+
+// Tile number `tile` (R rows) of a prompt batch; it becomes its number within its sequence. False past the last. Every
+// sequence's numbers come with the first loads: the search costs one trip to memory per 64 sequences.
 template <int R>
-__device__ __forceinline__ bool prompt_tile(const PagedArgs &p, int &tile, Tile &t, int &rows_end, TokenSpan &span) {
-    t.seq = find_sequence(p.n_seq, tile, [&](int s) {
-        const TokenSpan x = token_span(p, s);
-        return (int)(((long long)(x.end - x.first) * p.group + R - 1) / R);
-    });
-    if (t.seq < 0) return false;
-    span = token_span(p, t.seq);
-    rows_end = (int)min((long long)(span.end - span.first) * p.group - (long long)R * tile, (long long)R);
-    t.n_kv = held(p, t.seq);
-    const int last = span.first + (int)(((long long)R * tile + rows_end - 1) / p.group);
-    t.top = max(min(p.len[t.seq] - (span.end - last) + 1, t.n_kv), 0);
-    return true;
+__device__ __forceinline__ bool prompt_tile(const PagedArgs &p, int &tile, Tile &t) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < p.n_seq; s0 += WAVE) {
+        const int s = s0 + lane;
+        int units = 0, first = s, end = s + 1, len = 0;
+        if (s < p.n_seq) {
+            len = p.len[s];
+            if (p.start) {
+                first = min(max(p.start[s], 0), p.n_tok);
+                end = max(min(p.start[s + 1], p.n_tok), first);
+            }
+            units = (int)(((long long)(end - first) * p.group + R - 1) / R);
+        }
+        const int sum = wave_incl_sum_i(units);
+        const unsigned long long past = __ballot(sum > tile);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            tile -= __builtin_amdgcn_readlane(sum - units, l);
+            t.seq = s0 + l;
+            t.first = __builtin_amdgcn_readlane(first, l);
+            t.end = __builtin_amdgcn_readlane(end, l);
+            t.len = __builtin_amdgcn_readlane(len, l);
+            t.rows = (int)min((long long)(t.end - t.first) * p.group - (long long)R * tile, (long long)R);
+            t.n_kv = readable_of(p, t.len);
+            const int last = t.first + (int)(((long long)R * tile + t.rows - 1) / p.group);
+            t.top = max(min(t.len - (t.end - last) + 1, t.n_kv), 0);
+            return true;
+        }
+        tile -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
 }
 
 // Row i of it (the last one for rows that it has not).
 template <int R>
-__device__ __forceinline__ Row prompt_row(const PagedArgs &p, int tile, const Tile &t, int rows_end, TokenSpan span, int kvh,
-                                          int i) {
-    const long long at = (long long)R * tile + min(i, rows_end - 1);
-    const int tok = span.first + (int)(at / p.group), head = (int)(at % p.group);
+__device__ __forceinline__ Row prompt_row(const PagedArgs &p, int tile, const Tile &t, int kvh, int i) {
+    const uint32_t at = (uint32_t)R * tile + min(i, t.rows - 1);
+    const uint32_t tok = at / (uint32_t)p.group, head = at - tok * p.group;
     Row r;
-    r.limit = max(min(p.len[t.seq] - (span.end - tok) + 1, t.n_kv), 0);
-    r.at = i < rows_end ? (long long)tok * p.n_head + kvh * p.group + head : -1;
+    r.limit = max(min(t.len - (t.end - t.first) + (int)tok + 1, t.n_kv), 0);
+    r.at = i < t.rows ? (long long)(t.first + tok) * p.n_head + kvh * p.group + head : -1;
     return r;
 }
 
-// The group of a sequence: its members [first, end) and the positions that they share (whole pages); none shared where a
+// A group of sequences: its members [first, end) and the positions that they share (whole pages); none shared where a
 // group has no two members.
 struct Group {
     int first, end, shared;
@@ -84,48 +117,51 @@ __device__ __forceinline__ Group group_at(const PagedAttendArgs &a, int g) {
     x.shared = x.end - x.first < 2 ? 0 : max(a.shared[g], 0) & ~((1 << a.p.page_log) - 1);
     return x;
 }
-__device__ __forceinline__ Group group_of(const PagedAttendArgs &a, int s, int *number = nullptr) {
+// The group of a sequence, by itself if it is in none.
+__device__ __forceinline__ Group group_of(const PagedAttendArgs &a, int s, int &number) {
+    Group x = {s, s + 1, 0};
+    if (a.n_groups <= 8) {
+        for (int g = 0; g < a.n_groups; ++g) {
+            const Group y = group_at(a, g);
+            if (s >= y.first && s < y.end) x = y, number = g;
+        }
+        return x;
+    }
     int lo = 0, hi = a.n_groups;  // the last group that begins at or before s
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (a.group_at[mid] <= s) lo = mid + 1;
         else hi = mid;
     }
-    Group x = {s, s + 1, 0};
     if (lo) {
         const Group y = group_at(a, lo - 1);
-        if (s >= y.first && s < y.end) {
-            x = y;
-            if (number) *number = lo - 1;
-        }
+        if (s >= y.first && s < y.end) x = y, number = lo - 1;
     }
     return x;
 }
 
 // Tile number `tile` of the rows of all groups that share something.
-template <int R>
-__device__ __forceinline__ int prefix_units(const PagedAttendArgs &a, int g) {
-    const Group x = group_at(a, g);
+template <int R> __device__ __forceinline__ int prefix_units(const PagedAttendArgs &a, const Group &x) {
     return x.shared ? (int)(((long long)(x.end - x.first) * a.p.group + R - 1) / R) : 0;
 }
 template <int R>
-__device__ __forceinline__ bool prefix_tile(const PagedAttendArgs &a, int &tile, Tile &t, int &rows_end, Group &g) {
-    const int n = find_sequence(a.n_groups, tile, [&](int i) { return prefix_units<R>(a, i); });
+__device__ __forceinline__ bool prefix_tile(const PagedAttendArgs &a, int &tile, Tile &t) {
+    const int n = find_sequence(a.n_groups, tile, [&](int i) { return prefix_units<R>(a, group_at(a, i)); });
     if (n < 0) return false;
-    g = group_at(a, n);
-    rows_end = (int)min((long long)(g.end - g.first) * a.p.group - (long long)R * tile, (long long)R);
-    t.seq = g.first;
-    t.n_kv = t.top = (int)min((long long)g.shared, (long long)a.p.max_page << a.p.page_log);
+    const Group g = group_at(a, n);
+    t.seq = t.first = g.first;
+    t.end = g.end;
+    t.rows = (int)min((long long)(g.end - g.first) * a.p.group - (long long)R * tile, (long long)R);
+    t.n_kv = t.top = readable_of(a.p, g.shared);
     return true;
 }
 template <int R>
-__device__ __forceinline__ Row prefix_row(const PagedAttendArgs &a, int tile, const Tile &t, int rows_end, const Group &g,
-                                          int kvh, int i) {
-    const long long at = (long long)R * tile + min(i, rows_end - 1);
-    const int seq = g.first + (int)(at / a.p.group), head = (int)(at % a.p.group);
+__device__ __forceinline__ Row prefix_row(const PagedAttendArgs &a, int tile, const Tile &t, int kvh, int i) {
+    const uint32_t at = (uint32_t)R * tile + min(i, t.rows - 1);
+    const uint32_t seq = t.first + at / (uint32_t)a.p.group, head = at % (uint32_t)a.p.group;
     Row r;
-    r.limit = min(held(a.p, seq), t.n_kv);
-    r.at = i < rows_end ? (long long)seq * a.p.n_head + kvh * a.p.group + head : -1;
+    r.limit = min(readable_of(a.p, a.p.len[seq]), t.n_kv);
+    r.at = i < t.rows ? (long long)seq * a.p.n_head + kvh * a.p.group + head : -1;
     return r;
 }
 
@@ -138,20 +174,6 @@ __device__ __forceinline__ int parts_of(int steps, int most, int least) {
 __device__ __forceinline__ int2 part_steps(int steps, int parts, int z) {
     return make_int2((int)((long long)steps * z / parts), (int)((long long)steps * (z + 1) / parts));
 }
-
-template <class E, int HD>
-__device__ __forceinline__ void write_part(const Split &sp, size_t slot, const RowState<E, HD> &st, float l) {
-    const int lane = threadIdx.x & 63;
-    float4 *o = sp.part_o + slot * (HD / 8 * 64) + lane;
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            o[(d * 4 + i / 4) * 64] = make_float4(st.o[d][i], st.o[d][i + 1], st.o[d][i + 2], st.o[d][i + 3]);
-    if (lane < 32) sp.part_ml[slot * 32 + lane] = make_float2(st.m, l);
-}
-
-// ---- one wave, straight from the pages -----------------------------------------------
 
 // Where a kv head's pages are.
 template <class E> struct Pages {
@@ -167,66 +189,254 @@ __device__ __forceinline__ Pages<E> pages_of(const PagedArgs &p, int seq, int kv
             (size_t)p.n_kv_head * HD << p.page_log, (1 << p.page_log) - 1};
 }
 
-template <class E, int HD>
-__device__ __forceinline__ void load_rows(run4 (&q)[HD / (2 * E::RUN)], const void *from, long long at) {
-    const typename E::T *x = (const typename E::T *)from + (size_t)max(at, 0LL) * HD;
-    const int h = (threadIdx.x >> 5) & 1;
-#pragma unroll
-    for (int c = 0; c < HD / (2 * E::RUN); ++c) q[c] = *(const run4 *)(x + (2 * c + h) * E::RUN);
+__device__ __forceinline__ float over(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+template <class E> __device__ __forceinline__ void put_out(void *out, bool f32, size_t at, float4 x) {
+    if (f32) put4<ElemF32>(out, at, x);
+    else put4<E>(out, at, x);
 }
 
-// 32 rows against the positions t0 .. t0 + 31 of every STRIDE from `begin` to `end` (a multiple of 32 from begin, or
-// all that the rows attend to).
+// ---- up to 16 rows -----------------------------------------------------------------
+
+// A row's runs for the first product of 16 rows.
+template <class E, int HD>
+__device__ __forceinline__ void load_few(run4 (&q)[HD / (4 * E::RUN)], const void *from, long long at) {
+    const typename E::T *x = (const typename E::T *)from + (size_t)max(at, 0LL) * HD;
+    const int g = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int c = 0; c < HD / (4 * E::RUN); ++c) q[c] = *(const run4 *)(x + (4 * c + g) * E::RUN);
+}
+
+// 16 rows against the positions t0 .. t0 + 31 for t0 = begin, begin + STRIDE, ... below end; begin and STRIDE are multiples of
+// 32, uniform over the wave. K of a step (and V, where the registers allow) is loaded whole before the first product.
 template <class E, int HD, int STRIDE>
-__device__ __forceinline__ void attend_pages(const PagedArgs &p, const Pages<E> &g, const Tile &t, int limit, int begin,
-                                             int end, const run4 (&q)[HD / (2 * E::RUN)], float scale,
-                                             RowState<E, HD> &st) {
+__device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &pg, int n_kv, int limit, int begin, int end,
+                                           const run4 (&q)[HD / (4 * E::RUN)], float scale, FewState<E, HD> &st) {
     typedef typename E::T T;
-    typedef RowState<E, HD> S;
+    typedef FewState<E, HD> S;
     constexpr int RUN = E::RUN;
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+    constexpr bool EARLY = HD * sizeof(T) <= 512;
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    const int all = wave_reduce(limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
     for (int t0 = begin; t0 < end; t0 += STRIDE) {
-        const int pos = t0 + kv_row<E>(lane & 31), posc = min(pos, t.n_kv - 1);
-        const int page = page_of(p, g.table, posc);
-        // bit m: the position of the first product's row m can be read
-        const uint32_t valid = (uint32_t)__ballot(page >= 0 && pos < t.n_kv);
-        const T *k = g.k + (size_t)max(page, 0) * g.step + (size_t)(posc & g.mask) * HD;
-        v16f s[1];
+        // the pages of the two halves of the step
+        const int id0 = pg.table[min(t0, n_kv - 1) >> p.page_log], id1 = pg.table[min(t0 + 16, n_kv - 1) >> p.page_log];
+        const bool ok0 = (unsigned)id0 < (unsigned)p.n_page, ok1 = (unsigned)id1 < (unsigned)p.n_page;
+        const size_t at0 = (size_t)(ok0 ? id0 : 0) * pg.step, at1 = (size_t)(ok1 ? id1 : 0) * pg.step;
+        // bit i: position t0 + i can be read
+        uint32_t valid = (ok0 ? 0x0000FFFFu : 0u) | (ok1 ? 0xFFFF0000u : 0u);
+        if (n_kv - t0 < 32) valid &= (1u << (n_kv - t0)) - 1u;
+        run4 k[2][S::QS], v[S::PS][S::DB];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[0][i] = 0.0f;
+        for (int b = 0; b < 2; ++b) {
+            const int r = few_row<E>(b, m);
+            const T *x = pg.k + (r & 16 ? at1 : at0) + (size_t)((t0 + r) & pg.mask) * HD;
 #pragma unroll
-        for (int c = 0; c < S::QS; ++c) s[0] = Mma<E>::mul(*(const run4 *)(k + (2 * c + h) * RUN), q[c], s[0]);
-        const bool whole = __all(limit >= t0 + 32) && valid == 0xFFFFFFFFu;
+            for (int c = 0; c < S::QS; ++c) k[b][c] = *(const run4 *)(x + (4 * c + g) * RUN);
+        }
+        const auto load_v = [&]() {
+#pragma unroll
+            for (int c = 0; c < S::PS; ++c) {
+                const int r = (4 * c + g) * RUN;
+                const T *x = pg.v + (r & 16 ? at1 : at0) + ((size_t)m << p.page_log) + ((t0 + r) & pg.mask);
+#pragma unroll
+                for (int d = 0; d < S::DB; ++d) v[c][d] = *(const run4 *)(x + ((size_t)(16 * d) << p.page_log));
+            }
+        };
+        if constexpr (EARLY) load_v();
+        v4f s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < S::QS; ++c)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) s[b] = mul16<E>(k[b][c], q[c], s[b]);
+        if constexpr (!EARLY) load_v();
+        const bool whole = t0 + 32 <= all && valid == 0xFFFFFFFFu;
         if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const bool seen = t0 + kv_reg<E>(i, h) < limit && (valid >> (8 * (i >> 2) + (i & 3) + 4 * h) & 1);
-                s[0][i] = seen ? s[0][i] : NEG_INF;
-            }
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = few_reg<E>(b, i, g);
+                    s[b][i] = t0 + at < limit && (valid >> at & 1) ? s[b][i] : NEG_INF;
+                }
         }
-        st.template softmax<1>(s, scale);
+        st.softmax(s, scale);
 #pragma unroll
         for (int c = 0; c < S::PS; ++c) {
-            const run4 w = S::weights(s[0], c);
-            const int vp = t0 + RUN * (2 * c + h), vpc = min(vp, (t.n_kv - 1) & ~(RUN - 1));
-            const int page = page_of(p, g.table, vpc);
-            const T *v = g.v + (size_t)max(page, 0) * g.step + (vpc & g.mask);
-            const auto v_run = [&](int d) { return *(const run4 *)(v + ((size_t)(32 * d + (lane & 31)) << p.page_log)); };
+            const run4 w = S::weights(s, c);
             if (whole) {
 #pragma unroll
-                for (int d = 0; d < S::DB; ++d) st.o[d] = Mma<E>::mul(v_run(d), w, st.o[d]);
+                for (int d = 0; d < S::DB; ++d) st.o[d] = mul16<E>(v[c][d], w, st.o[d]);
             } else {
-                // positions that no row attends to may hold anything
-                const int n = page < 0 ? 0 : min(max(end - vp, 0), RUN);
-                st.add_masked(v_run, (1u << n) - 1u, w, t0 + 2 * RUN * c, limit);
+                st.add_masked([&](int d) { return v[c][d]; }, valid >> ((4 * c + g) * RUN), w, t0 + 4 * RUN * c, limit);
             }
         }
     }
 }
 
-// ---- many rows -------------------------------------------------------------------
+// Rows of a wave of paged_tiles (32, from `limit` and `at` of their lanes) once more, 16 at a time straight from the pages,
+// every infinity or NaN in V added only where it belongs. A function of its own: its registers would cost paged_tiles
+// some of the reads that it keeps in flight.
+template <class E, int HD>
+__device__ __attribute__((noinline)) void attend_again(const PagedAttendArgs *a, const Parts *parts, const Tile *t, int kvh,
+                                                       int begin, int end, size_t slot, int limit, long long at) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll 1
+    for (int b = 0; b < 2; ++b) {
+        const int from = 16 * b + (lane & 15), lim = __shfl(limit, from, WAVE);
+        const long long row = __shfl(at, from, WAVE);
+        run4 q[HD / (4 * E::RUN)];
+        load_few<E, HD>(q, a->q, row);
+        FewState<E, HD> st;
+        st.clear();
+        attend_few<E, HD, 32>(a->p, pages_of<E, HD>(a->p, t->seq, kvh), t->n_kv, lim, begin, end, q, a->scale, st);
+        const float l = add_groups(st.l), f = over(l);
+        if (parts) {
+            if (g == 0) parts->ml[slot * 32 + from] = make_float2(st.m, l);
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d)
+                parts->o[(slot * (HD / 4) + 4 * d + g) * 32 + from] = make_float4(st.o[d][0], st.o[d][1], st.o[d][2], st.o[d][3]);
+        } else if (row >= 0) {
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d)
+                put_out<E>(a->out, a->out_f32, (size_t)row * HD + 16 * d + 4 * g,
+                           make_float4(st.o[d][0] * f, st.o[d][1] * f, st.o[d][2] * f, st.o[d][3] * f));
+        }
+    }
+}
 
-typedef __attribute__((address_space(3))) void *lds_ptr;
+// Least positions of a part of paged_few: one step of each wave.
+constexpr int FEW_STEP = 128;
+
+// A sequence's own positions in a decode batch (behind those that its group shares), cut into parts.
+struct Own {
+    int n, shared;  // positions that can be read; of these the group's
+    __device__ __forceinline__ int tail() const { return max(n - shared, 0); }
+    // parts of `cut`; one at least where nothing is shared, so that an empty sequence's rows are written
+    __device__ __forceinline__ int units(int cut) const {
+        const int u = tail() ? (tail() - 1) / cut + 1 : 0;
+        return shared && n ? u : max(u, 1);
+    }
+};
+__device__ __forceinline__ Own own_of(const PagedAttendArgs &a, int s) {
+    Own x = {0, 0};
+    if (s >= a.p.n_seq) return x;
+    int number;
+    x.n = readable_of(a.p, a.p.len[s]);
+    if (a.n_groups) x.shared = group_of(a, s, number).shared;
+    return x;
+}
+// Positions per part, so that all parts together are about as many as the host wants: by the sum of the tails, which is
+// exact in f64. (2^31 - 128 at most: one part.)
+__device__ __forceinline__ int decode_cut(const PagedAttendArgs &a, const Split &sp) {
+    double sum = 0.0;
+    for (int s = threadIdx.x & 63; s < a.p.n_seq; s += WAVE) sum += (double)own_of(a, s).tail();
+    return (int)min(max(ceil(wave_sum_d(sum) * sp.per_item), 1.0) * FEW_STEP, 2147483520.0);
+}
+
+// DECODE: blockIdx.x a part of a sequence, blockIdx.y a kv head and block of 16 of its query heads. Otherwise blockIdx.x
+// a tile of 16 rows of a prompt batch and a kv head, blockIdx.y a part of its positions.
+template <class E, int HD, bool DECODE>
+__global__ __launch_bounds__(256) void paged_few(PagedAttendArgs a, Split sp) {
+    typedef FewState<E, HD> S;
+    __shared__ float2 stats[4][16];
+    __shared__ float part[4][HD / 4][64];
+    const PagedArgs &p = a.p;
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Tile t;
+    Row r;
+    int begin, end, parts, kvh;
+    size_t slot;
+    if constexpr (DECODE) {
+        const int cut = decode_cut(a, sp);
+        int unit = blockIdx.x;
+        Own own;
+        t.seq = -1;
+        for (int s0 = 0; s0 < p.n_seq; s0 += WAVE) {
+            const Own mine = own_of(a, s0 + lane);
+            const int units = s0 + lane < p.n_seq ? mine.units(cut) : 0, sum = wave_incl_sum_i(units);
+            const unsigned long long past = __ballot(sum > unit);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                unit -= __builtin_amdgcn_readlane(sum - units, l);
+                own.n = __builtin_amdgcn_readlane(mine.n, l);
+                own.shared = __builtin_amdgcn_readlane(mine.shared, l);
+                t.seq = s0 + l;
+                break;
+            }
+            unit -= __builtin_amdgcn_readlane(sum, 63);
+        }
+        if (t.seq < 0) return;
+        const int per = (p.group + 15) / 16, head = (blockIdx.y % per) * 16 + m;
+        kvh = blockIdx.y / per;
+        t.n_kv = r.limit = own.n;
+        r.at = head < p.group ? (long long)t.seq * p.n_head + kvh * p.group + head : -1;
+        begin = (int)min((long long)own.shared + (long long)unit * cut, 0x7FFFFFFFLL);
+        end = (int)min((long long)begin + cut, (long long)t.n_kv);
+        parts = own.shared && own.n ? 2 : own.units(cut);
+        slot = (size_t)blockIdx.x * gridDim.y + blockIdx.y;
+    } else {
+        kvh = blockIdx.x % p.n_kv_head;
+        const int unit = gridDim.x / p.n_kv_head - 1 - blockIdx.x / p.n_kv_head;
+        int tile = unit;
+        if (!prompt_tile<16>(p, tile, t)) return;
+        r = prompt_row<16>(p, tile, t, kvh, m);
+        const int steps = (t.top + FEW_STEP - 1) / FEW_STEP;
+        parts = parts_of(steps, sp.parts, 1);
+        if ((int)blockIdx.y >= parts) return;
+        const int2 range = part_steps(steps, parts, blockIdx.y);
+        begin = range.x * FEW_STEP;
+        end = min(range.y * FEW_STEP, t.top);
+        slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y;
+    }
+    run4 q[S::QS];
+    load_few<E, HD>(q, a.q, r.at);
+    S st;
+    st.clear();
+    attend_few<E, HD, FEW_STEP>(p, pages_of<E, HD>(p, t.seq, kvh), t.n_kv, r.limit, begin + 32 * wave, end, q, a.scale, st);
+
+    // the four waves' positions together: every wave adds a quarter of the dimensions
+    const float mine = add_groups(st.l);
+    if (g == 0) stats[wave][m] = make_float2(st.m, mine);
+#pragma unroll
+    for (int d = 0; d < S::DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[wave][d * 4 + i][lane] = st.o[d][i];
+    __syncthreads();
+    float top = NEG_INF, l = 0.0f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stats[w][m].x);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = exp2_fast(stats[w][m].x - against(top));
+        l = __builtin_fmaf(stats[w][m].y, f[w], l);
+    }
+    const float by = parts > 1 ? 1.0f : over(l);
+    if (parts > 1 && wave == 0 && g == 0 && m < sp.few.rows) sp.few.ml[slot * sp.few.rows + m] = make_float2(top, l);
+#pragma unroll
+    for (int j = 0; j < S::DB / 4; ++j) {
+        const int d = wave * (S::DB / 4) + j;
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x[i] = __builtin_fmaf(part[w][d * 4 + i][lane], f[w], x[i]);
+            x[i] *= by;
+        }
+        const float4 y = make_float4(x[0], x[1], x[2], x[3]);
+        if (parts > 1) {
+            if (m < sp.few.rows) sp.few.o[(slot * (HD / 4) + 4 * d + g) * sp.few.rows + m] = y;
+        } else if (r.at >= 0) {
+            put_out<E>(a.out, a.out_f32, (size_t)r.at * HD + 16 * d + 4 * g, y);
+        }
+    }
+}
+
+// ---- many rows -------------------------------------------------------------------
 
 // x, as something that the compiler cannot keep the results of between tiles: addresses are cheaper made again than held
 // in registers.
@@ -248,44 +458,11 @@ template <class E, int N> __device__ __forceinline__ void order_reads() {
     __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * MFMA, 0);
 }
 
-// Least steps of a part.
-constexpr int TILE_STEPS = 4;
-
-// O over the sum, to this lane's row (at < 0: none).
-template <class E, int HD>
-__device__ __forceinline__ void write_rows(void *out, bool f32, long long at, RowState<E, HD> &st, float l) {
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
-    if (at >= 0) st.write(out, f32, (size_t)at);
+// Positions per tile (two buffers of K and V in at most 128 KB), and least tiles of a part.
+template <class E, int HD> __host__ __device__ constexpr int tile_positions() {
+    return HD * sizeof(typename E::T) <= 512 ? 64 : 32;
 }
-
-// A wave's rows once more, straight from the pages, every infinity or NaN in V added only where it belongs. A function of
-// its own: its registers would cost paged_tiles some of the reads that it keeps in flight.
-struct Again {
-    PagedArgs p;
-    Split sp;
-    Tile t;
-    int kvh, begin, end;
-    const void *q;
-    void *out;  // null: a part, to `slot`
-    bool out_f32;
-    float scale;
-    size_t slot;
-};
-template <class E, int HD>
-__device__ __attribute__((noinline)) void attend_again(const Again &x, int limit, long long at) {
-    run4 q[HD / (2 * E::RUN)];
-    load_rows<E, HD>(q, x.q, at);
-    RowState<E, HD> st;
-    st.clear();
-    attend_pages<E, HD, 32>(x.p, pages_of<E, HD>(x.p, x.t.seq, x.kvh), x.t, limit, x.begin, x.end, q, x.scale, st);
-    const float l = add_halves(st.l);
-    if (x.out) write_rows<E, HD>(x.out, x.out_f32, at, st, l);
-    else write_part<E, HD>(x.sp, x.slot, st, l);
-}
+template <class E> __host__ __device__ constexpr int tile_least() { return E::RUN == 8 ? 4 : 1; }
 
 // W waves of 32 rows each.
 template <class E, int HD, int W, bool PREFIX>
@@ -293,7 +470,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
     typedef typename E::T T;
     typedef RowState<E, HD> S;
     constexpr int RUN = E::RUN, R = 32 * W, THREADS = 64 * W;
-    constexpr int KT = HD * sizeof(T) * 256 <= 131072 ? 64 : 32;  // positions per tile: two buffers of K and V in 128 KB
+    constexpr int KT = tile_positions<E, HD>();
     constexpr int SUB = KT / 32;
     constexpr int KCH = HD / RUN, VCH = KT / RUN;                 // 16-byte runs per row of a tile
     constexpr int N = KT * KCH / THREADS;                             // loads of each thread per K (V) tile
@@ -304,19 +481,17 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
 
     // the last tiles, which have the most positions, go first
     const int unit = gridDim.x / p.n_kv_head - 1 - blockIdx.x / p.n_kv_head, kvh = blockIdx.x % p.n_kv_head;
-    int tile = unit, rows_end;
+    int tile = unit;
     Tile t;
     Row row;
     if constexpr (PREFIX) {
-        Group g;
-        if (!prefix_tile<R>(a, tile, t, rows_end, g)) return;
-        row = prefix_row<R>(a, tile, t, rows_end, g, kvh, 32 * wave + m);
+        if (!prefix_tile<R>(a, tile, t)) return;
+        row = prefix_row<R>(a, tile, t, kvh, 32 * wave + m);
     } else {
-        TokenSpan span;
-        if (!prompt_tile<R>(p, tile, t, rows_end, span)) return;
-        row = prompt_row<R>(p, tile, t, rows_end, span, kvh, 32 * wave + m);
+        if (!prompt_tile<R>(p, tile, t)) return;
+        row = prompt_row<R>(p, tile, t, kvh, 32 * wave + m);
     }
-    const int steps = (t.top + KT - 1) / KT, parts = parts_of(steps, sp.parts, TILE_STEPS);
+    const int steps = (t.top + KT - 1) / KT, parts = parts_of(steps, sp.parts, tile_least<E>());
     if ((int)blockIdx.y >= parts) return;
     const int2 range = part_steps(steps, parts, blockIdx.y);
     // positions that all rows of this wave attend to, and that any does
@@ -324,7 +499,11 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
     const int any = wave_reduce(row.limit, 0, [](int x, int y) { return max(x, y); });
 
     run4 q[S::QS];
-    load_rows<E, HD>(q, a.q, row.at);
+    {
+        const T *x = (const T *)a.q + (size_t)max(row.at, 0LL) * HD;
+#pragma unroll
+        for (int c = 0; c < S::QS; ++c) q[c] = *(const run4 *)(x + (2 * c + (lane >> 5)) * RUN);
+    }
     S st;
     st.clear();
     const Pages<E> g = pages_of<E, HD>(p, t.seq, kvh);
@@ -478,352 +657,243 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
         }
     }
     const size_t slot = ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y) * W + wave;
+    const bool part = PREFIX || parts > 1;
     if (again) {
-        Again x;
-        x.p = p;
-        x.sp = sp;
-        x.t = t;
-        x.kvh = kvh;
-        x.begin = range.x * KT;
-        x.end = min(range.y * KT, any);
-        x.q = a.q;
-        x.out = PREFIX || parts > 1 ? nullptr : a.out;
-        x.out_f32 = a.out_f32;
-        x.scale = a.scale;
-        x.slot = slot;
-        attend_again<E, HD>(x, row.limit, row.at);
+        const PagedAttendArgs args = a;
+        attend_again<E, HD>(&args, part ? &sp.many : nullptr, &t, kvh, range.x * KT, min(range.y * KT, any), slot, row.limit,
+                            row.at);
         return;
     }
-    const float l = add_halves(st.l);
-    if (PREFIX || parts > 1) write_part<E, HD>(sp, slot, st, l);
-    else write_rows<E, HD>(a.out, a.out_f32, row.at, st, l);
-}
-
-// ---- up to 32 rows ---------------------------------------------------------------
-
-// Least positions of a part: one step of each wave.
-constexpr int ROWS_STEP = 128;
-
-// A decode batch's own positions (behind the shared ones): tail(s) of sequence s, cut into parts of `cut`.
-struct DecodePlan {
-    int cut;
-};
-__device__ __forceinline__ int tail_of(const PagedAttendArgs &a, int s) {
-    const int n = held(a.p, s);
-    return a.n_groups ? max(n - group_of(a, s).shared, 0) : n;
-}
-__device__ __forceinline__ DecodePlan decode_plan(const PagedAttendArgs &a, const Split &sp) {
-    const int lane = threadIdx.x & 63;
-    double sum = 0.0;  // exact: lengths are integers
-    for (int s = lane; s < a.p.n_seq; s += WAVE) sum += (double)tail_of(a, s);
-    sum = wave_sum_d(sum);
-    DecodePlan d;
-    // (at most 2^31 - 1 positions per sequence: a part of a whole sequence at the most)
-    d.cut = (int)min(max(ceil(sum / sp.target / ROWS_STEP), 1.0) * ROWS_STEP, 2147483520.0);
-    return d;
-}
-// Parts of sequence s: one at least where nothing is shared, so that an empty sequence's rows are written.
-__device__ __forceinline__ int decode_units(const PagedAttendArgs &a, const DecodePlan &d, int s) {
-    const int n = held(a.p, s), shared = a.n_groups ? group_of(a, s).shared : 0;
-    const int units = n > shared ? (n - shared - 1) / d.cut + 1 : 0;
-    return shared && n ? units : max(units, 1);
-}
-
-// DECODE: blockIdx.x a part of a sequence, blockIdx.y a kv head and block of 32 of its query heads. Otherwise blockIdx.x
-// a tile of 32 rows of a prompt batch and a kv head, blockIdx.y a part of its positions.
-template <class E, int HD, bool DECODE>
-__global__ __launch_bounds__(256) void paged_rows(PagedAttendArgs a, Split sp) {
-    typedef RowState<E, HD> S;
-    __shared__ float stats[2][4][32];
-    __shared__ __align__(16) float part[2][S::DB * 16][64];
-    const PagedArgs &p = a.p;
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-    Tile t;
-    Row r;
-    int begin, end, parts, kvh;
-    size_t slot;
-    if constexpr (DECODE) {
-        const DecodePlan plan = decode_plan(a, sp);
-        int unit = blockIdx.x;
-        t.seq = find_sequence(p.n_seq, unit, [&](int s) { return decode_units(a, plan, s); });
-        if (t.seq < 0) return;
-        const int per = (p.group + 31) / 32, head = (blockIdx.y % per) * 32 + (lane & 31);
-        kvh = blockIdx.y / per;
-        t.n_kv = r.limit = held(p, t.seq);
-        const int shared = a.n_groups ? group_of(a, t.seq).shared : 0;
-        r.at = head < p.group ? (long long)t.seq * p.n_head + kvh * p.group + head : -1;
-        begin = (int)min((long long)shared + (long long)unit * plan.cut, 0x7FFFFFFFLL);
-        end = (int)min((long long)begin + plan.cut, (long long)t.n_kv);
-        parts = shared && t.n_kv ? 2 : decode_units(a, plan, t.seq);
-        slot = sp.prefix_slots + (size_t)blockIdx.x * gridDim.y + blockIdx.y;
-    } else {
-        kvh = blockIdx.x % p.n_kv_head;
-        const int unit = gridDim.x / p.n_kv_head - 1 - blockIdx.x / p.n_kv_head;
-        int tile = unit, rows_end;
-        TokenSpan span;
-        if (!prompt_tile<32>(p, tile, t, rows_end, span)) return;
-        r = prompt_row<32>(p, tile, t, rows_end, span, kvh, lane & 31);
-        const int steps = (t.top + ROWS_STEP - 1) / ROWS_STEP;
-        parts = parts_of(steps, sp.parts, 1);
-        if ((int)blockIdx.y >= parts) return;
-        const int2 range = part_steps(steps, parts, blockIdx.y);
-        begin = range.x * ROWS_STEP;
-        end = min(range.y * ROWS_STEP, t.top);
-        slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y;
-    }
-    run4 q[S::QS];
-    load_rows<E, HD>(q, a.q, r.at);
-    S st;
-    st.clear();
-    attend_pages<E, HD, ROWS_STEP>(p, pages_of<E, HD>(p, t.seq, kvh), t, r.limit, begin + 32 * wave, end, q, a.scale, st);
-
-    // the four waves' positions together
-    st.l = add_halves(st.l);
-    if (h == 0) {
-        stats[0][wave][lane] = st.m;
-        stats[1][wave][lane] = st.l;
-    }
-    __syncthreads();
-    float m = NEG_INF, l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[0][w][lane & 31]);
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-        l = __builtin_fmaf(stats[1][w][lane & 31], exp2_fast(stats[0][w][lane & 31] - against(m)), l);
-    const float f = exp2_fast(st.m - against(m)) * (parts > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l);
+    const float l = add_halves(st.l), f = part ? 1.0f : over(l);
+    const int h = lane >> 5;
+    if (part && h == 0) sp.many.ml[slot * 32 + m] = make_float2(st.m, l);
 #pragma unroll
     for (int d = 0; d < S::DB; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
-#pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-            for (int d = 0; d < S::DB; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) part[wave - half][d * 16 + i][lane] = st.o[d][i];
+        for (int i = 0; i < 16; i += 4) {
+            const int four = 8 * d + i / 2 + h;  // dimensions 4 four ..
+            const float4 y = make_float4(st.o[d][i] * f, st.o[d][i + 1] * f, st.o[d][i + 2] * f, st.o[d][i + 3] * f);
+            if (part) sp.many.o[(slot * (HD / 4) + four) * 32 + m] = y;
+            else if (row.at >= 0) put_out<E>(a.out, a.out_f32, (size_t)row.at * HD + 4 * four, y);
         }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int d = 0; d < S::DB; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) st.o[d][i] += part[wave][d * 16 + i][lane];
-        }
-        __syncthreads();
-    }
-    if (wave) return;
-    if (parts > 1) {
-        st.m = m;
-        write_part<E, HD>(sp, slot, st, l);
-    } else if (r.at >= 0) {
-        st.write(a.out, a.out_f32, (size_t)r.at);
-    }
 }
 
 // ---- the parts together ------------------------------------------------------------
 
-// Adds parts [0, n) of a 32-row block, slot(z) each, to the running maximum, sum and this wave's quarter of O; twice
-// over the statistics, once over O.
-template <int HD, class Slot>
-__device__ __forceinline__ float join_top(const Split &sp, int n, float top, Slot slot) {
-    for (int z = 0; z < n; ++z) top = fmaxf(top, sp.part_ml[slot(z) * 32 + (threadIdx.x & 31)].x);
-    return top;
-}
-template <int HD, class Slot>
-__device__ __forceinline__ void join_add(const Split &sp, int n, float top, float &l, float4 (&o)[HD / 32], Slot slot) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int z = 0; z < n; ++z) {
-        const float2 ml = sp.part_ml[slot(z) * 32 + (lane & 31)];
-        const float f = exp2_fast(ml.x - against(top));
-        l = __builtin_fmaf(ml.y, f, l);
-        const float4 *x = sp.part_o + slot(z) * (HD / 8 * 64) + lane;
+// Up to ROWS rows (of HD values) out of `n` parts: part z's statistics of row r are ml(z, r), its O of four dimensions
+// o(z, r, four). Every thread has its own parts' statistics, then its own pieces of O over all parts, whose loads depend on
+// nothing and overlap.
+constexpr int JOIN_MOST = 512;  // parts of a row at the most
+template <class E, int HD, int ROWS, class Ml, class O, class At>
+__device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, Ml ml, O o, At at) {
+    __shared__ float weight[JOIN_MOST * 16];
+    __shared__ float side[256 / ROWS][ROWS];
+    const int r = threadIdx.x % ROWS, k = threadIdx.x / ROWS;
+    constexpr int K = 256 / ROWS;
+    const bool here = r < rows;
+    float top = NEG_INF;
+    for (int z = k; z < n; z += K)
+        if (here) top = fmaxf(top, ml(z, r).x);
+    side[k][r] = top;
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-            const float4 y = x[(wave * (HD / 32) + i) * 64];
-            o[i].x = __builtin_fmaf(y.x, f, o[i].x);
-            o[i].y = __builtin_fmaf(y.y, f, o[i].y);
-            o[i].z = __builtin_fmaf(y.z, f, o[i].z);
-            o[i].w = __builtin_fmaf(y.w, f, o[i].w);
+    for (int i = 0; i < K; ++i) top = fmaxf(top, side[i][r]);
+    __syncthreads();
+    float l = 0.0f;
+    for (int z = k; z < n; z += K)
+        if (here) {
+            const float2 x = ml(z, r);
+            const float f = exp2_fast(x.x - against(top));
+            weight[z * ROWS + r] = f;
+            l = __builtin_fmaf(x.y, f, l);
         }
-    }
-}
-template <class E, int HD>
-__device__ __forceinline__ void join_write(const PagedAttendArgs &a, float l, const float4 (&o)[HD / 32], long long at) {
-    const int h = (threadIdx.x >> 5) & 1, wave = threadIdx.x >> 6;
-    if (at < 0) return;
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    side[k][r] = l;
+    __syncthreads();
+    l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-        const int q = wave * (HD / 32) + i;  // four dimensions 32 (q / 4) + 8 (q % 4) + 4 h
-        const size_t to = (size_t)at * HD + 32 * (q / 4) + 8 * (q % 4) + 4 * h;
-        const float4 x = make_float4(o[i].x * f, o[i].y * f, o[i].z * f, o[i].w * f);
-        if (a.out_f32) put4<ElemF32>(a.out, to, x);
-        else put4<E>(a.out, to, x);
+    for (int i = 0; i < K; ++i) l += side[i][r];
+    const float by = over(l);
+    const long long row = here ? at(r) : -1;
+    if (row < 0) return;
+    for (int four = k; four < HD / 4; four += K) {
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int z = 0; z < n; ++z) {
+            const float4 x = o(z, r, four);
+            const float f = weight[z * ROWS + r];
+            y.x = __builtin_fmaf(x.x, f, y.x);
+            y.y = __builtin_fmaf(x.y, f, y.y);
+            y.z = __builtin_fmaf(x.z, f, y.z);
+            y.w = __builtin_fmaf(x.w, f, y.w);
+        }
+        put_out<E>(a.out, a.out_f32, (size_t)row * HD + 4 * four, make_float4(y.x * by, y.y * by, y.z * by, y.w * by));
     }
 }
 
-// blockIdx.x: a tile of R rows and kv head of a prompt batch, blockIdx.y: 32 of its rows.
+// blockIdx.x: a tile of R rows and kv head of a prompt batch, blockIdx.y: 16 of its rows.
 template <class E, int HD, int R>
 __global__ __launch_bounds__(256) void paged_join(PagedAttendArgs a, Split sp) {
     const PagedArgs &p = a.p;
     const int unit = blockIdx.x / p.n_kv_head, kvh = blockIdx.x % p.n_kv_head;
-    constexpr int KT = R == 32 ? ROWS_STEP : HD * sizeof(typename E::T) * 256 <= 131072 ? 64 : 32;
-    int tile = unit, rows_end;
+    constexpr bool FEW = R == 16;
+    constexpr int STEP = FEW ? FEW_STEP : tile_positions<E, HD>();
+    int tile = unit;
     Tile t;
-    TokenSpan span;
-    if (!prompt_tile<R>(p, tile, t, rows_end, span)) return;
-    const int parts = parts_of((t.top + KT - 1) / KT, sp.parts, R == 32 ? 1 : TILE_STEPS);
-    if (parts < 2 || 32 * (int)blockIdx.y >= rows_end) return;
-    const Row r = prompt_row<R>(p, tile, t, rows_end, span, kvh, 32 * blockIdx.y + (threadIdx.x & 31));
-    const auto slot = [&](int z) {
-        return ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + z) * (R / 32) + blockIdx.y;
-    };
-    float l = 0.0f;
-    float4 o[HD / 32] = {};
-    join_add<HD>(sp, parts, join_top<HD>(sp, parts, NEG_INF, slot), l, o, slot);
-    join_write<E, HD>(a, l, o, r.at);
+    if (!prompt_tile<R>(p, tile, t)) return;
+    const int parts = parts_of((t.top + STEP - 1) / STEP, sp.parts, FEW ? 1 : tile_least<E>());
+    const int first = 16 * blockIdx.y;
+    if (parts < 2 || first >= t.rows) return;
+    const Parts x = FEW ? sp.few : sp.many;
+    const size_t slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts;
+    const int block = FEW ? 0 : first / 32, place = FEW ? 0 : first % 32;
+    const auto at = [&](int z) { return FEW ? slot + z : (slot + z) * (R / 32) + block; };
+    join<E, HD, 16>(
+        a, parts, min(t.rows - first, 16), [&](int z, int r) { return x.ml[at(z) * (FEW ? 16 : 32) + place + r]; },
+        [&](int z, int r, int four) { return x.o[(at(z) * (HD / 4) + four) * (FEW ? 16 : 32) + place + r]; },
+        [&](int r) { return prompt_row<R>(p, tile, t, kvh, first + r).at; });
 }
 
-// blockIdx.x: a sequence, blockIdx.y: a kv head and block of 32 of its query heads. R: rows of the prefix's tiles.
+// blockIdx.x: a sequence, blockIdx.y: a kv head and block of 16 of its query heads. R: rows of the prefix's tiles.
 template <class E, int HD, int R>
 __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Split sp) {
     const PagedArgs &p = a.p;
-    const int lane = threadIdx.x & 63, seq = blockIdx.x, per = (p.group + 31) / 32;
-    const int kvh = blockIdx.y / per, head = (blockIdx.y % per) * 32 + (lane & 31);
-    const DecodePlan plan = decode_plan(a, sp);
-    const int units = decode_units(a, plan, seq);
-    int number = 0;
-    const Group g = a.n_groups ? group_of(a, seq, &number) : Group{seq, seq + 1, 0};
-    const bool prefix = g.shared && held(p, seq);
+    const int lane = threadIdx.x & 63, seq = blockIdx.x, per = (p.group + 15) / 16;
+    const int kvh = blockIdx.y / per, head = (blockIdx.y % per) * 16;
+    const int cut = decode_cut(a, sp);
+    const Own own = own_of(a, seq);
+    const int units = own.units(cut);
+    const bool prefix = own.shared && own.n;
     if (!prefix && units < 2) return;
     int before = 0;  // parts of the sequences before this one
-    for (int s = lane; s < seq; s += WAVE) before += decode_units(a, plan, s);
+    for (int s = lane; s < seq; s += WAVE) before += own_of(a, s).units(cut);
     before = wave_reduce(before, 0, [](int x, int y) { return x + y; });
-    const auto slot = [&](int z) { return sp.prefix_slots + (size_t)(before + z) * gridDim.y + blockIdx.y; };
-    float top = join_top<HD>(sp, units, NEG_INF, slot), l = 0.0f;
-    float4 o[HD / 32] = {};
+    int parts = 0, base = 0;  // of the prefix, and the number of the group's first row among its 32-row blocks
+    long long first = 0;
     if (prefix) {
-        // this lane's row among the group's: its 32-row block and its place there, in the prefix's parts
-        int tiles = 0;
-        for (int i = lane; i < number; i += WAVE) tiles += prefix_units<R>(a, i);
-        tiles = wave_reduce(tiles, 0, [](int x, int y) { return x + y; });
-        const int n_kv = (int)min((long long)g.shared, (long long)p.max_page << p.page_log);
-        constexpr int KT = HD * sizeof(typename E::T) * 256 <= 131072 ? 64 : 32;
-        const int parts = parts_of((n_kv + KT - 1) / KT, sp.parts, TILE_STEPS);
-        const long long row = (long long)(seq - g.first) * p.group + min(head, p.group - 1);
-        const size_t unit = tiles + (size_t)(row / R);
-        const auto at = [&](int z) {
-            return ((unit * p.n_kv_head + kvh) * sp.parts + z) * (R / 32) + (size_t)(row % R) / 32;
-        };
-        const int place = (int)(row & 31), wave = threadIdx.x >> 6;
-        for (int z = 0; z < parts; ++z) top = fmaxf(top, sp.part_ml[at(z) * 32 + place].x);
-        for (int z = 0; z < parts; ++z) {
-            const float2 ml = sp.part_ml[at(z) * 32 + place];
-            const float f = exp2_fast(ml.x - against(top));
-            l = __builtin_fmaf(ml.y, f, l);
-            const float4 *x = sp.part_o + at(z) * (HD / 8 * 64) + (lane & 32) + place;
-#pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
-                const float4 y = x[(wave * (HD / 32) + i) * 64];
-                o[i].x = __builtin_fmaf(y.x, f, o[i].x);
-                o[i].y = __builtin_fmaf(y.y, f, o[i].y);
-                o[i].z = __builtin_fmaf(y.z, f, o[i].z);
-                o[i].w = __builtin_fmaf(y.w, f, o[i].w);
-            }
-        }
+        int number = 0, tiles = 0;
+        const Group g = group_of(a, seq, number);
+        for (int i = lane; i < number; i += WAVE) tiles += prefix_units<R>(a, group_at(a, i));
+        base = wave_reduce(tiles, 0, [](int x, int y) { return x + y; });
+        constexpr int KT = tile_positions<E, HD>();
+        parts = parts_of((readable_of(p, g.shared) + KT - 1) / KT, sp.parts, tile_least<E>());
+        first = (long long)(seq - g.first) * p.group + head;
     }
-    join_add<HD>(sp, units, top, l, o, slot);
-    join_write<E, HD>(a, l, o, head < p.group ? (long long)seq * p.n_head + kvh * p.group + head : -1);
+    const auto many = [&](int z, int r) {  // the slot of a row's 32-row block
+        const long long x = first + r;
+        return (((size_t)base + (size_t)(x / R)) * p.n_kv_head + kvh) * sp.parts * (R / 32) + (size_t)z * (R / 32) +
+               (size_t)(x % R) / 32;
+    };
+    const auto few = [&](int z) { return (size_t)(before + z - parts) * gridDim.y + blockIdx.y; };
+    const int w = sp.few.rows;
+    join<E, HD, 16>(
+        a, parts + units, min(p.group - head, 16),
+        [&](int z, int r) {
+            return z < parts ? sp.many.ml[many(z, r) * 32 + (first + r) % 32] : sp.few.ml[few(z) * w + r];
+        },
+        [&](int z, int r, int four) {
+            return z < parts ? sp.many.o[(many(z, r) * (HD / 4) + four) * 32 + (first + r) % 32]
+                             : sp.few.o[(few(z) * (HD / 4) + four) * w + r];
+        },
+        [&](int r) { return (long long)seq * p.n_head + kvh * p.group + head + r; });
 }
 
 // ---- launches ------------------------------------------------------------------------
 
 constexpr int CUS = 256;
 
-size_t slot_bytes(int hd) { return (size_t)hd * 128 + 256; }
-
-// Scratch for `slots` parts (null: none is needed, or none is to be had).
-bool room(Split &sp, size_t slots, int hd) {
-    if (!slots) return true;
-    char *p = (char *)lib_scratch(slots * slot_bytes(hd));
+// Scratch for slots of both kinds; false: none is to be had.
+bool room(Split &sp, size_t many, size_t few, int few_rows, int hd) {
+    const size_t o_many = many * hd * 32, o_few = few * hd * few_rows;  // floats
+    char *p = (char *)lib_scratch((o_many + o_few) * 4 + (many * 32 + few * few_rows) * 8);
     if (!p) return false;
-    sp.part_o = (float4 *)p;
-    sp.part_ml = (float2 *)(p + slots * (size_t)hd * 128);
+    sp.many.o = (float4 *)p;
+    sp.few.o = (float4 *)(p + o_many * 4);
+    sp.many.ml = (float2 *)(p + (o_many + o_few) * 4);
+    sp.few.ml = sp.many.ml + many * 32;
+    sp.many.rows = 32;
+    sp.few.rows = few_rows;
     return true;
 }
 
 int queued() { return hipGetLastError() == hipSuccess ? 0 : -1; }
 
+int fit(long long want, long long most, long long cap) { return (int)std::max(1LL, std::min({want, most, cap})); }
+
 template <class E, int HD, int W>
 int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
-    constexpr int R = 32 * W, KT = HD * sizeof(typename E::T) * 256 <= 131072 ? 64 : 32;
+    constexpr int R = 32 * W, KT = tile_positions<E, HD>();
     const long long rows = (long long)p.n_tok * p.group, tiles = rows / R + p.n_seq;
     const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
-    const long long most = ((long long)p.max_page << p.page_log) / (KT * TILE_STEPS);
+    const long long most = ((long long)p.max_page << p.page_log) / (KT * tile_least<E>());
     Split sp{};
-    sp.parts = (int)std::max(1LL, std::min({(want + busy - 1) / busy, most, 64LL}));
-    if (tiles * p.n_kv_head > 0x7FFFFFFF / 256) return -1;
-    if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * (R / 32), HD)) return -1;
+    sp.parts = fit((want + busy - 1) / busy, most, 64);
+    if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
+    if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * W, 0, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
     hipLaunchKernelGGL((paged_tiles<E, HD, W, false>), grid, dim3(64 * W), 0, st, a, sp);
-    if (sp.parts > 1)
-        hipLaunchKernelGGL((paged_join<E, HD, R>), dim3(grid.x, R / 32), dim3(256), 0, st, a, sp);
+    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, R>), dim3(grid.x, R / 16), dim3(256), 0, st, a, sp);
     return queued();
 }
 
 template <class E, int HD>
-int prompt_rows(const PagedAttendArgs &a, hipStream_t st) {
+int prompt_few(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
-    const long long rows = (long long)p.n_tok * p.group, tiles = rows / 32 + p.n_seq;
-    const long long busy = (rows + 31) / 32 * p.n_kv_head, want = 2 * CUS;
-    const long long most = ((long long)p.max_page << p.page_log) / ROWS_STEP;
+    const long long rows = (long long)p.n_tok * p.group, tiles = rows / 16 + p.n_seq;
+    const long long busy = (rows + 15) / 16 * p.n_kv_head, want = 2 * CUS;
+    const long long most = ((long long)p.max_page << p.page_log) / FEW_STEP;
     Split sp{};
-    sp.parts = (int)std::max(1LL, std::min({(want + busy - 1) / busy, most, 256LL}));
-    if (tiles * p.n_kv_head > 0x7FFFFFFF / 256) return -1;
-    if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts, HD)) return -1;
+    sp.parts = fit((want + busy - 1) / busy, most, 256);
+    if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
+    if (sp.parts > 1 && !room(sp, 0, (size_t)tiles * p.n_kv_head * sp.parts, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
-    hipLaunchKernelGGL((paged_rows<E, HD, false>), grid, dim3(256), 0, st, a, sp);
-    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, 32>), dim3(grid.x, 1), dim3(256), 0, st, a, sp);
+    hipLaunchKernelGGL((paged_few<E, HD, false>), grid, dim3(256), 0, st, a, sp);
+    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, 16>), dim3(grid.x), dim3(256), 0, st, a, sp);
     return queued();
 }
+
+// Whether eight waves' rows fit the registers of four SIMDs.
+template <class E, int HD> constexpr bool wide() { return HD * sizeof(typename E::T) <= 256; }
 
 template <class E, int HD>
 int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
-    const long long rows = (long long)a.p.n_tok * a.p.group / a.p.n_seq;  // of a sequence, on average
-    if (rows <= 96) return prompt_rows<E, HD>(a, st);
-    return rows >= 1024 ? prompt_tiles<E, HD, 8>(a, st) : prompt_tiles<E, HD, 4>(a, st);
+    const PagedArgs &p = a.p;
+    const long long total = (long long)p.n_tok * p.group, rows = total / p.n_seq;  // and of a sequence, on average
+    const long long top = (long long)p.max_page << p.page_log;
+    // few rows per sequence, or not enough of them to fill the GPU and short contexts: 16 rows at a time
+    if (rows <= 64 || (total * p.n_kv_head <= 64 * 128 && top <= 512)) return prompt_few<E, HD>(a, st);
+    if constexpr (wide<E, HD>())
+        if (rows >= 1024 && total * p.n_kv_head >= 512 * 256) return prompt_tiles<E, HD, 8>(a, st);
+    return prompt_tiles<E, HD, 4>(a, st);
 }
 
 template <class E, int HD, int W>
 int decode_with(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
-    constexpr int R = 32 * W, KT = HD * sizeof(typename E::T) * 256 <= 131072 ? 64 : 32;
-    const int per = (p.group + 31) / 32, cols = p.n_kv_head * per;
+    constexpr int R = 32 * W, KT = tile_positions<E, HD>();
+    const int per = (p.group + 15) / 16, cols = p.n_kv_head * per;
     const long long top = (long long)p.max_page << p.page_log;
     Split sp{};
-    // parts of the sequences' own positions: 4 workgroups per CU, one part per sequence at least
-    sp.target = std::max(1, 4 * CUS / cols);
-    const long long cut_min = ROWS_STEP, items =
-        std::min<long long>((long long)p.n_seq + sp.target, (long long)p.n_seq * ((top + cut_min - 1) / cut_min));
-    long long tiles = 0;
+    // parts of the sequences' own positions: 4 workgroups per CU, one part per sequence at least, JOIN_MOST of a row at most
+    const int target = std::min(std::max(1, 4 * CUS / cols), JOIN_MOST - 66);
+    sp.per_item = 1.0 / ((double)target * FEW_STEP);
+    const long long items = std::min<long long>((long long)p.n_seq + target + 1,
+                                                (long long)p.n_seq * ((top + FEW_STEP - 1) / FEW_STEP));
+    long long tiles = 0, slots = 0;
     if (a.n_groups) {
         const long long rows = (long long)p.n_seq * p.group;
         tiles = rows / R + a.n_groups;
         const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
-        sp.parts = (int)std::max(1LL, std::min({(want + busy - 1) / busy, top / (KT * TILE_STEPS), 64LL}));
-        const long long slots = tiles * p.n_kv_head * sp.parts * (R / 32);
-        if (slots > 0x7FFFFFFF / 256) return -1;
-        sp.prefix_slots = (int)slots;
+        sp.parts = fit((want + busy - 1) / busy, top / (KT * tile_least<E>()), 64);
+        slots = tiles * p.n_kv_head * sp.parts * W;
     }
-    if (items > 0x7FFFFFFF / 256 || cols > 65535) return -1;
-    const bool join = a.n_groups || top > ROWS_STEP;
-    if (join && !room(sp, sp.prefix_slots + (size_t)items * cols, HD)) return -1;
+    if (items > 0x7FFFFFFF / 512 || cols > 65535 || tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
+    const bool join = a.n_groups || top > FEW_STEP;
+    if (join && !room(sp, slots, (size_t)items * cols, std::min(p.group, 16), HD)) return -1;
     if (a.n_groups)
-        hipLaunchKernelGGL((paged_tiles<E, HD, W, true>), dim3((unsigned)(tiles * p.n_kv_head), sp.parts), dim3(64 * W),
-                           0, st, a, sp);
-    hipLaunchKernelGGL((paged_rows<E, HD, true>), dim3((unsigned)items, cols), dim3(256), 0, st, a, sp);
+        hipLaunchKernelGGL((paged_tiles<E, HD, W, true>), dim3((unsigned)(tiles * p.n_kv_head), sp.parts), dim3(64 * W), 0,
+                           st, a, sp);
+    hipLaunchKernelGGL((paged_few<E, HD, true>), dim3((unsigned)items, cols), dim3(256), 0, st, a, sp);
     if (join) hipLaunchKernelGGL((paged_join_decode<E, HD, R>), dim3(p.n_seq, cols), dim3(256), 0, st, a, sp);
     return queued();
 }
@@ -831,7 +901,9 @@ int decode_with(const PagedAttendArgs &a, hipStream_t st) {
 template <class E, int HD>
 int decode_as(const PagedAttendArgs &a, hipStream_t st) {
     const long long rows = a.n_groups ? (long long)a.p.n_seq * a.p.group / a.n_groups : 0;  // of a group, on average
-    return rows >= 1024 ? decode_with<E, HD, 8>(a, st) : decode_with<E, HD, 4>(a, st);
+    if constexpr (wide<E, HD>())
+        if (rows >= 1024) return decode_with<E, HD, 8>(a, st);
+    return decode_with<E, HD, 4>(a, st);
 }
 
 template <class E>

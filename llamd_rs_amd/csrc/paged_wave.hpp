@@ -1,5 +1,5 @@
-// paged_wave.hpp -- attention of one wave: 32 query rows that share a kv head against 32 cached positions at a time, with
-// the running maximum and sum of the softmax.
+// paged_wave.hpp -- attention of one wave: query rows that share a kv head against cached positions, with the running
+// maximum and sum of the softmax. First 32 rows at a time, then 16.
 //
 // A row is a query head of a token. The wave forms S^T = K Q^T and O^T += V^T P^T with 32x32 matrix instructions, so
 // that a lane holds values of one row (lane & 31) throughout: the maximum and the sum are the lane's own but for one
@@ -166,7 +166,7 @@ template <class E, int HD> struct RowState {
         }
     }
 
-    // Scores (kv_reg's order) to weights, added to l.
+    // Scores (kv_reg's order) to weights, which add to l.
     template <int SUB> __device__ __forceinline__ void weigh(v16f (&s)[SUB], float scale) {
         const float ref = against(m);
         float sum = 0.0f;
@@ -193,37 +193,6 @@ template <class E, int HD> struct RowState {
         return to_run<E>(x);
     }
 
-    // One step of the second product where some of V is not to be read as it stands: of the runs v(d) of the dimension
-    // blocks, the elements of `keep` are positions that a row attends to, the others may hold anything. An infinity or
-    // NaN at a position that only some rows attend to gives the others nothing, not 0 * inf: such elements are left
-    // out of the product and added one position at a time (pos0 + e) to the rows that see it.
-    template <class Load>
-    __device__ __forceinline__ void add_masked(Load v, uint32_t keep, run4 p, int pos0, int limit) {
-        const int h = (threadIdx.x >> 5) & 1;
-        uint32_t any = 0;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            const run4 x = keep_elements<E>(v(d), keep);
-            const uint32_t bad = not_finite<E>(x);
-            any |= bad;
-            o[d] = Mma<E>::mul(keep_elements<E>(x, ~bad), p, o[d]);
-        }
-        if (!__any(any != 0)) return;
-#pragma unroll 1
-        for (int e = 0; e < 2 * E::RUN; ++e) {
-            const uint32_t one = (e / E::RUN == h) ? 1u << (e % E::RUN) : 0u;
-            if (!__any((any & one) != 0)) continue;
-            const bool seen = pos0 + e < limit;
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const run4 x = keep_elements<E>(v(d), keep & one);
-                const v16f t = Mma<E>::mul(keep_elements<E>(x, not_finite<E>(x)), keep_elements<E>(p, one), o[d]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] = seen ? t[i] : o[d][i];
-            }
-        }
-    }
-
     // O to a row of HD values, of the type or f32.
     template <class W> __device__ __forceinline__ void write_as(void *out, size_t row) const {
         const int h = (threadIdx.x >> 5) & 1;
@@ -237,6 +206,123 @@ template <class E, int HD> struct RowState {
     __device__ __forceinline__ void write(void *out, bool f32, size_t row) const {
         if (f32) write_as<ElemF32>(out, row);
         else write_as<E>(out, row);
+    }
+};
+
+// ---- 16 rows ----------------------------------------------------------------------
+// The same for up to 16 rows and 32 positions with 16x16 matrix instructions, whose four groups of 16 lanes hold a run each:
+// a row's values lie in four lanes, and half the registers and columns are left unused.
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+template <class E> __device__ __forceinline__ v4f mul16(run4 a, run4 b, v4f c);
+template <> __device__ __forceinline__ v4f mul16<ElemF16>(run4 a, run4 b, v4f c) {
+    typedef Mma<ElemF16>::V V;
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ v4f mul16<ElemBF16>(run4 a, run4 b, v4f c) {
+    typedef Mma<ElemBF16>::V V;
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ v4f mul16<ElemF32>(run4 a, run4 b, v4f c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+}
+
+// The maximum (sum) over the four groups.
+__device__ __forceinline__ float max_groups(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float add_groups(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return add_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Position (0..31) of row m of block b of the first product's left operand, and of a lane's score register (b, i).
+template <class E> __device__ __forceinline__ int few_row(int b, int m) {
+    return E::RUN == 8 ? 8 * (m >> 2) + 4 * b + (m & 3) : 16 * b + m;
+}
+template <class E> __device__ __forceinline__ int few_reg(int b, int i, int g) {
+    return E::RUN == 8 ? 8 * g + 4 * b + i : 16 * b + 4 * g + i;
+}
+
+template <class E, int HD> struct FewState {
+    static constexpr int DB = HD / 16;            // blocks of 16 dimensions
+    static constexpr int QS = HD / (4 * E::RUN);  // steps of the first product
+    static constexpr int PS = 32 / (4 * E::RUN);  // steps of the second
+    v4f o[DB];   // dimension 16 d + 4 group + i
+    float m, l;  // what x is taken against, and this lane's part of the sum
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        m = NEG_INF;
+        l = 0.0f;
+    }
+
+    __device__ __forceinline__ void softmax(v4f (&s)[2], float scale) {
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][i]);
+        top = max_groups(top) * scale;
+        if (__any(top > m + LAZY)) {
+            const float m1 = fmaxf(m, top), shrink = exp2_fast(m - against(m1));
+            m = m1;
+            l *= shrink;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= shrink;
+        }
+        const float ref = against(m);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[b][i] = exp2_fast(__builtin_fmaf(s[b][i], scale, -ref));
+                l += s[b][i];
+            }
+    }
+
+    static __device__ __forceinline__ run4 weights(const v4f (&s)[2], int c) {
+        float x[E::RUN];
+#pragma unroll
+        for (int j = 0; j < E::RUN; ++j) x[j] = E::RUN == 8 ? s[j / 4][j % 4] : s[c][j % 4];
+        return to_run<E>(x);
+    }
+
+    // One step of the second product where some of V is not to be read as it stands: of the runs v(d) of the dimension
+    // blocks, the elements of `keep` can be read, the others may hold anything. An infinity or NaN at a position that
+    // only some rows attend to gives the others nothing, not 0 * inf: such elements are left out of the product and
+    // added one position at a time (pos0 + e) to the rows that see it.
+    template <class Load>
+    __device__ __forceinline__ void add_masked(Load v, uint32_t keep, run4 p, int pos0, int limit) {
+        const int g = (threadIdx.x >> 4) & 3;
+        uint32_t any = 0;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            const run4 x = keep_elements<E>(v(d), keep);
+            const uint32_t bad = not_finite<E>(x);
+            any |= bad;
+            o[d] = mul16<E>(keep_elements<E>(x, ~bad), p, o[d]);
+        }
+        if (!__any(any != 0)) return;
+#pragma unroll 1
+        for (int e = 0; e < 4 * E::RUN; ++e) {
+            const uint32_t one = (e / E::RUN == g) ? 1u << (e % E::RUN) : 0u;
+            if (!__any((any & one) != 0)) continue;
+            const bool seen = pos0 + e < limit;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const run4 x = keep_elements<E>(v(d), keep & one);
+                const v4f t = mul16<E>(keep_elements<E>(x, not_finite<E>(x)), keep_elements<E>(p, one), o[d]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] = seen ? t[i] : o[d][i];
+            }
+        }
     }
 };
 

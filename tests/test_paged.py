@@ -36,7 +36,7 @@ def call(name, pages=None, batch=None, **kw):
     (dict(k=None), {}), (dict(v=None), {}), (dict(k=(1 << 20) + 8), {}), (dict(type=2), {}), (dict(hd=96), {}),
     (dict(hd=0), {}), (dict(page=8), {}), (dict(page=48), {}), (dict(page=512), {}), (dict(page=0), {}),
     (dict(n_page=0), {}), (dict(n_head_kv=0), {}), (dict(n_head_kv=5), {}), (dict(n_head_kv=64), {}),
-    ({}, dict(n_seq=-1)), ({}, dict(n_tok=-1)), ({}, dict(max_page=0)), ({}, dict(len=None)), ({}, dict(table=None)),
+    ({}, dict(n_seq=-1)), ({}, dict(n_tok=-1)), ({}, dict(max_page=0)), ({}, dict(max_page=(1 << 24) + 1)), ({}, dict(len=None)), ({}, dict(table=None)),
     ({}, dict(start=None, n_tok=1))])
 def test_refused_descriptors(name, pages, batch):
     assert call(name, pages, batch) == -1
