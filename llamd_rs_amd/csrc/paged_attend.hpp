@@ -277,31 +277,31 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
 }
 
 // Rows of a wave of paged_tiles (32, from `limit` and `at` of their lanes) once more, 16 at a time straight from the pages,
-// every infinity or NaN in V added only where it belongs. A function of its own: its registers would cost paged_tiles
-// some of the reads that it keeps in flight.
+// every infinity or NaN in V added only where it belongs. (Inline: a call would give the kernel scratch memory, with which
+// workgroups start at a third of the rate, 14 us for 512 of them instead of 5.)
 template <class E, int HD>
-__device__ __attribute__((noinline)) void attend_again(const PagedAttendArgs *a, const Parts *parts, const Tile *t, int kvh,
-                                                       int begin, int end, size_t slot, int limit, long long at) {
+__device__ __forceinline__ void attend_again(const PagedAttendArgs &a, const Parts &parts, bool part, int seq, int n_kv,
+                                             int kvh, int begin, int end, size_t slot, int limit, long long at) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
 #pragma unroll 1
     for (int b = 0; b < 2; ++b) {
         const int from = 16 * b + (lane & 15), lim = __shfl(limit, from, WAVE);
         const long long row = __shfl(at, from, WAVE);
         run4 q[HD / (4 * E::RUN)];
-        load_few<E, HD>(q, a->q, row);
+        load_few<E, HD>(q, a.q, row);
         FewState<E, HD> st;
         st.clear();
-        attend_few<E, HD, 32>(a->p, pages_of<E, HD>(a->p, t->seq, kvh), t->n_kv, lim, begin, end, q, a->scale, st);
+        attend_few<E, HD, 32>(a.p, pages_of<E, HD>(a.p, seq, kvh), n_kv, lim, begin, end, q, a.scale, st);
         const float l = add_groups(st.l), f = over(l);
-        if (parts) {
-            if (g == 0) parts->ml[slot * 32 + from] = make_float2(st.m, l);
+        if (part) {
+            if (g == 0) parts.ml[slot * 32 + from] = make_float2(st.m, l);
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d)
-                parts->o[(slot * (HD / 4) + 4 * d + g) * 32 + from] = make_float4(st.o[d][0], st.o[d][1], st.o[d][2], st.o[d][3]);
+                parts.o[(slot * (HD / 4) + 4 * d + g) * 32 + from] = make_float4(st.o[d][0], st.o[d][1], st.o[d][2], st.o[d][3]);
         } else if (row >= 0) {
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d)
-                put_out<E>(a->out, a->out_f32, (size_t)row * HD + 16 * d + 4 * g,
+                put_out<E>(a.out, a.out_f32, (size_t)row * HD + 16 * d + 4 * g,
                            make_float4(st.o[d][0] * f, st.o[d][1] * f, st.o[d][2] * f, st.o[d][3] * f));
         }
     }
@@ -659,8 +659,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
     const size_t slot = ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y) * W + wave;
     const bool part = PREFIX || parts > 1;
     if (again) {
-        const PagedAttendArgs args = a;
-        attend_again<E, HD>(&args, part ? &sp.many : nullptr, &t, kvh, range.x * KT, min(range.y * KT, any), slot, row.limit,
+        attend_again<E, HD>(a, sp.many, part, t.seq, t.n_kv, kvh, range.x * KT, min(range.y * KT, any), slot, row.limit,
                             row.at);
         return;
     }
