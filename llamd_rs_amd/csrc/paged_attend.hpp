@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "launch.hpp"
 #include "paged_wave.hpp"
@@ -494,8 +495,15 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
     const int steps = (t.top + KT - 1) / KT, parts = parts_of(steps, sp.parts, tile_least<E>());
     if ((int)blockIdx.y >= parts) return;
     const int2 range = part_steps(steps, parts, blockIdx.y);
-    // positions that all rows of this wave attend to, and that any does
-    const int all = wave_reduce(row.limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
+    // positions that all rows attend to, and that any of this wave's does
+    __shared__ int least[W];
+    const int mine = wave_reduce(row.limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
+    if (lane == 0) least[wave] = mine;
+    __syncthreads();
+    int all = least[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) all = min(all, least[w]);
+    all = __builtin_amdgcn_readfirstlane(all);
     const int any = wave_reduce(row.limit, 0, [](int x, int y) { return max(x, y); });
 
     run4 q[S::QS];
@@ -595,7 +603,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
         put_k(kr, range.x);
         put_v(vr, range.x, valid);
         next = entry(min(range.x + 1, last));
-        for (int step = range.x; step < range.y; ++step) {
+        const auto attend_step = [&](auto masked, int step) {
             __syncthreads();  // the step's tile is there, and the other buffer is read
             const int t0 = step * KT;
             if (step < last) {
@@ -603,7 +611,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
                 load_v(vr, step + 1, next);
             }
             const int after = entry(min(step + 2, last));
-            if (t0 < any) {
+            if (!masked || t0 < any) {
                 const run4 *kt = lds[step & 1][0], *vt = lds[step & 1][1];
                 // this lane's first run of a K and V tile's block; the others by exchanging bits of its place
                 const uint32_t x = fresh(threadIdx.x);
@@ -617,13 +625,24 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
                 for (int b = 0; b < SUB; ++b)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+                // every operand is read AHEAD products before its own (left alone, the compiler reads it right before, and
+                // each product waits for LDS)
+                constexpr int NK = SUB * S::QS, AHEAD = 6;
+                run4 ring[AHEAD];
+                const auto read = [&](int i) {
+                    if (i < NK) ring[i % AHEAD] = kt[32 * (i % SUB) * KCH + (k_first ^ (2 * (i / SUB)))];
+                };
 #pragma unroll
-                for (int c = 0; c < S::QS; ++c)
+                for (int i = 0; i < AHEAD; ++i) read(i);
 #pragma unroll
-                    for (int b = 0; b < SUB; ++b) s[b] = Mma<E>::mul(kt[32 * b * KCH + (k_first ^ (2 * c))], q[c], s[b]);
-                order_reads<E, SUB * S::QS>();
+                for (int i = 0; i < NK; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    s[i % SUB] = Mma<E>::mul(ring[i % AHEAD], q[i / SUB], s[i % SUB]);
+                    read(i + AHEAD);
+                }
+                __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(0);
-                if (t0 + KT > all || valid != ~0ull) {
+                if constexpr (masked) {
                     // a position that a row does not attend to weighs nothing, whatever lies there; but nothing times an
                     // infinity or NaN is NaN: where V has one, these rows are done again (attend_again)
 #pragma unroll
@@ -654,7 +673,12 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
                 put_v(vr, step + 1, valid);
                 next = after;
             }
-        }
+        };
+        // steps that all rows see whole, then the others: in one loop, the two would meet with their scores in different
+        // registers, and every step would move them
+        int step = range.x;
+        for (; step < min(all / KT, range.y) && valid == ~0ull; ++step) attend_step(std::false_type{}, step);
+        for (; step < range.y; ++step) attend_step(std::true_type{}, step);
     }
     const size_t slot = ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y) * W + wave;
     const bool part = PREFIX || parts > 1;
