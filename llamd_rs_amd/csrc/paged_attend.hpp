@@ -95,6 +95,64 @@ __device__ __forceinline__ bool prompt_tile(const PagedArgs &p, int &tile, Tile 
     return false;
 }
 
+// The same for tile number `order` of the batch's tiles by their positions, most first (in units of 2^STEP_LOG): long tiles
+// that start last would leave the GPU to themselves. `unit` becomes the tile's number among all, `tile` that within its
+// sequence. For batches of up to 64 sequences; larger ones, and one sequence, go from the last tile to the first.
+template <int R, int STEP_LOG>
+__device__ __forceinline__ bool prompt_tile_by_size(const PagedArgs &p, int order, int n_units, int &unit, int &tile, Tile &t) {
+    if (p.n_seq == 1 || p.n_seq > WAVE) {
+        unit = tile = n_units - 1 - order;
+        return prompt_tile<R>(p, tile, t);
+    }
+    const int lane = threadIdx.x & 63;
+    int tiles = 0, first = lane, end = lane + 1, len = 0;
+    if (lane < p.n_seq) {
+        len = p.len[lane];
+        if (p.start) {
+            first = min(max(p.start[lane], 0), p.n_tok);
+            end = max(min(p.start[lane + 1], p.n_tok), first);
+        }
+        tiles = (int)(((long long)(end - first) * p.group + R - 1) / R);
+    }
+    const int n_kv = readable_of(p, len), before = len - (end - first);  // positions before its first token
+    // tiles of the lane's sequence that have more than x positions: those whose last token is at x or further
+    const auto more = [&](long long x) {
+        if (x >= n_kv) return 0;
+        const long long y = max(x - before, 0LL);  // token number y on
+        if (y >= end - first) return 0;
+        return tiles - (int)(y * p.group / R);
+    };
+    const auto sum = [](int x) { return wave_reduce(x, 0, [](int u, int v) { return u + v; }); };
+    if (order >= sum(tiles)) return false;
+    int most = wave_reduce(n_kv, 0, [](int u, int v) { return max(u, v); });
+    // the least number of steps such that no more than `order` tiles have more
+    int lo = 0, hi = ((most - 1) >> STEP_LOG) + 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sum(more((long long)mid << STEP_LOG)) <= order) hi = mid;
+        else lo = mid + 1;
+    }
+    // (0 steps: the tiles that see nothing)
+    const int above = more((long long)lo << STEP_LOG), upto = lo ? more((long long)(lo - 1) << STEP_LOG) : tiles;
+    int at = order - sum(above);
+    const int here = upto - above, scan = wave_incl_sum_i(here);
+    const unsigned long long past = __ballot(scan > at);
+    const int l = __builtin_ctzll(past);
+    at -= __builtin_amdgcn_readlane(scan - here, l);
+    // of a sequence's tiles, the last `above` have more
+    tile = __builtin_amdgcn_readlane(tiles - above, l) - 1 - at;
+    unit = __builtin_amdgcn_readlane(wave_incl_sum_i(tiles) - tiles, l) + tile;
+    t.seq = l;
+    t.first = __builtin_amdgcn_readlane(first, l);
+    t.end = __builtin_amdgcn_readlane(end, l);
+    t.len = __builtin_amdgcn_readlane(len, l);
+    t.rows = (int)min((long long)(t.end - t.first) * p.group - (long long)R * tile, (long long)R);
+    t.n_kv = readable_of(p, t.len);
+    const int last = t.first + (int)(((long long)R * tile + t.rows - 1) / p.group);
+    t.top = max(min(t.len - (t.end - last) + 1, t.n_kv), 0);
+    return true;
+}
+
 // Row i of it (the last one for rows that it has not).
 template <int R>
 __device__ __forceinline__ Row prompt_row(const PagedArgs &p, int tile, const Tile &t, int kvh, int i) {
@@ -480,16 +538,15 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
     const int lane = threadIdx.x & 63, m = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    // the last tiles, which have the most positions, go first
-    const int unit = gridDim.x / p.n_kv_head - 1 - blockIdx.x / p.n_kv_head, kvh = blockIdx.x % p.n_kv_head;
-    int tile = unit;
+    const int kvh = blockIdx.x % p.n_kv_head;
+    int unit = blockIdx.x / p.n_kv_head, tile = unit;
     Tile t;
     Row row;
     if constexpr (PREFIX) {
         if (!prefix_tile<R>(a, tile, t)) return;
         row = prefix_row<R>(a, tile, t, kvh, 32 * wave + m);
     } else {
-        if (!prompt_tile<R>(p, tile, t)) return;
+        if (!prompt_tile_by_size<R, KT == 64 ? 6 : 5>(p, unit, gridDim.x / p.n_kv_head, unit, tile, t)) return;
         row = prompt_row<R>(p, tile, t, kvh, 32 * wave + m);
     }
     const int steps = (t.top + KT - 1) / KT, parts = parts_of(steps, sp.parts, tile_least<E>());
