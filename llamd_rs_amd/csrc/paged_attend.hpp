@@ -277,7 +277,8 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
     constexpr bool EARLY = HD * sizeof(T) <= 512;
     const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
     const int all = wave_reduce(limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
-    for (int t0 = begin; t0 < end; t0 += STRIDE) {
+    // a step; false, with nothing done, if it is not `masked` and some position in it cannot be read
+    const auto step = [&](auto masked, int t0) {
         // the pages of the two halves of the step
         const int id0 = pg.table[min(t0, n_kv - 1) >> p.page_log], id1 = pg.table[min(t0 + 16, n_kv - 1) >> p.page_log];
         const bool ok0 = (unsigned)id0 < (unsigned)p.n_page, ok1 = (unsigned)id1 < (unsigned)p.n_page;
@@ -285,6 +286,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
         // bit i: position t0 + i can be read
         uint32_t valid = (ok0 ? 0x0000FFFFu : 0u) | (ok1 ? 0xFFFF0000u : 0u);
         if (n_kv - t0 < 32) valid &= (1u << (n_kv - t0)) - 1u;
+        if (!masked && valid != 0xFFFFFFFFu) return false;
         run4 k[2][S::QS], v[S::PS][S::DB];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -293,16 +295,18 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
 #pragma unroll
             for (int c = 0; c < S::QS; ++c) k[b][c] = *(const run4 *)(x + (4 * c + g) * RUN);
         }
+        const auto v_run = [&](int c, int d, uint32_t plus) {
+            const int r = (4 * c + g) * RUN;
+            const T *x = pg.v + (r & 16 ? at1 : at0) + ((size_t)m << p.page_log) + ((t0 + r) & pg.mask);
+            return *(const run4 *)(x + (((size_t)(16 * d) << p.page_log) + plus));
+        };
         const auto load_v = [&]() {
 #pragma unroll
-            for (int c = 0; c < S::PS; ++c) {
-                const int r = (4 * c + g) * RUN;
-                const T *x = pg.v + (r & 16 ? at1 : at0) + ((size_t)m << p.page_log) + ((t0 + r) & pg.mask);
+            for (int c = 0; c < S::PS; ++c)
 #pragma unroll
-                for (int d = 0; d < S::DB; ++d) v[c][d] = *(const run4 *)(x + ((size_t)(16 * d) << p.page_log));
-            }
+                for (int d = 0; d < S::DB; ++d) v[c][d] = v_run(c, d, 0u);
         };
-        if constexpr (EARLY) load_v();
+        if constexpr (EARLY && !masked) load_v();
         v4f s[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) s[b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -310,9 +314,8 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
         for (int c = 0; c < S::QS; ++c)
 #pragma unroll
             for (int b = 0; b < 2; ++b) s[b] = mul16<E>(k[b][c], q[c], s[b]);
-        if constexpr (!EARLY) load_v();
-        const bool whole = t0 + 32 <= all && valid == 0xFFFFFFFFu;
-        if (!whole) {
+        if constexpr (!EARLY && !masked) load_v();
+        if constexpr (masked) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -325,14 +328,19 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
 #pragma unroll
         for (int c = 0; c < S::PS; ++c) {
             const run4 w = S::weights(s, c);
-            if (whole) {
+            if constexpr (masked) {
+                st.add_masked([&](int d, uint32_t plus) { return v_run(c, d, plus); }, valid >> ((4 * c + g) * RUN), w, t0 + 4 * RUN * c, limit);
+            } else {
 #pragma unroll
                 for (int d = 0; d < S::DB; ++d) st.o[d] = mul16<E>(v[c][d], w, st.o[d]);
-            } else {
-                st.add_masked([&](int d) { return v[c][d]; }, valid >> ((4 * c + g) * RUN), w, t0 + 4 * RUN * c, limit);
             }
         }
-    }
+        return true;
+    };
+    // steps that all rows see whole, then the others
+    int t0 = begin;
+    while (t0 < end && t0 + 32 <= all && step(std::false_type{}, t0)) t0 += STRIDE;
+    for (; t0 < end; t0 += STRIDE) step(std::true_type{}, t0);
 }
 
 // Rows of a wave of paged_tiles (32, from `limit` and `at` of their lanes) once more, 16 at a time straight from the pages,
@@ -387,18 +395,58 @@ __device__ __forceinline__ Own own_of(const PagedAttendArgs &a, int s) {
     if (a.n_groups) x.shared = group_of(a, s, number).shared;
     return x;
 }
-// Positions per part, so that all parts together are about as many as the host wants: by the sum of the tails, which is
-// exact in f64. (2^31 - 128 at most: one part.)
-__device__ __forceinline__ int decode_cut(const PagedAttendArgs &a, const Split &sp) {
-    double sum = 0.0;
-    for (int s = threadIdx.x & 63; s < a.p.n_seq; s += WAVE) sum += (double)own_of(a, s).tail();
-    return (int)min(max(ceil(wave_sum_d(sum) * sp.per_item), 1.0) * FEW_STEP, 2147483520.0);
+// The batch's parts. Up to 64 sequences lie in the lanes of a wave (`mine`), read once.
+struct DecodePlan {
+    Own mine;  // of sequence `lane`
+    int cut;   // positions per part, so that all parts together are about as many as the host wants
+};
+__device__ __forceinline__ DecodePlan decode_plan(const PagedAttendArgs &a, const Split &sp) {
+    const int lane = threadIdx.x & 63;
+    DecodePlan d;
+    d.mine = own_of(a, lane);
+    double sum = (double)d.mine.tail();  // exact
+    for (int s = lane + WAVE; s < a.p.n_seq; s += WAVE) sum += (double)own_of(a, s).tail();
+    // (2^31 - 128 at most: one part)
+    d.cut = (int)min(max(ceil(wave_sum_d(sum) * sp.per_item), 1.0) * FEW_STEP, 2147483520.0);
+    return d;
+}
+// The sequence of part number `part` (its number within the sequence afterwards); -1: past the last.
+__device__ __forceinline__ int part_sequence(const PagedAttendArgs &a, const DecodePlan &d, int &part, Own &own) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < a.p.n_seq; s0 += WAVE) {
+        const Own x = s0 ? own_of(a, s0 + lane) : d.mine;
+        const int units = s0 + lane < a.p.n_seq ? x.units(d.cut) : 0, sum = wave_incl_sum_i(units);
+        const unsigned long long past = __ballot(sum > part);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            part -= __builtin_amdgcn_readlane(sum - units, l);
+            own.n = __builtin_amdgcn_readlane(x.n, l);
+            own.shared = __builtin_amdgcn_readlane(x.shared, l);
+            return s0 + l;
+        }
+        part -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return -1;
+}
+// Parts of the sequences before sequence `seq`, and its own positions.
+__device__ __forceinline__ int parts_before(const PagedAttendArgs &a, const DecodePlan &d, int seq, Own &own) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int s0 = 0; s0 <= seq; s0 += WAVE) {
+        const Own x = s0 ? own_of(a, s0 + lane) : d.mine;
+        if (s0 + lane < seq) before += x.units(d.cut);
+        if (seq - s0 < WAVE) {
+            own.n = __builtin_amdgcn_readlane(x.n, seq - s0);
+            own.shared = __builtin_amdgcn_readlane(x.shared, seq - s0);
+        }
+    }
+    return wave_reduce(before, 0, [](int x, int y) { return x + y; });
 }
 
 // DECODE: blockIdx.x a part of a sequence, blockIdx.y a kv head and block of 16 of its query heads. Otherwise blockIdx.x
 // a tile of 16 rows of a prompt batch and a kv head, blockIdx.y a part of its positions.
 template <class E, int HD, bool DECODE>
-__global__ __launch_bounds__(256) void paged_few(PagedAttendArgs a, Split sp) {
+__global__ __launch_bounds__(256, E::RUN == 4 && HD <= 128 ? 3 : 1) void paged_few(PagedAttendArgs a, Split sp) {
     typedef FewState<E, HD> S;
     __shared__ float2 stats[4][16];
     __shared__ float part[4][HD / 4][64];
@@ -410,24 +458,11 @@ __global__ __launch_bounds__(256) void paged_few(PagedAttendArgs a, Split sp) {
     int begin, end, parts, kvh;
     size_t slot;
     if constexpr (DECODE) {
-        const int cut = decode_cut(a, sp);
+        const DecodePlan plan = decode_plan(a, sp);
+        const int cut = plan.cut;
         int unit = blockIdx.x;
         Own own;
-        t.seq = -1;
-        for (int s0 = 0; s0 < p.n_seq; s0 += WAVE) {
-            const Own mine = own_of(a, s0 + lane);
-            const int units = s0 + lane < p.n_seq ? mine.units(cut) : 0, sum = wave_incl_sum_i(units);
-            const unsigned long long past = __ballot(sum > unit);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                unit -= __builtin_amdgcn_readlane(sum - units, l);
-                own.n = __builtin_amdgcn_readlane(mine.n, l);
-                own.shared = __builtin_amdgcn_readlane(mine.shared, l);
-                t.seq = s0 + l;
-                break;
-            }
-            unit -= __builtin_amdgcn_readlane(sum, 63);
-        }
+        t.seq = part_sequence(a, plan, unit, own);
         if (t.seq < 0) return;
         const int per = (p.group + 15) / 16, head = (blockIdx.y % per) * 16 + m;
         kvh = blockIdx.y / per;
@@ -760,54 +795,71 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
 
 // ---- the parts together ------------------------------------------------------------
 
-// Up to ROWS rows (of HD values) out of `n` parts: part z's statistics of row r are ml(z, r), its O of four dimensions
-// o(z, r, four). Every thread has its own parts' statistics, then its own pieces of O over all parts, whose loads depend on
-// nothing and overlap.
-constexpr int JOIN_MOST = 512;  // parts of a row at the most
-template <class E, int HD, int ROWS, class Ml, class O, class At>
+// Up to ROWS rows' 32 dimensions (number blockIdx.z) out of `n` parts: part z's statistics of row r are ml(z, r), its O of
+// four dimensions o(z, r, four). Small workgroups and groups of threads that share the parts among them: few loads wait for
+// each other, which is what this would spend its time on (1 x 4100 positions, 33 parts: 14 -> 4 us).
+constexpr int JOIN_MOST = 256;  // parts of a row at the most
+template <class E, int ROWS, class Ml, class O, class At>
 __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, Ml ml, O o, At at) {
-    __shared__ float weight[JOIN_MOST * 16];
-    __shared__ float side[256 / ROWS][ROWS];
-    const int r = threadIdx.x % ROWS, k = threadIdx.x / ROWS;
-    constexpr int K = 256 / ROWS;
+    constexpr int FOURS = 8, GROUPS = 256 / (ROWS * FOURS), K = 256 / ROWS, HELD = 4;
+    __shared__ float2 stats[JOIN_MOST * ROWS];
+    __shared__ float side[K][ROWS];
+    __shared__ float4 sums[GROUPS][FOURS * ROWS];
+    const int r = threadIdx.x % ROWS, k = threadIdx.x / ROWS, f = k % FOURS, group = k / FOURS;
+    const int four = blockIdx.z * FOURS + f;
     const bool here = r < rows;
+    for (int z = k; z < n; z += K) stats[z * ROWS + r] = here ? ml(z, r) : make_float2(NEG_INF, 0.0f);
+    float4 held[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int z = group + i * GROUPS;
+        held[i] = here && z < n ? o(z, r, four) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
     float top = NEG_INF;
-    for (int z = k; z < n; z += K)
-        if (here) top = fmaxf(top, ml(z, r).x);
+    for (int z = k; z < n; z += K) top = fmaxf(top, stats[z * ROWS + r].x);  // this thread's own writes
     side[k][r] = top;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < K; ++i) top = fmaxf(top, side[i][r]);
     __syncthreads();
     float l = 0.0f;
-    for (int z = k; z < n; z += K)
-        if (here) {
-            const float2 x = ml(z, r);
-            const float f = exp2_fast(x.x - against(top));
-            weight[z * ROWS + r] = f;
-            l = __builtin_fmaf(x.y, f, l);
-        }
+    for (int z = k; z < n; z += K) {
+        const float2 x = stats[z * ROWS + r];
+        const float w = exp2_fast(x.x - against(top));
+        stats[z * ROWS + r].x = w;
+        l = __builtin_fmaf(x.y, w, l);
+    }
     side[k][r] = l;
     __syncthreads();
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < K; ++i) l += side[i][r];
-    const float by = over(l);
-    const long long row = here ? at(r) : -1;
-    if (row < 0) return;
-    for (int four = k; four < HD / 4; four += K) {
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int z = 0; z < n; ++z) {
-            const float4 x = o(z, r, four);
-            const float f = weight[z * ROWS + r];
-            y.x = __builtin_fmaf(x.x, f, y.x);
-            y.y = __builtin_fmaf(x.y, f, y.y);
-            y.z = __builtin_fmaf(x.z, f, y.z);
-            y.w = __builtin_fmaf(x.w, f, y.w);
-        }
-        put_out<E>(a.out, a.out_f32, (size_t)row * HD + 4 * four, make_float4(y.x * by, y.y * by, y.z * by, y.w * by));
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&](float4 x, float w) {
+        y.x = __builtin_fmaf(x.x, w, y.x);
+        y.y = __builtin_fmaf(x.y, w, y.y);
+        y.z = __builtin_fmaf(x.z, w, y.z);
+        y.w = __builtin_fmaf(x.w, w, y.w);
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int z = group + i * GROUPS;
+        if (z < n) add(held[i], stats[z * ROWS + r].x);
     }
+    if (here) {
+#pragma unroll 8
+        for (int z = group + HELD * GROUPS; z < n; z += GROUPS) add(o(z, r, four), stats[z * ROWS + r].x);
+    }
+    sums[group][f * ROWS + r] = y;
+    __syncthreads();
+    const long long row = here && !group ? at(r) : -1;
+    if (row < 0) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) add(sums[i][f * ROWS + r], 1.0f);
+    const float by = over(l);
+    // (the row length from the grid: 32 dimensions each)
+    put_out<E>(a.out, a.out_f32, (size_t)row * (32 * gridDim.z) + 4 * four,
+               make_float4(y.x * by, y.y * by, y.z * by, y.w * by));
 }
 
 // blockIdx.x: a tile of R rows and kv head of a prompt batch, blockIdx.y: 16 of its rows.
@@ -827,26 +879,24 @@ __global__ __launch_bounds__(256) void paged_join(PagedAttendArgs a, Split sp) {
     const size_t slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts;
     const int block = FEW ? 0 : first / 32, place = FEW ? 0 : first % 32;
     const auto at = [&](int z) { return FEW ? slot + z : (slot + z) * (R / 32) + block; };
-    join<E, HD, 16>(
+    join<E, 16>(
         a, parts, min(t.rows - first, 16), [&](int z, int r) { return x.ml[at(z) * (FEW ? 16 : 32) + place + r]; },
         [&](int z, int r, int four) { return x.o[(at(z) * (HD / 4) + four) * (FEW ? 16 : 32) + place + r]; },
         [&](int r) { return prompt_row<R>(p, tile, t, kvh, first + r).at; });
 }
 
-// blockIdx.x: a sequence, blockIdx.y: a kv head and block of 16 of its query heads. R: rows of the prefix's tiles.
-template <class E, int HD, int R>
+// blockIdx.x: a sequence, blockIdx.y: a kv head and block of 16 of its query heads. R: rows of the prefix's tiles. ROWS: at
+// least the rows of a slot.
+template <class E, int HD, int R, int ROWS>
 __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Split sp) {
     const PagedArgs &p = a.p;
     const int lane = threadIdx.x & 63, seq = blockIdx.x, per = (p.group + 15) / 16;
     const int kvh = blockIdx.y / per, head = (blockIdx.y % per) * 16;
-    const int cut = decode_cut(a, sp);
-    const Own own = own_of(a, seq);
-    const int units = own.units(cut);
+    const DecodePlan plan = decode_plan(a, sp);
+    Own own;
+    const int before = parts_before(a, plan, seq, own), units = own.units(plan.cut);
     const bool prefix = own.shared && own.n;
     if (!prefix && units < 2) return;
-    int before = 0;  // parts of the sequences before this one
-    for (int s = lane; s < seq; s += WAVE) before += own_of(a, s).units(cut);
-    before = wave_reduce(before, 0, [](int x, int y) { return x + y; });
     int parts = 0, base = 0;  // of the prefix, and the number of the group's first row among its 32-row blocks
     long long first = 0;
     if (prefix) {
@@ -865,7 +915,7 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
     };
     const auto few = [&](int z) { return (size_t)(before + z - parts) * gridDim.y + blockIdx.y; };
     const int w = sp.few.rows;
-    join<E, HD, 16>(
+    join<E, ROWS>(
         a, parts + units, min(p.group - head, 16),
         [&](int z, int r) {
             return z < parts ? sp.many.ml[many(z, r) * 32 + (first + r) % 32] : sp.few.ml[few(z) * w + r];
@@ -907,12 +957,12 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
     const long long most = ((long long)p.max_page << p.page_log) / (KT * tile_least<E>());
     Split sp{};
-    sp.parts = fit((want + busy - 1) / busy, most, 64);
+    sp.parts = fit(want / busy, most, 64);
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * W, 0, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
     hipLaunchKernelGGL((paged_tiles<E, HD, W, false>), grid, dim3(64 * W), 0, st, a, sp);
-    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, R>), dim3(grid.x, R / 16), dim3(256), 0, st, a, sp);
+    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, R>), dim3(grid.x, R / 16, HD / 32), dim3(256), 0, st, a, sp);
     return queued();
 }
 
@@ -923,12 +973,12 @@ int prompt_few(const PagedAttendArgs &a, hipStream_t st) {
     const long long busy = (rows + 15) / 16 * p.n_kv_head, want = 2 * CUS;
     const long long most = ((long long)p.max_page << p.page_log) / FEW_STEP;
     Split sp{};
-    sp.parts = fit((want + busy - 1) / busy, most, 256);
+    sp.parts = fit(want / busy, most, 128);
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     if (sp.parts > 1 && !room(sp, 0, (size_t)tiles * p.n_kv_head * sp.parts, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
     hipLaunchKernelGGL((paged_few<E, HD, false>), grid, dim3(256), 0, st, a, sp);
-    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, 16>), dim3(grid.x), dim3(256), 0, st, a, sp);
+    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, 16>), dim3(grid.x, 1, HD / 32), dim3(256), 0, st, a, sp);
     return queued();
 }
 
@@ -964,7 +1014,7 @@ int decode_with(const PagedAttendArgs &a, hipStream_t st) {
         const long long rows = (long long)p.n_seq * p.group;
         tiles = rows / R + a.n_groups;
         const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
-        sp.parts = fit((want + busy - 1) / busy, top / (KT * tile_least<E>()), 64);
+        sp.parts = fit(want / busy, top / (KT * tile_least<E>()), 64);
         slots = tiles * p.n_kv_head * sp.parts * W;
     }
     if (items > 0x7FFFFFFF / 512 || cols > 65535 || tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
@@ -974,7 +1024,11 @@ int decode_with(const PagedAttendArgs &a, hipStream_t st) {
         hipLaunchKernelGGL((paged_tiles<E, HD, W, true>), dim3((unsigned)(tiles * p.n_kv_head), sp.parts), dim3(64 * W), 0,
                            st, a, sp);
     hipLaunchKernelGGL((paged_few<E, HD, true>), dim3((unsigned)items, cols), dim3(256), 0, st, a, sp);
-    if (join) hipLaunchKernelGGL((paged_join_decode<E, HD, R>), dim3(p.n_seq, cols), dim3(256), 0, st, a, sp);
+    if (join) {
+        const dim3 grid(p.n_seq, cols, HD / 32);
+        if (p.group <= 8) hipLaunchKernelGGL((paged_join_decode<E, HD, R, 8>), grid, dim3(256), 0, st, a, sp);
+        else hipLaunchKernelGGL((paged_join_decode<E, HD, R, 16>), grid, dim3(256), 0, st, a, sp);
+    }
     return queued();
 }
 

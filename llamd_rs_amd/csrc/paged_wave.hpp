@@ -294,7 +294,7 @@ template <class E, int HD> struct FewState {
         return to_run<E>(x);
     }
 
-    // One step of the second product where some of V is not to be read as it stands: of the runs v(d) of the dimension
+    // One step of the second product where some of V is not to be read as it stands: of the runs v(d, 0) of the dimension
     // blocks, the elements of `keep` can be read, the others may hold anything. An infinity or NaN at a position that
     // only some rows attend to gives the others nothing, not 0 * inf: such elements are left out of the product and
     // added one position at a time (pos0 + e) to the rows that see it.
@@ -304,10 +304,11 @@ template <class E, int HD> struct FewState {
         uint32_t any = 0;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            const run4 x = keep_elements<E>(v(d), keep);
+            const run4 x = keep_elements<E>(v(d, 0u), keep);
             const uint32_t bad = not_finite<E>(x);
             any |= bad;
             o[d] = mul16<E>(keep_elements<E>(x, ~bad), p, o[d]);
+            __builtin_amdgcn_sched_barrier(0);  // one d's masks at a time: registers
         }
         if (!__any(any != 0)) return;
 #pragma unroll 1
@@ -315,12 +316,15 @@ template <class E, int HD> struct FewState {
             const uint32_t one = (e / E::RUN == g) ? 1u << (e % E::RUN) : 0u;
             if (!__any((any & one) != 0)) continue;
             const bool seen = pos0 + e < limit;
+            uint32_t none = 0;
+            asm volatile("" : "+v"(none));  // the runs are read again: held in registers throughout, they would crowd out others
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const run4 x = keep_elements<E>(v(d), keep & one);
+                const run4 x = keep_elements<E>(v(d, none), keep & one);
                 const v4f t = mul16<E>(keep_elements<E>(x, not_finite<E>(x)), keep_elements<E>(p, one), o[d]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[d][i] = seen ? t[i] : o[d][i];
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
