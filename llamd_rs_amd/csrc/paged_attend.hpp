@@ -795,26 +795,30 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
 
 // ---- the parts together ------------------------------------------------------------
 
-// Up to ROWS rows' 32 dimensions (number blockIdx.z) out of `n` parts: part z's statistics of row r are ml(z, r), its O of
-// four dimensions o(z, r, four). Small workgroups and groups of threads that share the parts among them: few loads wait for
-// each other, which is what this would spend its time on (1 x 4100 positions, 33 parts: 14 -> 4 us).
+// Up to ROWS rows of HD values (blockIdx.z of gridDim.z equal shares of the dimensions) out of `n` parts: part z's statistics
+// of row r are ml(z, r), its O of four dimensions o(z, r, four). Groups of threads share the parts among them, and the first
+// loads of O do not wait for the statistics: few loads wait for each other, which is what this would spend its time on
+// (1 x 4100 positions, 33 parts: 14 -> 6 us).
 constexpr int JOIN_MOST = 256;  // parts of a row at the most
-template <class E, int ROWS, class Ml, class O, class At>
+template <class E, int HD, int ROWS, class Ml, class O, class At>
 __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, Ml ml, O o, At at) {
     constexpr int FOURS = 8, GROUPS = 256 / (ROWS * FOURS), K = 256 / ROWS, HELD = 4;
     __shared__ float2 stats[JOIN_MOST * ROWS];
     __shared__ float side[K][ROWS];
     __shared__ float4 sums[GROUPS][FOURS * ROWS];
     const int r = threadIdx.x % ROWS, k = threadIdx.x / ROWS, f = k % FOURS, group = k / FOURS;
-    const int four = blockIdx.z * FOURS + f;
+    const int share = HD / 4 / gridDim.z, begin = blockIdx.z * share;
     const bool here = r < rows;
     for (int z = k; z < n; z += K) stats[z * ROWS + r] = here ? ml(z, r) : make_float2(NEG_INF, 0.0f);
     float4 held[HELD];
+    const auto hold = [&](int four) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        const int z = group + i * GROUPS;
-        held[i] = here && z < n ? o(z, r, four) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
+        for (int i = 0; i < HELD; ++i) {
+            const int z = group + i * GROUPS;
+            held[i] = here && z < n ? o(z, r, four) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+    hold(begin + f);
     float top = NEG_INF;
     for (int z = k; z < n; z += K) top = fmaxf(top, stats[z * ROWS + r].x);  // this thread's own writes
     side[k][r] = top;
@@ -834,32 +838,36 @@ __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, 
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < K; ++i) l += side[i][r];
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const auto add = [&](float4 x, float w) {
-        y.x = __builtin_fmaf(x.x, w, y.x);
-        y.y = __builtin_fmaf(x.y, w, y.y);
-        y.z = __builtin_fmaf(x.z, w, y.z);
-        y.w = __builtin_fmaf(x.w, w, y.w);
-    };
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        const int z = group + i * GROUPS;
-        if (z < n) add(held[i], stats[z * ROWS + r].x);
-    }
-    if (here) {
-#pragma unroll 8
-        for (int z = group + HELD * GROUPS; z < n; z += GROUPS) add(o(z, r, four), stats[z * ROWS + r].x);
-    }
-    sums[group][f * ROWS + r] = y;
-    __syncthreads();
-    const long long row = here && !group ? at(r) : -1;
-    if (row < 0) return;
-#pragma unroll
-    for (int i = 1; i < GROUPS; ++i) add(sums[i][f * ROWS + r], 1.0f);
     const float by = over(l);
-    // (the row length from the grid: 32 dimensions each)
-    put_out<E>(a.out, a.out_f32, (size_t)row * (32 * gridDim.z) + 4 * four,
-               make_float4(y.x * by, y.y * by, y.z * by, y.w * by));
+    const long long row = here ? at(r) : -1;
+    for (int four = begin + f; four < begin + share; four += FOURS) {
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const auto add = [&](float4 x, float w) {
+            y.x = __builtin_fmaf(x.x, w, y.x);
+            y.y = __builtin_fmaf(x.y, w, y.y);
+            y.z = __builtin_fmaf(x.z, w, y.z);
+            y.w = __builtin_fmaf(x.w, w, y.w);
+        };
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int z = group + i * GROUPS;
+            if (z < n) add(held[i], stats[z * ROWS + r].x);
+        }
+        if (four + FOURS < begin + share) hold(four + FOURS);
+        if (here) {
+#pragma unroll 8
+            for (int z = group + HELD * GROUPS; z < n; z += GROUPS) add(o(z, r, four), stats[z * ROWS + r].x);
+        }
+        sums[group][f * ROWS + r] = y;
+        __syncthreads();
+        if (row >= 0 && !group) {
+#pragma unroll
+            for (int i = 1; i < GROUPS; ++i) add(sums[i][f * ROWS + r], 1.0f);
+            put_out<E>(a.out, a.out_f32, (size_t)row * HD + 4 * four,
+                       make_float4(y.x * by, y.y * by, y.z * by, y.w * by));
+        }
+        __syncthreads();
+    }
 }
 
 // blockIdx.x: a tile of R rows and kv head of a prompt batch, blockIdx.y: 16 of its rows.
@@ -879,7 +887,7 @@ __global__ __launch_bounds__(256) void paged_join(PagedAttendArgs a, Split sp) {
     const size_t slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts;
     const int block = FEW ? 0 : first / 32, place = FEW ? 0 : first % 32;
     const auto at = [&](int z) { return FEW ? slot + z : (slot + z) * (R / 32) + block; };
-    join<E, 16>(
+    join<E, HD, 16>(
         a, parts, min(t.rows - first, 16), [&](int z, int r) { return x.ml[at(z) * (FEW ? 16 : 32) + place + r]; },
         [&](int z, int r, int four) { return x.o[(at(z) * (HD / 4) + four) * (FEW ? 16 : 32) + place + r]; },
         [&](int r) { return prompt_row<R>(p, tile, t, kvh, first + r).at; });
@@ -915,7 +923,7 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
     };
     const auto few = [&](int z) { return (size_t)(before + z - parts) * gridDim.y + blockIdx.y; };
     const int w = sp.few.rows;
-    join<E, ROWS>(
+    join<E, HD, ROWS>(
         a, parts + units, min(p.group - head, 16),
         [&](int z, int r) {
             return z < parts ? sp.many.ml[many(z, r) * 32 + (first + r) % 32] : sp.few.ml[few(z) * w + r];
@@ -962,7 +970,7 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * W, 0, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
     hipLaunchKernelGGL((paged_tiles<E, HD, W, false>), grid, dim3(64 * W), 0, st, a, sp);
-    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, R>), dim3(grid.x, R / 16, HD / 32), dim3(256), 0, st, a, sp);
+    if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, R>), dim3(grid.x, R / 16), dim3(256), 0, st, a, sp);
     return queued();
 }
 
