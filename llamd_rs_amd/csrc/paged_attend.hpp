@@ -443,13 +443,24 @@ __device__ __forceinline__ int parts_before(const PagedAttendArgs &a, const Deco
     return wave_reduce(before, 0, [](int x, int y) { return x + y; });
 }
 
-// DECODE: blockIdx.x a part of a sequence, blockIdx.y a kv head and block of 16 of its query heads. Otherwise blockIdx.x
-// a tile of 16 rows of a prompt batch and a kv head, blockIdx.y a part of its positions.
+// A workgroup's place in a grid of nx x ny.
+struct Place {
+    int x, y, nx, ny;
+};
+
+// What a workgroup of four waves keeps in LDS for up to 16 rows.
+template <int HD> struct FewShared {
+    float part[4][HD / 4][64];
+    float2 stats[4][16];
+};
+
+// DECODE: at.x a part of a sequence, at.y a kv head and block of 16 of its query heads. Otherwise at.x a tile of 16 rows of a
+// prompt batch and a kv head, at.y a part of its positions.
 template <class E, int HD, bool DECODE>
-__global__ __launch_bounds__(256, E::RUN == 4 && HD <= 128 ? 3 : 1) void paged_few(PagedAttendArgs a, Split sp) {
+__device__ __forceinline__ void few_rows(const PagedAttendArgs &a, const Split &sp, Place at, FewShared<HD> &shared) {
     typedef FewState<E, HD> S;
-    __shared__ float2 stats[4][16];
-    __shared__ float part[4][HD / 4][64];
+    auto &stats = shared.stats;
+    auto &part = shared.part;
     const PagedArgs &p = a.p;
     const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -460,31 +471,31 @@ __global__ __launch_bounds__(256, E::RUN == 4 && HD <= 128 ? 3 : 1) void paged_f
     if constexpr (DECODE) {
         const DecodePlan plan = decode_plan(a, sp);
         const int cut = plan.cut;
-        int unit = blockIdx.x;
+        int unit = at.x;
         Own own;
         t.seq = part_sequence(a, plan, unit, own);
         if (t.seq < 0) return;
-        const int per = (p.group + 15) / 16, head = (blockIdx.y % per) * 16 + m;
-        kvh = blockIdx.y / per;
+        const int per = (p.group + 15) / 16, head = (at.y % per) * 16 + m;
+        kvh = at.y / per;
         t.n_kv = r.limit = own.n;
         r.at = head < p.group ? (long long)t.seq * p.n_head + kvh * p.group + head : -1;
         begin = (int)min((long long)own.shared + (long long)unit * cut, 0x7FFFFFFFLL);
         end = (int)min((long long)begin + cut, (long long)t.n_kv);
         parts = own.shared && own.n ? 2 : own.units(cut);
-        slot = (size_t)blockIdx.x * gridDim.y + blockIdx.y;
+        slot = (size_t)at.x * at.ny + at.y;
     } else {
-        kvh = blockIdx.x % p.n_kv_head;
-        const int unit = gridDim.x / p.n_kv_head - 1 - blockIdx.x / p.n_kv_head;
+        kvh = at.x % p.n_kv_head;
+        const int unit = at.nx / p.n_kv_head - 1 - at.x / p.n_kv_head;
         int tile = unit;
         if (!prompt_tile<16>(p, tile, t)) return;
         r = prompt_row<16>(p, tile, t, kvh, m);
         const int steps = (t.top + FEW_STEP - 1) / FEW_STEP;
         parts = parts_of(steps, sp.parts, 1);
-        if ((int)blockIdx.y >= parts) return;
-        const int2 range = part_steps(steps, parts, blockIdx.y);
+        if (at.y >= parts) return;
+        const int2 range = part_steps(steps, parts, at.y);
         begin = range.x * FEW_STEP;
         end = min(range.y * FEW_STEP, t.top);
-        slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y;
+        slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts + at.y;
     }
     run4 q[S::QS];
     load_few<E, HD>(q, a.q, r.at);
@@ -530,6 +541,12 @@ __global__ __launch_bounds__(256, E::RUN == 4 && HD <= 128 ? 3 : 1) void paged_f
     }
 }
 
+template <class E, int HD, bool DECODE>
+__global__ __launch_bounds__(256, E::RUN == 4 && HD <= 128 ? 3 : 1) void paged_few(PagedAttendArgs a, Split sp) {
+    __shared__ __align__(16) FewShared<HD> shared;
+    few_rows<E, HD, DECODE>(a, sp, {(int)blockIdx.x, (int)blockIdx.y, (int)gridDim.x, (int)gridDim.y}, shared);
+}
+
 // ---- many rows -------------------------------------------------------------------
 
 // x, as something that the compiler cannot keep the results of between tiles: addresses are cheaper made again than held
@@ -558,9 +575,14 @@ template <class E, int HD> __host__ __device__ constexpr int tile_positions() {
 }
 template <class E> __host__ __device__ constexpr int tile_least() { return E::RUN == 8 ? 4 : 1; }
 
-// W waves of 32 rows each.
+template <class E, int HD> struct TileShared {
+    run4 lds[2][2][tile_positions<E, HD>() * HD / E::RUN];  // two buffers of K and V
+    int least[8];
+};
+
+// W waves of 32 rows each. at.x: a tile and kv head, at.y: a part of its positions.
 template <class E, int HD, int W, bool PREFIX>
-__global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256 ? 2 : 1) void paged_tiles(PagedAttendArgs a, Split sp) {
+__device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split &sp, Place at, TileShared<E, HD> &shared) {
     typedef typename E::T T;
     typedef RowState<E, HD> S;
     constexpr int RUN = E::RUN, R = 32 * W, THREADS = 64 * W;
@@ -568,27 +590,27 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
     constexpr int SUB = KT / 32;
     constexpr int KCH = HD / RUN, VCH = KT / RUN;                 // 16-byte runs per row of a tile
     constexpr int N = KT * KCH / THREADS;                             // loads of each thread per K (V) tile
-    __shared__ __align__(16) run4 lds[2][2][KT * KCH];
+    auto &lds = shared.lds;
+    auto &least = shared.least;
     const PagedArgs &p = a.p;
     const int lane = threadIdx.x & 63, m = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    const int kvh = blockIdx.x % p.n_kv_head;
-    int unit = blockIdx.x / p.n_kv_head, tile = unit;
+    const int kvh = at.x % p.n_kv_head;
+    int unit = at.x / p.n_kv_head, tile = unit;
     Tile t;
     Row row;
     if constexpr (PREFIX) {
         if (!prefix_tile<R>(a, tile, t)) return;
         row = prefix_row<R>(a, tile, t, kvh, 32 * wave + m);
     } else {
-        if (!prompt_tile_by_size<R, KT == 64 ? 6 : 5>(p, unit, gridDim.x / p.n_kv_head, unit, tile, t)) return;
+        if (!prompt_tile_by_size<R, KT == 64 ? 6 : 5>(p, unit, at.nx / p.n_kv_head, unit, tile, t)) return;
         row = prompt_row<R>(p, tile, t, kvh, 32 * wave + m);
     }
     const int steps = (t.top + KT - 1) / KT, parts = parts_of(steps, sp.parts, tile_least<E>());
-    if ((int)blockIdx.y >= parts) return;
-    const int2 range = part_steps(steps, parts, blockIdx.y);
+    if (at.y >= parts) return;
+    const int2 range = part_steps(steps, parts, at.y);
     // positions that all rows attend to, and that any of this wave's does
-    __shared__ int least[W];
     const int mine = wave_reduce(row.limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
     if (lane == 0) least[wave] = mine;
     __syncthreads();
@@ -772,7 +794,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
         for (; step < min(all / KT, range.y) && valid == ~0ull; ++step) attend_step(std::false_type{}, step);
         for (; step < range.y; ++step) attend_step(std::true_type{}, step);
     }
-    const size_t slot = ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + blockIdx.y) * W + wave;
+    const size_t slot = ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + at.y) * W + wave;
     const bool part = PREFIX || parts > 1;
     if (again) {
         attend_again<E, HD>(a, sp.many, part, t.seq, t.n_kv, kvh, range.x * KT, min(range.y * KT, any), slot, row.limit,
@@ -791,6 +813,31 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
             if (part) sp.many.o[(slot * (HD / 4) + four) * 32 + m] = y;
             else if (row.at >= 0) put_out<E>(a.out, a.out_f32, (size_t)row.at * HD + 4 * four, y);
         }
+}
+
+template <class E, int HD, int W>
+__global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256 ? 2 : 1) void paged_tiles(PagedAttendArgs a, Split sp) {
+    __shared__ __align__(16) TileShared<E, HD> shared;
+    tile_rows<E, HD, W, false>(a, sp, {(int)blockIdx.x, (int)blockIdx.y, (int)gridDim.x, (int)gridDim.y}, shared);
+}
+
+// A decode batch with groups: the first nx * ny workgroups have the tiles of the shared positions, the others the
+// sequences' own, which run beside them (32 sequences, 2000 shared positions and up to 500 of their own: 22 us, two launches
+// 15.5 + 14.5).
+template <class E, int HD>
+__global__ __launch_bounds__(256, HD * sizeof(typename E::T) <= 256 ? 2 : 1) void paged_decode(PagedAttendArgs a, Split sp,
+                                                                                           int nx, int ny, int cols) {
+    __shared__ __align__(16) union {
+        TileShared<E, HD> tile;
+        FewShared<HD> few;
+    } shared;
+    int at = blockIdx.x;
+    if (at < nx * ny) {
+        tile_rows<E, HD, 4, true>(a, sp, {at % nx, at / nx, nx, ny}, shared.tile);
+    } else {
+        at -= nx * ny;
+        few_rows<E, HD, true>(a, sp, {at / cols, at % cols, ((int)gridDim.x - nx * ny) / cols, cols}, shared.few);
+    }
 }
 
 // ---- the parts together ------------------------------------------------------------
@@ -969,7 +1016,7 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * W, 0, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
-    hipLaunchKernelGGL((paged_tiles<E, HD, W, false>), grid, dim3(64 * W), 0, st, a, sp);
+    hipLaunchKernelGGL((paged_tiles<E, HD, W>), grid, dim3(64 * W), 0, st, a, sp);
     if (sp.parts > 1) hipLaunchKernelGGL((paged_join<E, HD, R>), dim3(grid.x, R / 16), dim3(256), 0, st, a, sp);
     return queued();
 }
@@ -1005,10 +1052,10 @@ int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
     return prompt_tiles<E, HD, 4>(a, st);
 }
 
-template <class E, int HD, int W>
-int decode_with(const PagedAttendArgs &a, hipStream_t st) {
+template <class E, int HD>
+int decode_as(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
-    constexpr int R = 32 * W, KT = tile_positions<E, HD>();
+    constexpr int R = 128, KT = tile_positions<E, HD>();
     const int per = (p.group + 15) / 16, cols = p.n_kv_head * per;
     const long long top = (long long)p.max_page << p.page_log;
     Split sp{};
@@ -1021,31 +1068,26 @@ int decode_with(const PagedAttendArgs &a, hipStream_t st) {
     if (a.n_groups) {
         const long long rows = (long long)p.n_seq * p.group;
         tiles = rows / R + a.n_groups;
-        const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
+        const long long busy = (rows + R - 1) / R * p.n_kv_head, want = 2 * CUS;
         sp.parts = fit(want / busy, top / (KT * tile_least<E>()), 64);
-        slots = tiles * p.n_kv_head * sp.parts * W;
+        slots = tiles * p.n_kv_head * sp.parts * 4;
     }
     if (items > 0x7FFFFFFF / 512 || cols > 65535 || tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     const bool join = a.n_groups || top > FEW_STEP;
     if (join && !room(sp, slots, (size_t)items * cols, std::min(p.group, 16), HD)) return -1;
-    if (a.n_groups)
-        hipLaunchKernelGGL((paged_tiles<E, HD, W, true>), dim3((unsigned)(tiles * p.n_kv_head), sp.parts), dim3(64 * W), 0,
-                           st, a, sp);
-    hipLaunchKernelGGL((paged_few<E, HD, true>), dim3((unsigned)items, cols), dim3(256), 0, st, a, sp);
+    if (a.n_groups) {
+        const long long nx = tiles * p.n_kv_head, grid = nx * sp.parts + items * cols;
+        if (grid > 0x7FFFFFFF / 512) return -1;
+        hipLaunchKernelGGL((paged_decode<E, HD>), dim3((unsigned)grid), dim3(256), 0, st, a, sp, (int)nx, sp.parts, cols);
+    } else {
+        hipLaunchKernelGGL((paged_few<E, HD, true>), dim3((unsigned)items, cols), dim3(256), 0, st, a, sp);
+    }
     if (join) {
         const dim3 grid(p.n_seq, cols, HD / 32);
         if (p.group <= 8) hipLaunchKernelGGL((paged_join_decode<E, HD, R, 8>), grid, dim3(256), 0, st, a, sp);
         else hipLaunchKernelGGL((paged_join_decode<E, HD, R, 16>), grid, dim3(256), 0, st, a, sp);
     }
     return queued();
-}
-
-template <class E, int HD>
-int decode_as(const PagedAttendArgs &a, hipStream_t st) {
-    const long long rows = a.n_groups ? (long long)a.p.n_seq * a.p.group / a.n_groups : 0;  // of a group, on average
-    if constexpr (wide<E, HD>())
-        if (rows >= 1024) return decode_with<E, HD, 8>(a, st);
-    return decode_with<E, HD, 4>(a, st);
 }
 
 template <class E>
