@@ -36,6 +36,8 @@ DEVICE_FLAGS = [
     "-ffp-contract=off",
     "-fno-fast-math",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    # MFMA results in VGPRs: no accumulator-register reads after every MFMA
+    "-mllvm", "-amdgpu-mfma-vgpr-form",
     # leading scalar kernel arguments arrive preloaded in SGPRs (gfx950's
     # kernarg preload): a latency-bound launch starts its first loads without
     # waiting for the kernarg segment
@@ -47,11 +49,6 @@ DEVICE_FLAGS = [
 ]
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", f"-I{ROOT / 'include'}",
               f"-I{CSRC}"]
-
-# MFMA results in VGPRs: no accumulator-register reads after every MFMA. (The
-# compiler crashes with it on the widest f32 kernels of these files.)
-MFMA_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-ACCUMULATOR_FORM = {"paged_attend_f32.hip"}
 
 HIP_SOURCES = ["q6k_mv.hip", "q8k.hip", "moe.hip", "moe_decode.hip", "group.hip", "norm.hip",
                "decode.hip", "noalloc.hip", "compat.hip", "paged_store.hip",
@@ -78,7 +75,7 @@ def build_hip(jobs: int = 8) -> Path:
     objs = []
     for src in HIP_SOURCES:
         obj = BUILD / (Path(src).stem + ".o")
-        steps.append([HIPCC, *DEVICE_FLAGS, *([] if src in ACCUMULATOR_FORM else MFMA_FORM), "-c", str(CSRC / src), "-o", str(obj)])
+        steps.append([HIPCC, *DEVICE_FLAGS, "-c", str(CSRC / src), "-o", str(obj)])
         objs.append(obj)
     for src in HOST_HIP_SOURCES:
         obj = BUILD / (Path(src).stem + ".o")

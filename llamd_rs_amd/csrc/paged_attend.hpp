@@ -822,8 +822,8 @@ __global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256
 }
 
 // A decode batch with groups: the first nx * ny workgroups have the tiles of the shared positions, the others the
-// sequences' own, which run beside them (32 sequences, 2000 shared positions and up to 500 of their own: 22 us, two launches
-// 15.5 + 14.5).
+// sequences' own, which run beside them (48 sequences, 4100 shared positions and up to 500 of their own: 22 us; as two
+// launches 15.5 + 14.5).
 template <class E, int HD>
 __global__ __launch_bounds__(256, HD * sizeof(typename E::T) <= 256 ? 2 : 1) void paged_decode(PagedAttendArgs a, Split sp,
                                                                                            int nx, int ny, int cols) {
@@ -1012,7 +1012,10 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
     const long long most = ((long long)p.max_page << p.page_log) / (KT * tile_least<E>());
     Split sp{};
-    sp.parts = fit(want / busy, most, 64);
+    // (f32's steps are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the
+    // workgroups then need two turns; 2048 tokens of 12 heads of 64 take 114 us so, 142 in one turn, 4096 282, 389)
+    const long long turns = E::RUN == 4 ? std::min(2 * want / busy, 4LL) : 0;
+    sp.parts = fit(std::max(want / busy, turns), most, 64);
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * W, 0, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
