@@ -651,12 +651,15 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
 #pragma unroll
             for (int i = 0; i < N; ++i) x[i] = *(const run4 *)(k + i * (THREADS * 16) + tid * 16);
         } else {
+            // (a wave's 64 runs are rows of one page: 64 / KCH rows from a multiple of that)
+            static_assert(64 / KCH <= 16, "a wave's runs in one page");
             const int page = page_or_0(id);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const uint32_t r = (THREADS * i + tid) / KCH, c = tid % KCH;
-                x[i] = *(const run4 *)(g.k + (size_t)__shfl(page, r, WAVE) * g.step +
-                                       (size_t)((t0 + r) & g.mask) * HD + c * RUN);
+                const int r = (THREADS * i + 64 * wave) / KCH;
+                const char *k = (const char *)(g.k + (size_t)__builtin_amdgcn_readlane(page, r) * g.step +
+                                               (size_t)((t0 + r) & g.mask) * HD);
+                x[i] = *(const run4 *)(k + (tid & 63) * 16);
             }
         }
     };
