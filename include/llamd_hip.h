@@ -444,7 +444,8 @@ int llamd_hip_be_get_rows(const float *table, int table_rows, int row_len, const
  * Scores, softmax statistics and sums are f32; weights are rounded to the
  * cache's type for their product with V, the result once at the end. With an
  * f32 cache every product and sum is f32. Results do not depend on timing.
- * Pointers are 16-byte aligned (the integer arrays 4). */
+ * Pointers are 16-byte aligned (the integer arrays 4, freqs 8); results may not
+ * overlap what a call reads. */
 #define LLAMD_HIP_F32 0 /* ggml's type numbers */
 #define LLAMD_HIP_F16 1
 #define LLAMD_HIP_BF16 30

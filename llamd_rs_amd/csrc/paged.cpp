@@ -25,6 +25,15 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
     return x < y + nb && y < x + na;
 }
 
+size_t page_bytes(const llamd_hip_pages *c) {
+    return (size_t)c->n_page * c->n_head_kv * c->page * c->hd * type_bytes(c->type);
+}
+
+// Whether [x, x + n) meets the K or V pages.
+bool meets_pages(const llamd_hip_pages *c, const void *x, size_t n) {
+    return overlap(x, n, c->k, page_bytes(c)) || overlap(x, n, c->v, page_bytes(c));
+}
+
 // The checks that every entry point shares; -1 with the reason.
 int describe(const char *what, const llamd_hip_pages *c, const llamd_hip_batch *b, int n_head, PagedArgs *p) {
     if (!c || !b) return set_error("%s: null descriptor", what);
@@ -41,7 +50,10 @@ int describe(const char *what, const llamd_hip_pages *c, const llamd_hip_batch *
         return set_error("%s: n_seq %d, n_tok %d, max_page %d", what, b->n_seq, b->n_tok, b->max_page);
     if ((long long)b->max_page * c->page > 1 << 30)
         return set_error("%s: tables of %d pages of %d (2^30 positions at most)", what, b->max_page, c->page);
+    if (overlap(c->k, page_bytes(c), c->v, page_bytes(c))) return set_error("%s: K overlaps V", what);
     if (b->n_seq && (!b->len || !b->table)) return set_error("%s: null lengths or table", what);
+    if (((uintptr_t)b->start | (uintptr_t)b->len | (uintptr_t)b->table) & 3)
+        return set_error("%s: starts, lengths and table must be 4-byte aligned", what);
     if (!b->start && b->n_tok < b->n_seq)
         return set_error("%s: %d tokens for %d sequences of one token", what, b->n_tok, b->n_seq);
     p->k = c->k;
@@ -71,6 +83,7 @@ int describe_attend(const char *what, const llamd_hip_pages *c, const llamd_hip_
     const size_t values = (size_t)b->n_tok * n_head * c->hd;
     if (overlap(q, values * type_bytes(c->type), out, values * type_bytes(out_type)))
         return set_error("%s: out overlaps q", what);
+    if (meets_pages(c, out, values * type_bytes(out_type))) return set_error("%s: out overlaps the pages", what);
     a->q = q;
     a->out = out;
     a->out_f32 = out_type == PT_F32;
@@ -126,8 +139,8 @@ int llamd_hip_paged_store(const llamd_hip_pages *c, const llamd_hip_batch *b, co
     const int kv = c->n_head_kv * c->hd;
     if ((q && (ld_q < n_head * c->hd || ld_q % 4)) || ld_k < kv || ld_k % 4 || ld_v < kv || ld_v % 4)
         return set_error("paged_store: row lengths %d, %d, %d (at least the heads', multiples of 4)", ld_q, ld_k, ld_v);
-    if (n_rot < 0 || n_rot > c->hd || n_rot % 2 || (n_rot && !freqs) || (interleaved & ~1))
-        return set_error("paged_store: n_rot %d (even, at most %d, with frequencies), interleaved %d", n_rot, c->hd,
+    if (n_rot < 0 || n_rot > c->hd || n_rot % 2 || (n_rot && !freqs) || ((uintptr_t)freqs & 7) || (interleaved & ~1))
+        return set_error("paged_store: n_rot %d (even, at most %d, with 8-byte aligned frequencies), interleaved %d", n_rot, c->hd,
                          interleaved);
     if (!(eps >= 0.0f) || !isfinite(eps) || !isfinite(mscale))
         return set_error("paged_store: eps %g, mscale %g", (double)eps, (double)mscale);
@@ -137,6 +150,7 @@ int llamd_hip_paged_store(const llamd_hip_pages *c, const llamd_hip_batch *b, co
         if (overlap(q, (rows * ld_q + (size_t)n_head * c->hd) * 4, q_out, n_out) ||
             overlap(k, (rows * ld_k + kv) * 4, q_out, n_out) || overlap(v, (rows * ld_v + kv) * 4, q_out, n_out))
             return set_error("paged_store: q_out overlaps q, k or v");
+        if (meets_pages(c, q_out, n_out)) return set_error("paged_store: q_out overlaps the pages");
     }
     if (!b->n_seq || !b->n_tok) return 0;
     a.x[0] = q;
@@ -173,6 +187,8 @@ int llamd_hip_paged_decode(const llamd_hip_pages *c, const llamd_hip_batch *b, c
         return set_error("paged_decode: %d tokens for %d sequences", b->n_tok, b->n_seq);
     if (n_group < 0 || n_group > b->n_seq || (n_group && (!group || !shared)))
         return set_error("paged_decode: %d groups of %d sequences", n_group, b->n_seq);
+    if (((uintptr_t)group | (uintptr_t)shared) & 3)
+        return set_error("paged_decode: groups must be 4-byte aligned");
     if (!b->n_seq) return 0;
     a.group_at = group;
     a.shared = shared;

@@ -25,28 +25,6 @@ struct ElemBF16 {
     static __device__ __forceinline__ __bf16 put(float x) { return (__bf16)x; }
 };
 
-// The tokens [first, end) of sequence s, inside [0, n_tok] whatever the device array holds.
-struct TokenSpan {
-    int first, end;
-};
-__device__ __forceinline__ TokenSpan token_span(const PagedArgs &p, int s) {
-    TokenSpan t;
-    if (p.start) {
-        t.first = min(max(p.start[s], 0), p.n_tok);
-        t.end = max(min(p.start[s + 1], p.n_tok), t.first);
-    } else {
-        t.first = s;
-        t.end = s + 1;
-    }
-    return t;
-}
-
-// Positions of sequence s that the table can hold.
-__device__ __forceinline__ int held(const PagedArgs &p, int s) {
-    const long long top = (long long)p.max_page << p.page_log;
-    return (int)min((long long)max(p.len[s], 0), min(top, (long long)0x7FFFFFFF));
-}
-
 // The page of a position (inside the table) of a table row, -1 if the id is none of the cache's.
 __device__ __forceinline__ int page_of(const PagedArgs &p, const int32_t *row, int pos) {
     const int id = row[pos >> p.page_log];

@@ -584,8 +584,7 @@ class PagedCache:
               interleaved: bool = False, mscale: float = 1.0) -> np.ndarray:
         """q [n_tok, n_head * hd], k, v [n_tok, n_head_kv * hd]; the rotated q
         (f32 values of the cache's type), k and v in the pages."""
-        n, _, page, hd = self.shape_k
-        kvh = self.shape_k[1]
+        _, kvh, _, hd = self.shape_k
         q, k, v = _f32(q), _f32(k), _f32(v)
         if q.shape[1:] != (self.n_head * hd,) or k.shape != (q.shape[0], kvh * hd) or v.shape != k.shape:
             raise ValueError("q must be [n_tok, n_head * hd], k and v [n_tok, n_head_kv * hd]")

@@ -422,6 +422,193 @@ def test_decode_batch_of_many(gpu, kind):
     R.check(c.decode(q, table, lengths), want, bound)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_decode_not_finite_values_that_a_member_does_not_see(gpu, kind, bad):
+    """Infinities and NaN at shared positions behind a short member's length (the prefix's tiles), and at positions behind
+    a sequence's length in its last page."""
+    rng = np.random.default_rng(36)
+    heads, kvh, hd, page = 8, 2, 64, 32
+    lengths, group, shared = [300, 70, 310, 256, 40], [0, 4], [256]
+    table, n_page, _ = shared_tables(rng, group, shared, lengths, page)
+    c, k, v = filled(gpu, rng, kind, table, n_page, page, heads, kvh, hd, lengths)
+    for pos in (80, 255):
+        v[table[0, pos // page], 0, 3:50:5, pos % page] = bad
+    v[table[0, 280 // page], 1, 7, 280 % page] = bad
+    c.write(k, v)
+    q = rounded(rng.standard_normal((5, heads * hd)), kind)
+    want, bound = want_decode(q, k, v, table, lengths, heads, kvh, hd, hd ** -0.5, kind, group, shared)
+    assert np.isfinite(want[[1, 4]]).all() and not np.isfinite(want[0]).all() and not np.isfinite(want[3]).all()
+    R.check(c.decode(q, table, lengths, group, shared), want, bound)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_decode_many_groups_in_a_large_batch(gpu, kind):
+    """More groups than are looked through one by one, more sequences than a wave has lanes; groups of one and of none,
+    sequences before, between and behind the groups."""
+    rng = np.random.default_rng(37)
+    heads, kvh, hd, page, n = 4, 2, 64, 16, 150
+    sizes = [2, 1, 0, 7, 3, 30, 1, 2, 2, 5, 17, 4, 33, 2, 6]
+    group = [4] + [4 + x for x in np.cumsum(sizes).tolist()]
+    shared = [int(x) for x in rng.integers(0, 120, len(sizes))]
+    lengths = [int(x) for x in rng.integers(0, 60, n)]
+    for g, m in enumerate(shared):
+        for s in range(group[g], group[g + 1]):
+            lengths[s] = m + int(rng.integers(0, 90)) if s % 5 else int(rng.integers(0, 90))
+    for g, m in enumerate(shared):
+        if group[g + 1] > group[g]:
+            lengths[group[g]] = max(lengths[group[g]], m)
+    table, n_page, copies = shared_tables(rng, group, shared, lengths, page)
+    c, k, v = filled(gpu, rng, kind, table, n_page, page, heads, kvh, hd, lengths)
+    for to, of, m in copies:
+        k[to, :, :m], v[to, :, :, :m] = k[of, :, :m], v[of, :, :, :m]
+    c.write(k, v)
+    q = rounded(rng.standard_normal((n, heads * hd)) * 1.5, kind)
+    want, bound = want_decode(q, k, v, table, lengths, heads, kvh, hd, hd ** -0.5, kind, group, shared)
+    R.check(c.decode(q, table, lengths, group, shared), want, bound)
+
+
+# ---- large calls --------------------------------------------------------------------
+
+def some_prompt_rows(c, q, k, v, table, lengths, start, heads, kvh, hd, kind, picked):
+    """Results of the picked tokens of a prompt batch against the restatement."""
+    got = c.prompt(q, table, lengths, start)
+    page = k.shape[2]
+    for s, n in enumerate(lengths):
+        rows = np.array([t for t in picked if start[s] <= t < start[s + 1]])
+        if not len(rows):
+            continue
+        at = np.arange(n)
+        ids = table[s][at // page]
+        limits = n - (start[s + 1] - rows) + 1
+        want, bound = R.attend(q[rows].reshape(-1, heads, hd), k[ids, :, at % page], v[ids, :, :, at % page], limits,
+                               hd ** -0.5, kind)
+        R.check(got[rows], want.reshape(len(rows), -1), bound.reshape(len(rows), -1), s)
+
+
+@pytest.mark.parametrize("kind,heads,kvh,hd,page,new,old", [
+    ("bf16", 32, 4, 128, 64, [5000], [0]), ("f16", 32, 8, 64, 16, [4200], [77]), ("f32", 40, 20, 64, 32, [3700], [5]),
+    ("bf16", 64, 8, 128, 128, [1100, 1300], [900, 0]), ("f16", 16, 2, 256, 64, [2100], [0]),
+    ("f32", 12, 12, 64, 64, [2050], [0]), ("f32", 8, 1, 256, 16, [900], [300])])
+def test_prompt_of_thousands(gpu, kind, heads, kvh, hd, page, new, old):
+    rng = np.random.default_rng(51)
+    lengths = [a + b for a, b in zip(new, old)]
+    table, n_page = tables(rng, lengths, page)
+    start = np.concatenate([[0], np.cumsum(new)])
+    c, k, v = filled(gpu, rng, kind, table, n_page, page, heads, kvh, hd, lengths)
+    q = rounded(rng.standard_normal((start[-1], heads * hd)) * 1.5, kind)
+    edges = [0, 1, 31, 32, 63, 64, 127, start[-1] - 1, start[-1] - 2, start[-1] // 2] + [int(x) for x in start[1:-1]]
+    picked = sorted(set(edges + rng.integers(0, start[-1], 8).tolist()))
+    some_prompt_rows(c, q, k, v, table, lengths, start, heads, kvh, hd, kind, picked)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_prompt_of_many_long_sequences(gpu, kind):
+    """More sequences than a wave has lanes, with enough rows each for the tiles; one without tokens, one of one."""
+    rng = np.random.default_rng(52)
+    heads, kvh, hd, page = 16, 1, 64, 32
+    new = [int(x) for x in rng.integers(5, 40, 70)]
+    new[3], new[66] = 0, 1
+    lengths = [a + int(b) for a, b in zip(new, rng.integers(0, 300, 70))]
+    table, n_page = tables(rng, lengths, page)
+    start = np.concatenate([[0], np.cumsum(new)])
+    c, k, v = filled(gpu, rng, kind, table, n_page, page, heads, kvh, hd, lengths)
+    q = rounded(rng.standard_normal((start[-1], heads * hd)), kind)
+    picked = sorted(set([int(x) for x in start[:-1] if x < start[-1]] + rng.integers(0, start[-1], 30).tolist()))
+    some_prompt_rows(c, q, k, v, table, lengths, start, heads, kvh, hd, kind, picked)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n_rot,interleaved", [(64, False), (128, True), (20, True)])
+def test_store_of_thousands(gpu, kind, n_rot, interleaved):
+    """2300 tokens in 5 sequences: one wave per token, and values over many blocks of positions."""
+    rng = np.random.default_rng(53)
+    heads, kvh, hd, page = 4, 2, 128, 32
+    new, old = [1200, 0, 1, 1000, 99], [3, 9, 31, 17, 0]
+    lengths = [a + b for a, b in zip(new, old)]
+    table, n_page = tables(rng, lengths, page)
+    start = np.concatenate([[0], np.cumsum(new)])
+    n = int(start[-1])
+    q, k, v = (rng.standard_normal((n, h * hd)).astype(np.float32) for h in (heads, kvh, kvh))
+    freqs, m = gpu.rope_freqs(n_rot, 10000.0)
+    w = (1 + 0.2 * rng.standard_normal(hd)).astype(np.float32)
+    c = gpu.PagedCache(kind, n_page, page, heads, kvh, hd)
+    got = c.store(q, k, v, table, lengths, start, w, w, 1e-6, freqs, interleaved, m)
+    got_k, got_v = c.read()
+    want_k, bound_k, want_v = np.zeros(c.shape_k), np.zeros(c.shape_k), np.zeros(c.shape_v)
+    for s in range(5):
+        rows, pos = slice(start[s], start[s + 1]), np.arange(old[s], lengths[s])
+        if not len(pos):
+            continue
+        want, bound = R.store(q[rows].reshape(-1, heads, hd), w, pos, freqs, n_rot, interleaved, m, 1e-6, kind)
+        R.check(got[rows], want.reshape(len(pos), -1), bound.reshape(len(pos), -1), s)
+        ids, slots = table[s][pos // page], pos % page
+        want_k[ids, :, slots], bound_k[ids, :, slots] = R.store(k[rows].reshape(-1, kvh, hd), w, pos, freqs, n_rot,
+                                                                interleaved, m, 1e-6, kind)
+        want_v[ids, :, :, slots] = rounded(v[rows].reshape(-1, kvh, hd), kind)
+    R.check(got_k, want_k, bound_k, "k")
+    assert np.array_equal(got_v, want_v.astype(np.float32))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_pages_past_32_bits(gpu, kind):
+    """A cache of more than 2^32 elements: the same tokens at its far end and in a small cache give the same bits."""
+    rng = np.random.default_rng(54)
+    L, heads, kvh, hd, page = gpu.lib(), 8, 8, 256, 256
+    size = 4 if kind == "f32" else 2
+    n_page = 2 ** 32 // (kvh * hd * page) + 9
+    total = n_page * kvh * hd * page * size
+    far_k, far_v = gpu.DeviceBuffer(total), gpu.DeviceBuffer(total)
+    near = gpu.PagedCache(kind, 9, page, heads, kvh, hd)
+    far = gpu.Pages(far_k.ptr, far_v.ptr, near.pages.type, n_page, page, kvh, hd)
+    lengths, start = [300, 700], [0, 300, 1000]
+    table = np.array([[0, 1, -1], [7, 3, 5]], np.int32)
+    freqs, _ = gpu.rope_freqs(hd, 1e6)
+    x = [gpu.DeviceBuffer.from_array(rng.standard_normal((1000, h * hd)).astype(np.float32)) for h in (heads, kvh, kvh)]
+    f = gpu.DeviceBuffer.from_array(freqs)
+    got = []
+    for pages, ids in ((near.pages, table), (far, np.where(table < 0, -1, table + n_page - 9).astype(np.int32))):
+        t, o, d = (gpu.DeviceBuffer.from_array(np.zeros((1000, heads * hd), near.dtype)) for _ in range(3))
+        b, keep = near._batch(ids, lengths, start, 1000)
+        P, B = C.byref(pages), C.byref(b)
+        assert L.llamd_hip_paged_store(P, B, x[0].ptr, heads * hd, x[1].ptr, kvh * hd, x[2].ptr, kvh * hd, None, None, 1e-6,
+                                       f.ptr, hd, 0, 1.0, heads, t.ptr) == 0
+        assert L.llamd_hip_paged_prompt(P, B, t.ptr, heads, hd ** -0.5, near.pages.type, o.ptr) == 0
+        assert L.llamd_hip_paged_decode(P, B, None, None, 0, t.ptr, heads, hd ** -0.5, near.pages.type, d.ptr) == 0
+        got.append([y.download(np.empty((1000, heads * hd), near.dtype)) for y in (t, o, d)])
+    assert got[0][1].any() and got[0][2][:2].any()
+    assert all(np.array_equal(a, b) for a, b in zip(*got))
+    far_k.close(), far_v.close()
+
+
+def test_calls_from_two_threads(gpu):
+    """Calls of different sizes from two threads share the library's scratch: each gets what it gets alone."""
+    import threading
+    rng = np.random.default_rng(55)
+    heads, kvh, hd, page = 8, 1, 64, 16
+    jobs = []
+    for lengths, new in (([900, 3000], 1), ([700], 90)):
+        table, n_page = tables(rng, lengths, page)
+        c, _, _ = filled(gpu, rng, "bf16", table, n_page, page, heads, kvh, hd, lengths)
+        q = rounded(rng.standard_normal((new * len(lengths), heads * hd)), "bf16")
+        jobs.append((lambda c=c, q=q, t=table, n=lengths: c.decode(q, t, n)) if new == 1 else
+                    (lambda c=c, q=q, t=table, n=lengths, m=new: c.prompt(q, t, n, [0, m])))
+    alone = [j() for j in jobs]
+    seen = [[], []]
+
+    def run(i):
+        for _ in range(12):
+            seen[i].append(jobs[i]())
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(seen[i]) == 12 and all(np.array_equal(x, alone[i]) for x in seen[i])
+
+
 # ---- together ---------------------------------------------------------------------
 
 def run_calls(gpu, c, b, dev, heads, hd, group=None):

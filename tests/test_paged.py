@@ -72,6 +72,18 @@ def test_refused_decode(batch, kw):
     assert "paged_decode" in last_error()
 
 
+@pytest.mark.parametrize("name,pages,batch,kw", [
+    ("store", {}, {}, dict(out=(1 << 20) + 4096)), ("store", {}, {}, dict(out=(2 << 20) - 64)),
+    ("store", {}, {}, dict(freqs=4 * FAR + 4)), ("store", {}, dict(start=(3 << 20) + 2), {}),
+    ("prompt", {}, {}, dict(out=(1 << 20) + 4096)), ("prompt", {}, dict(table=(5 << 20) + 1), {}),
+    ("prompt", dict(v=(1 << 20) + 1024), {}, {}), ("decode", {}, {}, dict(out=(2 << 20) + (1 << 19) - 16)),
+    ("decode", {}, dict(len=(4 << 20) + 2), {}), ("decode", {}, {}, dict(group=FAR + 2, shared=2 * FAR, n_group=1, out=3 * FAR)),
+    ("decode", dict(k=2 << 20), {}, {})])
+def test_refused_overlaps_and_alignments(name, pages, batch, kw):
+    assert call(name, pages, batch, **kw) == -1
+    assert "paged_" + name in last_error()
+
+
 def test_null_descriptors_and_empty_batches():
     c, b = rocm.Pages(**GOOD_PAGES), rocm.Batch(**GOOD_BATCH)
     L = lib()
