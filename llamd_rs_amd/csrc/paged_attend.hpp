@@ -35,7 +35,8 @@ struct Parts {
 struct Split {
     Parts many, few;     // of paged_tiles (blocks of 32 rows) and of paged_few
     int parts;           // most parts of a row tile (prompt, prefix)
-    double per_item;     // decode: 1 / (positions' steps per workgroup wanted)
+    double per_item;     // decode: 1 / (positions of all sequences' parts wanted, in steps)
+    double per_row;      // decode: 1 / (parts of a sequence, in steps, while they are short)
 };
 
 // ---- rows ------------------------------------------------------------------------
@@ -374,8 +375,10 @@ __device__ __forceinline__ void attend_again(const PagedAttendArgs &a, const Par
     }
 }
 
-// Least positions of a part of paged_few: one step of each wave.
-constexpr int FEW_STEP = 128;
+// Least positions of a part of paged_few: one step of each wave. A sequence has no more than FEW_PARTS parts (each costs the
+// join) unless they would have more than LONG_PART steps (1 x 9000 positions: 17 us, in 71 parts 19.4; 1 x 60000: 35 us in
+// 118 parts, in 64 43).
+constexpr int FEW_STEP = 128, FEW_PARTS = 64, LONG_PART = 4;
 
 // A sequence's own positions in a decode batch (behind those that its group shares), cut into parts.
 struct Own {
@@ -404,10 +407,17 @@ __device__ __forceinline__ DecodePlan decode_plan(const PagedAttendArgs &a, cons
     const int lane = threadIdx.x & 63;
     DecodePlan d;
     d.mine = own_of(a, lane);
-    double sum = (double)d.mine.tail();  // exact
-    for (int s = lane + WAVE; s < a.p.n_seq; s += WAVE) sum += (double)own_of(a, s).tail();
+    int most = d.mine.tail();
+    double sum = (double)most;  // exact
+    for (int s = lane + WAVE; s < a.p.n_seq; s += WAVE) {
+        const int n = own_of(a, s).tail();
+        sum += (double)n;
+        most = max(most, n);
+    }
+    most = wave_reduce(most, 0, [](int x, int y) { return max(x, y); });
     // (2^31 - 128 at most: one part)
-    d.cut = (int)min(max(ceil(wave_sum_d(sum) * sp.per_item), 1.0) * FEW_STEP, 2147483520.0);
+    const double row = min(most * sp.per_row, (double)LONG_PART);
+    d.cut = (int)min(max(ceil(max(wave_sum_d(sum) * sp.per_item, row)), 1.0) * FEW_STEP, 2147483520.0);
     return d;
 }
 // The sequence of part number `part` (its number within the sequence afterwards); -1: past the last.
@@ -544,7 +554,14 @@ __device__ __forceinline__ void few_rows(const PagedAttendArgs &a, const Split &
 template <class E, int HD, bool DECODE>
 __global__ __launch_bounds__(256, E::RUN == 4 && HD <= 128 ? 3 : 1) void paged_few(PagedAttendArgs a, Split sp) {
     __shared__ __align__(16) FewShared<HD> shared;
-    few_rows<E, HD, DECODE>(a, sp, {(int)blockIdx.x, (int)blockIdx.y, (int)gridDim.x, (int)gridDim.y}, shared);
+    const int at = blockIdx.x, nx = gridDim.x;
+    if constexpr (DECODE) {
+        // all columns of a part together: parts that there are not come last (1 x 20000 positions: 25 us, first 20)
+        const int cols = a.p.n_kv_head * ((a.p.group + 15) / 16);
+        few_rows<E, HD, DECODE>(a, sp, {at / cols, at % cols, nx / cols, cols}, shared);
+    } else {
+        few_rows<E, HD, DECODE>(a, sp, {at, (int)blockIdx.y, nx, (int)gridDim.y}, shared);
+    }
 }
 
 // ---- many rows -------------------------------------------------------------------
@@ -574,6 +591,14 @@ template <class E, int HD> __host__ __device__ constexpr int tile_positions() {
     return HD * sizeof(typename E::T) <= 512 ? 64 : 32;
 }
 template <class E> __host__ __device__ constexpr int tile_least() { return E::RUN == 8 ? 4 : 1; }
+// ... of a part of a shared prefix, whose rows are few (48 sequences behind 4100 positions: 28.6 us, with 4 steps 30.9), and
+// the most tiles that a prompt's rows are not split for: the join costs as much (512 tokens 22 us, in two parts 27; 1024 33,
+// in four 41).
+template <class E> __host__ __device__ constexpr int prefix_least() { return E::RUN == 8 ? 8 : 1; }
+template <class E> __host__ __device__ constexpr int whole_steps() { return E::RUN == 8 ? 16 : 1; }
+template <class E> __device__ __forceinline__ int prompt_parts(int steps, int most) {
+    return steps <= whole_steps<E>() ? 1 : parts_of(steps, most, tile_least<E>());
+}
 
 template <class E, int HD> struct TileShared {
     run4 lds[2][2][tile_positions<E, HD>() * HD / E::RUN];  // two buffers of K and V
@@ -607,7 +632,8 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
         if (!prompt_tile_by_size<R, KT == 64 ? 6 : 5>(p, unit, at.nx / p.n_kv_head, unit, tile, t)) return;
         row = prompt_row<R>(p, tile, t, kvh, 32 * wave + m);
     }
-    const int steps = (t.top + KT - 1) / KT, parts = parts_of(steps, sp.parts, tile_least<E>());
+    const int steps = (t.top + KT - 1) / KT, parts = PREFIX ? parts_of(steps, sp.parts, prefix_least<E>())
+                                                    : prompt_parts<E>(steps, sp.parts);
     if (at.y >= parts) return;
     const int2 range = part_steps(steps, parts, at.y);
     // positions that all rows attend to, and that any of this wave's does
@@ -930,7 +956,7 @@ __global__ __launch_bounds__(256) void paged_join(PagedAttendArgs a, Split sp) {
     int tile = unit;
     Tile t;
     if (!prompt_tile<R>(p, tile, t)) return;
-    const int parts = parts_of((t.top + STEP - 1) / STEP, sp.parts, FEW ? 1 : tile_least<E>());
+    const int steps = (t.top + STEP - 1) / STEP, parts = FEW ? parts_of(steps, sp.parts, 1) : prompt_parts<E>(steps, sp.parts);
     const int first = 16 * blockIdx.y;
     if (parts < 2 || first >= t.rows) return;
     const Parts x = FEW ? sp.few : sp.many;
@@ -963,7 +989,7 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
         for (int i = lane; i < number; i += WAVE) tiles += prefix_units<R>(a, group_at(a, i));
         base = wave_reduce(tiles, 0, [](int x, int y) { return x + y; });
         constexpr int KT = tile_positions<E, HD>();
-        parts = parts_of((readable_of(p, g.shared) + KT - 1) / KT, sp.parts, tile_least<E>());
+        parts = parts_of((readable_of(p, g.shared) + KT - 1) / KT, sp.parts, prefix_least<E>());
         first = (long long)(seq - g.first) * p.group + head;
     }
     const auto many = [&](int z, int r) {  // the slot of a row's 32-row block
@@ -1013,7 +1039,8 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     constexpr int R = 32 * W, KT = tile_positions<E, HD>();
     const long long rows = (long long)p.n_tok * p.group, tiles = rows / R + p.n_seq;
     const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
-    const long long most = ((long long)p.max_page << p.page_log) / (KT * tile_least<E>());
+    const long long top = (long long)p.max_page << p.page_log;
+    const long long most = top <= KT * whole_steps<E>() ? 1 : top / (KT * tile_least<E>());
     Split sp{};
     // (f32's steps are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the
     // workgroups then need two turns; 2048 tokens of 12 heads of 64 take 114 us so, 142 in one turn, 4096 282, 389)
@@ -1051,8 +1078,8 @@ int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
     const long long total = (long long)p.n_tok * p.group, rows = total / p.n_seq;  // and of a sequence, on average
     const long long top = (long long)p.max_page << p.page_log;
-    // few rows per sequence, or not enough of them to fill the GPU and short contexts: 16 rows at a time
-    if (rows <= 64 || (total * p.n_kv_head <= 64 * 128 && top <= 512)) return prompt_few<E, HD>(a, st);
+    // few rows per sequence, or little work in all, which 16-row tiles spread further
+    if (rows <= 64 || total * p.n_kv_head * top <= 3 << 20) return prompt_few<E, HD>(a, st);
     if constexpr (wide<E, HD>())
         if (rows >= 1024 && total * p.n_kv_head >= 512 * 256) return prompt_tiles<E, HD, 8>(a, st);
     return prompt_tiles<E, HD, 4>(a, st);
@@ -1065,9 +1092,11 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
     const int per = (p.group + 15) / 16, cols = p.n_kv_head * per;
     const long long top = (long long)p.max_page << p.page_log;
     Split sp{};
-    // parts of the sequences' own positions: 4 workgroups per CU, one part per sequence at least, JOIN_MOST of a row at most
+    // parts of the sequences' own positions: 4 workgroups per CU, one part per sequence at least; a row's should fill the GPU
+    // once where there are few columns
     const int target = std::min(std::max(1, 4 * CUS / cols), JOIN_MOST - 66);
     sp.per_item = 1.0 / ((double)target * FEW_STEP);
+    sp.per_row = 1.0 / ((double)std::max(FEW_PARTS, CUS / cols) * FEW_STEP);
     const long long items = std::min<long long>((long long)p.n_seq + target + 1,
                                                 (long long)p.n_seq * ((top + FEW_STEP - 1) / FEW_STEP));
     long long tiles = 0, slots = 0;
@@ -1075,10 +1104,10 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
         const long long rows = (long long)p.n_seq * p.group;
         tiles = rows / R + a.n_groups;
         const long long busy = (rows + R - 1) / R * p.n_kv_head, want = 2 * CUS;
-        sp.parts = fit(want / busy, top / (KT * tile_least<E>()), 64);
+        sp.parts = fit(want / busy, top / (KT * prefix_least<E>()), 64);
         slots = tiles * p.n_kv_head * sp.parts * 4;
     }
-    if (items > 0x7FFFFFFF / 512 || cols > 65535 || tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
+    if (items * cols > 0x7FFFFFFF / 512 || cols > 65535 || tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     const bool join = a.n_groups || top > FEW_STEP;
     if (join && !room(sp, slots, (size_t)items * cols, std::min(p.group, 16), HD)) return -1;
     if (a.n_groups) {
@@ -1086,7 +1115,7 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
         if (grid > 0x7FFFFFFF / 512) return -1;
         hipLaunchKernelGGL((paged_decode<E, HD>), dim3((unsigned)grid), dim3(256), 0, st, a, sp, (int)nx, sp.parts, cols);
     } else {
-        hipLaunchKernelGGL((paged_few<E, HD, true>), dim3((unsigned)items, cols), dim3(256), 0, st, a, sp);
+        hipLaunchKernelGGL((paged_few<E, HD, true>), dim3((unsigned)(items * cols)), dim3(256), 0, st, a, sp);
     }
     if (join) {
         const dim3 grid(p.n_seq, cols, HD / 32);

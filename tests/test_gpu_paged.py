@@ -339,6 +339,19 @@ def test_decode(gpu, kind, heads, kvh, hd, page, lengths):
     assert not got[-1].any()   # the row behind the last sequence
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kvh,page,lengths", [
+    (8, 1, 256, [26_000]), (4, 4, 64, [11_000, 0, 3, 40_000]), (20, 1, 128, [9_000, 130]), (16, 8, 32, [8_321, 8_320, 8_193])])
+def test_decode_long(gpu, kind, heads, kvh, page, lengths):
+    """As many parts of a row as there may be, and parts of several steps."""
+    rng = np.random.default_rng(38)
+    table, n_page = tables(rng, lengths, page)
+    c, k, v = filled(gpu, rng, kind, table, n_page, page, heads, kvh, 64, lengths)
+    q = rounded(rng.standard_normal((len(lengths), heads * 64)) * 1.5, kind)
+    want, bound = want_decode(q, k, v, table, lengths, heads, kvh, 64, 0.125, kind)
+    R.check(c.decode(q, table, lengths), want, bound)
+
+
 def shared_tables(rng, group, shared, lengths, page):
     """Tables whose groups share the pages that their prefix fills; (table, n_page, pages that copies are made of)."""
     table, n_page = tables(rng, lengths, page)
