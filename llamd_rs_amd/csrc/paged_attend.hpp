@@ -7,10 +7,16 @@
 // takes consecutive ones: with 8 query heads per kv head, a tile of 256 rows is 32 tokens, whose keys and values are
 // read once for all 8.
 //
-// Two kernels form O. paged_tiles: many rows; the waves of a workgroup have 32 rows of their own each and share K and V
-// tiles in LDS. paged_few: up to 16 rows; the waves share the rows and have positions of their own, read straight into the
+// Two ways to form O. tile_rows: many rows; the waves of a workgroup have 32 rows of their own each and share K and V
+// tiles in LDS. few_rows: up to 16 rows; the waves share the rows and have positions of their own, read straight into the
 // matrix operands. Either may have a part of a row's positions only; then O (unnormalised), the maximum and the sum
-// go to scratch and paged_join or paged_join_decode puts the parts together.
+// go to scratch and paged_join or paged_join_decode puts the parts together, in a fixed order.
+//
+// Bound and measured (32 query heads on 4 kv heads of 128, one MI355X). Long prompts: the matrix cores, 975 TFLOP/s of the
+// causal half at 8192 tokens of bf16 (564 us; a library product of 8192^3 reaches 1349, both at the clock that the power
+// leaves); f32 110 to 119 of 154. Pieces and packed prompts: the steps of the longest tile in a row, 1.1 us each, behind 9
+// us to its first product (512 tokens after 7000 85 us, 9 prompts of up to 1400 43). Decode: memory, then the chain
+// length -> table -> keys and the second launch (1 x 4100 13.3 us, 13 x 1000 in f32 20.6, 48 behind 4100 shared 26.5).
 #pragma once
 
 #include <algorithm>
@@ -1042,6 +1048,7 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const long long top = (long long)p.max_page << p.page_log;
     const long long most = top <= KT * whole_steps<E>() ? 1 : top / (KT * tile_least<E>());
     Split sp{};
+    // parts for two workgroups per CU (512 tokens after 7000: 91 us, for four 98, in one part 163).
     // (f32's steps are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the
     // workgroups then need two turns; 2048 tokens of 12 heads of 64 take 114 us so, 142 in one turn, 4096 282, 389)
     const long long turns = E::RUN == 4 ? std::min(2 * want / busy, 4LL) : 0;
@@ -1078,8 +1085,11 @@ int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
     const long long total = (long long)p.n_tok * p.group, rows = total / p.n_seq;  // and of a sequence, on average
     const long long top = (long long)p.max_page << p.page_log;
-    // few rows per sequence, or little work in all, which 16-row tiles spread further
+    // few rows per sequence, or little work in all, which 16-row tiles spread further (single calls, 32 query and 4 kv heads:
+    // 45 tokens 8.8 us, with larger tiles 11.6; 6 x up to 16 after 500 positions, 2 M rows x positions, 19 and 25; 24 x up
+    // to 16 after 1000, 8 M, 39 and 32)
     if (rows <= 64 || total * p.n_kv_head * top <= 3 << 20) return prompt_few<E, HD>(a, st);
+    // eight waves where all CUs still have work (32 query heads on 4: 4096 tokens 175 us, four waves 195; 3000 110 and 101)
     if constexpr (wide<E, HD>())
         if (rows >= 1024 && total * p.n_kv_head >= 512 * 256) return prompt_tiles<E, HD, 8>(a, st);
     return prompt_tiles<E, HD, 4>(a, st);
@@ -1092,8 +1102,8 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
     const int per = (p.group + 15) / 16, cols = p.n_kv_head * per;
     const long long top = (long long)p.max_page << p.page_log;
     Split sp{};
-    // parts of the sequences' own positions: 4 workgroups per CU, one part per sequence at least; a row's should fill the GPU
-    // once where there are few columns
+    // parts of the sequences' own positions: 4 workgroups per CU, one part per sequence at least (64 x 2000 positions: 44 us,
+    // 2 per CU 51, 1 per CU 50); a row's should fill the GPU once where there are few columns
     const int target = std::min(std::max(1, 4 * CUS / cols), JOIN_MOST - 66);
     sp.per_item = 1.0 / ((double)target * FEW_STEP);
     sp.per_row = 1.0 / ((double)std::max(FEW_PARTS, CUS / cols) * FEW_STEP);
