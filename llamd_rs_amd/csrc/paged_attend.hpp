@@ -41,6 +41,7 @@ struct Parts {
 struct Split {
     Parts many, few;     // of paged_tiles (blocks of 32 rows) and of paged_few
     int parts;           // most parts of a row tile (prompt, prefix)
+    int tiles;           // decode: tiles of shared prefixes that there are slots for
     double per_item;     // decode: 1 / (positions of all sequences' parts wanted, in steps)
     double per_row;      // decode: 1 / (parts of a sequence, in steps, while they are short)
 };
@@ -149,6 +150,7 @@ __device__ __forceinline__ bool prompt_tile_by_size(const PagedArgs &p, int orde
     // of a sequence's tiles, the last `above` have more
     tile = __builtin_amdgcn_readlane(tiles - above, l) - 1 - at;
     unit = __builtin_amdgcn_readlane(wave_incl_sum_i(tiles) - tiles, l) + tile;
+    if (unit >= n_units) return false;  // starts that descend: sequences over the same tokens, more tiles than there are slots
     t.seq = l;
     t.first = __builtin_amdgcn_readlane(first, l);
     t.end = __builtin_amdgcn_readlane(end, l);
@@ -1000,8 +1002,9 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
     }
     const auto many = [&](int z, int r) {  // the slot of a row's 32-row block
         const long long x = first + r;
-        return (((size_t)base + (size_t)(x / R)) * p.n_kv_head + kvh) * sp.parts * (R / 32) + (size_t)z * (R / 32) +
-               (size_t)(x % R) / 32;
+        // (starts of groups that descend: more tiles than slots)
+        const size_t tile = (size_t)min((long long)base + x / R, (long long)sp.tiles - 1);
+        return (tile * p.n_kv_head + kvh) * sp.parts * (R / 32) + (size_t)z * (R / 32) + (size_t)(x % R) / 32;
     };
     const auto few = [&](int z) { return (size_t)(before + z - parts) * gridDim.y + blockIdx.y; };
     const int w = sp.few.rows;
@@ -1115,6 +1118,7 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
         tiles = rows / R + a.n_groups;
         const long long busy = (rows + R - 1) / R * p.n_kv_head, want = 2 * CUS;
         sp.parts = fit(want / busy, top / (KT * prefix_least<E>()), 64);
+        sp.tiles = (int)tiles;
         slots = tiles * p.n_kv_head * sp.parts * 4;
     }
     if (items * cols > 0x7FFFFFFF / 512 || cols > 65535 || tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;

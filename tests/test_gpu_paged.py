@@ -481,6 +481,26 @@ def test_decode_many_groups_in_a_large_batch(gpu, kind):
     R.check(c.decode(q, table, lengths, group, shared), want, bound)
 
 
+def test_starts_and_groups_over_the_same_rows(gpu):
+    """Starts (of sequences, of groups) that go back to 0 again and again claim more tiles than the rows make: nothing past
+    the rows or the scratch is touched, and the calls after that are right."""
+    rng = np.random.default_rng(39)
+    heads, kvh, hd, page, n = 16, 1, 64, 16, 20
+    lengths = [1500] * n
+    table, n_page = tables(rng, lengths[:1], page)
+    c, k, v = filled(gpu, rng, "bf16", table, n_page, page, heads, kvh, hd, lengths[:1])
+    q = rounded(rng.standard_normal((100, heads * hd)), "bf16")
+    many = np.repeat(table, n, 0)
+    got = c.prompt(q, many, lengths, [0, 90] * (n // 2) + [0])
+    assert not got[90:].any()
+    got = c.decode(q[:n], many, lengths, [0, n] * (n // 2) + [0], [1400] * n)
+    got = c.decode(q[:n], many, lengths, [0, n] * 3, [1400] * 5)
+    want, bound = want_prompt(q, k, v, table, [1500], [0, 90], heads, kvh, hd, hd ** -0.5, "bf16")
+    R.check(c.prompt(q, table, [1500], [0, 90])[:90], want[:90], bound[:90])
+    want, bound = want_decode(q[:n], k, v, many, lengths, heads, kvh, hd, hd ** -0.5, "bf16", [0, n], [1400])
+    R.check(c.decode(q[:n], many, lengths, [0, n], [1400]), want, bound)
+
+
 # ---- large calls --------------------------------------------------------------------
 
 def some_prompt_rows(c, q, k, v, table, lengths, start, heads, kvh, hd, kind, picked):
