@@ -266,6 +266,13 @@ template <class E> __device__ __forceinline__ void put_out(void *out, bool f32, 
 
 // ---- up to 16 rows -----------------------------------------------------------------
 
+// x, as something that the compiler cannot keep the results of between tiles: addresses are cheaper made again than held
+// in registers.
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // A row's runs for the first product of 16 rows.
 template <class E, int HD>
 __device__ __forceinline__ void load_few(run4 (&q)[HD / (4 * E::RUN)], const void *from, long long at) {
@@ -277,17 +284,18 @@ __device__ __forceinline__ void load_few(run4 (&q)[HD / (4 * E::RUN)], const voi
 
 // 16 rows against the positions t0 .. t0 + 31 for t0 = begin, begin + STRIDE, ... below end; begin and STRIDE are multiples of
 // 32, uniform over the wave. K of a step (and V, where the registers allow) is loaded whole before the first product.
-template <class E, int HD, int STRIDE>
+template <class E, int HD, int STRIDE, bool AGAIN = false>
 __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &pg, int n_kv, int limit, int begin, int end,
                                            const run4 (&q)[HD / (4 * E::RUN)], float scale, FewState<E, HD> &st) {
     typedef typename E::T T;
     typedef FewState<E, HD> S;
     constexpr int RUN = E::RUN;
     constexpr bool EARLY = HD * sizeof(T) <= 512;
-    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
     const int all = wave_reduce(limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
     // a step; false, with nothing done, if it is not `masked` and some position in it cannot be read
     const auto step = [&](auto masked, int t0) {
+        // (AGAIN: few registers are left, so addresses are made again every step)
+        const int lane = (AGAIN ? fresh(threadIdx.x) : threadIdx.x) & 63, g = lane >> 4, m = lane & 15;
         // the pages of the two halves of the step
         const int id0 = pg.table[min(t0, n_kv - 1) >> p.page_log], id1 = pg.table[min(t0 + 16, n_kv - 1) >> p.page_log];
         const bool ok0 = (unsigned)id0 < (unsigned)p.n_page, ok1 = (unsigned)id1 < (unsigned)p.n_page;
@@ -348,7 +356,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
     };
     // steps that all rows see whole, then the others
     int t0 = begin;
-    while (t0 < end && t0 + 32 <= all && step(std::false_type{}, t0)) t0 += STRIDE;
+    while (!AGAIN && t0 < end && t0 + 32 <= all && step(std::false_type{}, t0)) t0 += STRIDE;
     for (; t0 < end; t0 += STRIDE) step(std::true_type{}, t0);
 }
 
@@ -367,7 +375,7 @@ __device__ __forceinline__ void attend_again(const PagedAttendArgs &a, const Par
         load_few<E, HD>(q, a.q, row);
         FewState<E, HD> st;
         st.clear();
-        attend_few<E, HD, 32>(a.p, pages_of<E, HD>(a.p, seq, kvh), n_kv, lim, begin, end, q, a.scale, st);
+        attend_few<E, HD, 32, true>(a.p, pages_of<E, HD>(a.p, seq, kvh), n_kv, lim, begin, end, q, a.scale, st);
         const float l = add_groups(st.l), f = over(l);
         if (part) {
             if (g == 0) parts.ml[slot * 32 + from] = make_float2(st.m, l);
@@ -574,13 +582,6 @@ __global__ __launch_bounds__(256, E::RUN == 4 && HD <= 128 ? 3 : 1) void paged_f
 
 // ---- many rows -------------------------------------------------------------------
 
-// x, as something that the compiler cannot keep the results of between tiles: addresses are cheaper made again than held
-// in registers.
-__device__ __forceinline__ uint32_t fresh(uint32_t x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-
 // Asks the scheduler for N reads of a block's operands 6 ahead of their products (left alone it places each right before
 // its product, which then waits for LDS every time).
 template <class E, int N> __device__ __forceinline__ void order_reads() {
@@ -729,12 +730,19 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
             to[r * KCH + ((tid % KCH) ^ k_swap(r))] = x[i];
         }
     };
+    // (a position that a row does not attend to weighs nothing, whatever lies there; but nothing times an infinity or NaN
+    // is NaN: where some row does not see all of a tile that has one, the rows are done again, attend_again)
+    uint32_t bad = 0;
     const auto put_v = [&](run4 (&x)[N], int step, unsigned long long valid) {
         run4 *to = lds[step & 1][1];
         const uint32_t tid = fresh(threadIdx.x);
         if (valid != ~0ull) {
 #pragma unroll
             for (int i = 0; i < N; ++i) x[i] = keep_elements<E>(x[i], (uint32_t)(valid >> (tid % VCH * RUN)));
+        }
+        if ((step + 1) * KT > all) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) bad |= any_not_finite<E>(x[i]);
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -743,7 +751,6 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
         }
     };
 
-    bool again = false;
     if (range.x < range.y) {
         const int last = range.y - 1;
         run4 kr[N], vr[N];
@@ -794,19 +801,17 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(0);
                 if constexpr (masked) {
-                    // a position that a row does not attend to weighs nothing, whatever lies there; but nothing times an
-                    // infinity or NaN is NaN: where V has one, these rows are done again (attend_again)
+                    // bit 32 b + kv_reg(i, 0): the row attends to that register's position
+                    const int seen = row.limit - t0;
+                    unsigned long long mask = seen >= 64 ? valid : seen > 0 ? valid & ((1ull << seen) - 1) : 0ull;
+                    if (__any(mask != ~0ull)) {
+                        mask >>= RUN * h;
 #pragma unroll
-                    for (int b = 0; b < SUB; ++b)
+                        for (int b = 0; b < SUB; ++b)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int at = 32 * b + kv_reg<E>(i, h);
-                            s[b][i] = t0 + at < row.limit && (valid >> at & 1) ? s[b][i] : NEG_INF;
-                        }
-                    uint32_t bad = 0;
-#pragma unroll 4
-                    for (int i = 0; i < KT * KCH / 64; ++i) bad |= not_finite<E>(vt[i * 64 + (x & 63)]);
-                    again |= __any(bad != 0);
+                            for (int i = 0; i < 16; ++i)
+                                s[b][i] = (uint32_t)(mask >> (32 * b)) >> kv_reg<E>(i, 0) & 1u ? s[b][i] : NEG_INF;
+                    }
                 }
                 st.template softmax<SUB>(s, a.scale);
 #pragma unroll
@@ -833,10 +838,20 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
     }
     const size_t slot = ((size_t)(unit * p.n_kv_head + kvh) * sp.parts + at.y) * W + wave;
     const bool part = PREFIX || parts > 1;
-    if (again) {
-        attend_again<E, HD>(a, sp.many, part, t.seq, t.n_kv, kvh, range.x * KT, min(range.y * KT, any), slot, row.limit,
-                            row.at);
-        return;
+    if (range.x < range.y && range.y * KT > all) {
+        // (`least` was read before the first tile's barrier)
+        const bool some = __any(bad != 0);
+        if (lane == 0) least[wave] = some;
+        __syncthreads();
+        int again = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) again |= least[w];
+        again = __builtin_amdgcn_readfirstlane(again);
+        if (again) {
+            attend_again<E, HD>(a, sp.many, part, t.seq, t.n_kv, kvh, range.x * KT, min(range.y * KT, any), slot, row.limit,
+                                row.at);
+            return;
+        }
     }
     const float l = add_halves(st.l), f = part ? 1.0f : over(l);
     const int h = lane >> 5;

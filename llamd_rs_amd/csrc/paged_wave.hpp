@@ -111,6 +111,13 @@ template <class E> __device__ __forceinline__ uint32_t not_finite(run4 r) {
     return bits;
 }
 
+// Whether any element is one: its exponent's lowest bit added to an exponent of ones carries into the sign's place.
+template <class E> __device__ __forceinline__ uint32_t any_not_finite(run4 r) {
+    constexpr uint32_t EXP = Mma<E>::EXP, SIGN = E::RUN == 4 ? 0x80000000u : 0x80008000u;
+    constexpr uint32_t ONE = E::RUN == 4 ? EXP & -EXP : (EXP & 0xFFFFu & -(EXP & 0xFFFFu)) * 0x10001u;
+    return (((r[0] & EXP) + ONE) | ((r[1] & EXP) + ONE) | ((r[2] & EXP) + ONE) | ((r[3] & EXP) + ONE)) & SIGN;
+}
+
 template <class E> __device__ __forceinline__ run4 to_run(const float *x) {
     run4 r;
     if constexpr (E::RUN == 4) {
@@ -307,6 +314,7 @@ template <class E, int HD> struct FewState {
             const run4 x = keep_elements<E>(v(d, 0u), keep);
             const uint32_t bad = not_finite<E>(x);
             any |= bad;
+            asm volatile("" : "+v"(any));  // (added up here, not kept bit by bit to the end)
             o[d] = mul16<E>(keep_elements<E>(x, ~bad), p, o[d]);
             __builtin_amdgcn_sched_barrier(0);  // one d's masks at a time: registers
         }
