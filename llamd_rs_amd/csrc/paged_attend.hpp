@@ -645,6 +645,10 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
                                                     : prompt_parts<E>(steps, sp.parts);
     if (at.y >= parts) return;
     const int2 range = part_steps(steps, parts, at.y);
+    const Pages<E> g = pages_of<E, HD>(p, t.seq, kvh);
+    // the table's entry for position step * KT + lane, looked at a step later (a use at once would wait for it)
+    const auto entry = [&](int step) { return g.table[min(step * KT + (lane & (KT - 1)), t.n_kv - 1) >> p.page_log]; };
+    int next = range.x < range.y ? entry(range.x) : 0;  // the first one is what everything waits for
     // positions that all rows attend to, and that any of this wave's does
     const int mine = wave_reduce(row.limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
     if (lane == 0) least[wave] = mine;
@@ -663,14 +667,11 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
     }
     S st;
     st.clear();
-    const Pages<E> g = pages_of<E, HD>(p, t.seq, kvh);
 
     // runs of a tile's row are exchanged by the row's number, so that 16 lanes that read the same run of consecutive
     // rows meet all banks
     const auto k_swap = [](int r) { return KCH >= 16 ? r & 15 : (r >> 1) & 7; };
     const auto v_swap = [](int r) { return VCH >= 16 ? r & 15 : (r >> 1) & 7; };
-    // the table's entry for position step * KT + lane, looked at a step later (a use at once would wait for it)
-    const auto entry = [&](int step) { return g.table[min(step * KT + (lane & (KT - 1)), t.n_kv - 1) >> p.page_log]; };
     // This thread's runs of a K and V tile: number at = 256 i + thread, in row at / KCH (at / VCH). A tile inside one page
     // is a uniform address and a lane's offset; with smaller pages every run asks for its page. They pass through
     // registers: loads straight into LDS return a quarter as much per cycle.
@@ -754,7 +755,6 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
     if (range.x < range.y) {
         const int last = range.y - 1;
         run4 kr[N], vr[N];
-        int next = entry(range.x);
         load_k(kr, range.x, next);
         load_v(vr, range.x, next);
         unsigned long long valid = readable(range.x, next);
