@@ -12,11 +12,11 @@
 // matrix operands. Either may have a part of a row's positions only; then O (unnormalised), the maximum and the sum
 // go to scratch and paged_join or paged_join_decode puts the parts together, in a fixed order.
 //
-// Bound and measured (32 query heads on 4 kv heads of 128, one MI355X). Long prompts: the matrix cores, 975 TFLOP/s of the
-// causal half at 8192 tokens of bf16 (564 us; a library product of 8192^3 reaches 1349, both at the clock that the power
-// leaves); f32 110 to 119 of 154. Pieces and packed prompts: the steps of the longest tile in a row, 1.1 us each, behind 9
-// us to its first product (512 tokens after 7000 85 us, 9 prompts of up to 1400 43). Decode: memory, then the chain
-// length -> table -> keys and the second launch (1 x 4100 13.3 us, 13 x 1000 in f32 20.6, 48 behind 4100 shared 26.5).
+// Bound and measured (32 query heads on 4 kv heads of 128, one MI355X). Long prompts: the matrix cores, 995 TFLOP/s of the
+// causal half at 8192 tokens of bf16 (552 us; a library product of 8192^3 reaches 1349, both at the clock that the power
+// leaves); f32 110 to 119 of 154. Pieces and packed prompts: the steps of a CU's tiles, 1.1 us each, and 8 us to every
+// workgroup's first product (512 tokens after 7000 81 us, 9 prompts of up to 1400 41). Decode: memory, then the chain
+// length -> table -> keys and the second launch (1 x 4100 13.0 us, 13 x 1000 in f32 20.8, 48 behind 4100 shared 26.4).
 #pragma once
 
 #include <algorithm>
