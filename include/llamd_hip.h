@@ -434,7 +434,8 @@ int llamd_hip_be_get_rows(const float *table, int table_rows, int row_len, const
  * the buffers described:
  *   a position whose page id is outside [0, n_page), or past the table's end,
  *     is not stored, and attended to by no row;
- *   a row that attends to nothing (an empty sequence) gives 0;
+ *   a row that attends to nothing (an empty sequence), or whose scores are all
+ *     minus infinity, gives 0;
  *   tokens before start[0] or from start[n_seq] on belong to no sequence:
  *     their rows of q_out and out are left as they were.
  * A masked position has no part in a row whatever it holds (infinities and NaN

@@ -272,6 +272,34 @@ def test_prompt_not_finite_values_stay_with_those_who_see_them(gpu, kind, bad):
     R.check(c.prompt(q, table, [90, 50], start), want, bound)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_scores_of_minus_infinity(gpu, kind):
+    """Keys of minus infinity weigh nothing beside others; a row that sees nothing else gives 0."""
+    rng = np.random.default_rng(40)
+    heads, kvh, hd, page = 4, 2, 64, 16
+    table, n_page = tables(rng, [80, 20], page)
+    c, k, v = filled(gpu, rng, kind, table, n_page, page, heads, kvh, hd, [80, 20])
+    q = rounded(np.abs(rng.standard_normal((100, heads * hd))) + 0.5, kind)
+    k[table[0, 33 // page], :, 33 % page, 5] = -np.inf
+    for pos in range(20):
+        k[table[1, pos // page], 0, pos % page, 7] = -np.inf
+    c.write(k, v)
+    # position 33 of the first sequence weighs nothing: as if it were not visible; the second one's first kv head has no
+    # finite score
+    want, bound = np.zeros((100, heads, hd)), np.zeros((100, heads, hd))
+    for s, (first, n) in enumerate(((0, 80), (80, 20))):
+        at = np.arange(n)
+        ids = table[s][at // page]
+        rows = slice(first, first + n)
+        want[rows], bound[rows] = R.attend(q[rows].reshape(-1, heads, hd), k[ids, :, at % page], v[ids, :, :, at % page],
+                                           at + 1, hd ** -0.5, kind, None, at != 33 if s == 0 else None)
+    assert np.isnan(want[80:, :2]).all() and np.isfinite(want[:80]).all() and np.isfinite(want[80:, 2:]).all()
+    want[80:, :2] = bound[80:, :2] = 0
+    lists = [80, 20], [0, 80, 100]
+    R.check(c.prompt(q, table, *lists), want.reshape(100, -1), bound.reshape(100, -1))
+    R.check(c.decode(q[[79, 99]], table, [80, 20]), want[[79, 99]].reshape(2, -1), bound[[79, 99]].reshape(2, -1))
+
+
 def test_prompt_starts_that_make_no_sense(gpu):
     """Starts that descend or leave the buffer never reach past it; the sequences that do make sense are right."""
     rng = np.random.default_rng(26)
@@ -533,6 +561,25 @@ def test_prompt_of_thousands(gpu, kind, heads, kvh, hd, page, new, old):
     edges = [0, 1, 31, 32, 63, 64, 127, start[-1] - 1, start[-1] - 2, start[-1] // 2] + [int(x) for x in start[1:-1]]
     picked = sorted(set(edges + rng.integers(0, start[-1], 8).tolist()))
     some_prompt_rows(c, q, k, v, table, lengths, start, heads, kvh, hd, kind, picked)
+
+
+@pytest.mark.parametrize("kind,heads,kvh,hd,page,n,old", [
+    ("bf16", 32, 4, 128, 64, 4200, 0), ("f16", 64, 8, 64, 16, 2100, 90), ("f32", 8, 2, 256, 16, 300, 40),
+    ("f16", 16, 2, 256, 32, 500, 0), ("f32", 16, 4, 128, 128, 600, 1000), ("bf16", 32, 4, 128, 64, 200, 3000)])
+def test_prompt_not_finite_values_in_large_tiles(gpu, kind, heads, kvh, hd, page, n, old):
+    """The first rows that see an infinity or NaN in V, the last that do not, and rows of every wave about them; two
+    in one tile of positions, in different heads."""
+    rng = np.random.default_rng(56)
+    length = n + old
+    table, n_page = tables(rng, [length], page)
+    c, k, v = filled(gpu, rng, kind, table, n_page, page, heads, kvh, hd, [length])
+    q = rounded(rng.standard_normal((n, heads * hd)), kind)
+    spots = [(old + n // 2, 3, np.nan, 0), (old + n // 2 + 5, hd - 1, np.inf, kvh - 1), (old + n - 40, 0, -np.inf, 0)]
+    for pos, d, bad, h in spots:
+        v[table[0, pos // page], h, d, pos % page] = bad
+    c.write(k, v)
+    near = [n // 2 + i for i in (-33, -9, -1, 0, 1, 4, 5, 6, 20, 33)] + [0, n - 41, n - 40, n - 1]
+    some_prompt_rows(c, q, k, v, table, [length], np.array([0, n]), heads, kvh, hd, kind, near)
 
 
 @pytest.mark.parametrize("kind", KINDS)
