@@ -1083,7 +1083,8 @@ template <class E, int HD>
 int prompt_few(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
     const long long rows = (long long)p.n_tok * p.group, tiles = rows / 16 + p.n_seq;
-    const long long busy = (rows + 15) / 16 * p.n_kv_head, want = 2 * CUS;
+    // as many workgroups as are resident (16 tokens after 12000 positions: 33.5 us, for 2 per CU 42, for 4 40)
+    const long long busy = (rows + 15) / 16 * p.n_kv_head, want = (HD <= 128 ? 3 : 2) * CUS;
     const long long most = ((long long)p.max_page << p.page_log) / FEW_STEP;
     Split sp{};
     sp.parts = fit(want / busy, most, 128);
@@ -1103,10 +1104,10 @@ int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
     const long long total = (long long)p.n_tok * p.group, rows = total / p.n_seq;  // and of a sequence, on average
     const long long top = (long long)p.max_page << p.page_log;
-    // few rows per sequence, or little work in all, which 16-row tiles spread further (single calls, 32 query and 4 kv heads:
-    // 45 tokens 8.8 us, with larger tiles 11.6; 6 x up to 16 after 500 positions, 2 M rows x positions, 19 and 25; 24 x up
-    // to 16 after 1000, 8 M, 39 and 32)
-    if (rows <= 64 || total * p.n_kv_head * top <= 3 << 20) return prompt_few<E, HD>(a, st);
+    // few rows per sequence or in all, or little work by what the table holds: 16-row tiles spread it further, but each reads
+    // its keys again (32 query and 4 kv heads: 45 tokens 6.3 us, in larger tiles 9.6; 16 after 500 positions 12.0 and 20.6,
+    // after 3000 20.9 and 22.7; 64 after 500, 1.2 M rows x positions, 16.8 and 20.6; 32 after 3000, 3.1 M, 27.9 and 20.9)
+    if (rows <= 64 || total * p.n_kv_head <= 768 || total * p.n_kv_head * top <= 5 << 19) return prompt_few<E, HD>(a, st);
     // eight waves where all CUs still have work (32 query heads on 4: 4096 tokens 175 us, four waves 195; 3000 110 and 101)
     if constexpr (wide<E, HD>())
         if (rows >= 1024 && total * p.n_kv_head >= 512 * 256) return prompt_tiles<E, HD, 8>(a, st);
