@@ -898,7 +898,7 @@ __global__ __launch_bounds__(256, HD * sizeof(typename E::T) <= 256 ? 2 : 1) voi
 // of row r are ml(z, r), its O of four dimensions o(z, r, four). Groups of threads share the parts among them, and the first
 // loads of O do not wait for the statistics: few loads wait for each other, which is what this would spend its time on
 // (1 x 4100 positions, 33 parts: 14 -> 6 us).
-constexpr int JOIN_MOST = 256;  // parts of a row at the most
+constexpr int JOIN_MOST = 256, TILE_PARTS = 64;  // parts of a row at the most, of a prompt's tile
 template <class E, int HD, int ROWS, class Ml, class O, class At>
 __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, Ml ml, O o, At at) {
     constexpr int FOURS = 8, GROUPS = 256 / (ROWS * FOURS), K = 256 / ROWS, HELD = 4;
@@ -969,6 +969,58 @@ __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, 
     }
 }
 
+// The same for 16 rows with few parts and all their dimensions: every thread adds the parts of its own runs of four, whose
+// first loads do not wait for the statistics either.
+template <class E, int HD, class Ml, class O, class At>
+__device__ __forceinline__ void join_whole(const PagedAttendArgs &a, int n, int rows, Ml ml, O o, At at) {
+    constexpr int ROWS = 16, K = 256 / ROWS, RUNS = HD / 4 / K, HELD = 4;
+    __shared__ float2 stats[TILE_PARTS * ROWS];
+    const int r = threadIdx.x % ROWS, k = threadIdx.x / ROWS;
+    const bool here = r < rows;
+    for (int z = k; z < n; z += K) stats[z * ROWS + r] = here ? ml(z, r) : make_float2(NEG_INF, 0.0f);
+    float4 held[HELD][RUNS];
+#pragma unroll
+    for (int z = 0; z < HELD; ++z)
+#pragma unroll
+        for (int i = 0; i < RUNS; ++i) held[z][i] = here && z < n ? o(z, r, k + K * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __syncthreads();
+    float top = NEG_INF, l = 0.0f;
+    for (int z = 0; z < n; ++z) top = fmaxf(top, stats[z * ROWS + r].x);
+    const float ref = against(top);
+    float4 y[RUNS];
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&](int z, const float4 (&x)[RUNS]) {
+        const float2 s = stats[z * ROWS + r];
+        const float w = exp2_fast(s.x - ref);
+        l = __builtin_fmaf(s.y, w, l);
+#pragma unroll
+        for (int i = 0; i < RUNS; ++i) {
+            y[i].x = __builtin_fmaf(x[i].x, w, y[i].x);
+            y[i].y = __builtin_fmaf(x[i].y, w, y[i].y);
+            y[i].z = __builtin_fmaf(x[i].z, w, y[i].z);
+            y[i].w = __builtin_fmaf(x[i].w, w, y[i].w);
+        }
+    };
+#pragma unroll
+    for (int z = 0; z < HELD; ++z)
+        if (z < n) add(z, held[z]);
+#pragma unroll 2
+    for (int z = HELD; z < n; ++z) {
+        float4 x[RUNS];
+#pragma unroll
+        for (int i = 0; i < RUNS; ++i) x[i] = here ? o(z, r, k + K * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        add(z, x);
+    }
+    const long long row = here ? at(r) : -1;
+    if (row < 0) return;
+    const float by = over(l);
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+        put_out<E>(a.out, a.out_f32, (size_t)row * HD + 4 * (k + K * i),
+                   make_float4(y[i].x * by, y[i].y * by, y[i].z * by, y[i].w * by));
+}
+
 // blockIdx.x: a tile of R rows and kv head of a prompt batch, blockIdx.y: 16 of its rows.
 template <class E, int HD, int R>
 __global__ __launch_bounds__(256) void paged_join(PagedAttendArgs a, Split sp) {
@@ -986,10 +1038,11 @@ __global__ __launch_bounds__(256) void paged_join(PagedAttendArgs a, Split sp) {
     const size_t slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts;
     const int block = FEW ? 0 : first / 32, place = FEW ? 0 : first % 32;
     const auto at = [&](int z) { return FEW ? slot + z : (slot + z) * (R / 32) + block; };
-    join<E, HD, 16>(
-        a, parts, min(t.rows - first, 16), [&](int z, int r) { return x.ml[at(z) * (FEW ? 16 : 32) + place + r]; },
-        [&](int z, int r, int four) { return x.o[(at(z) * (HD / 4) + four) * (FEW ? 16 : 32) + place + r]; },
-        [&](int r) { return prompt_row<R>(p, tile, t, kvh, first + r).at; });
+    const auto ml = [&](int z, int r) { return x.ml[at(z) * (FEW ? 16 : 32) + place + r]; };
+    const auto o = [&](int z, int r, int four) { return x.o[(at(z) * (HD / 4) + four) * (FEW ? 16 : 32) + place + r]; };
+    const auto row = [&](int r) { return prompt_row<R>(p, tile, t, kvh, first + r).at; };
+    if constexpr (FEW) join<E, HD, 16>(a, parts, min(t.rows - first, 16), ml, o, row);
+    else join_whole<E, HD>(a, parts, min(t.rows - first, 16), ml, o, row);
 }
 
 // blockIdx.x: a sequence, blockIdx.y: a kv head and block of 16 of its query heads. R: rows of the prefix's tiles. ROWS: at
@@ -1070,7 +1123,7 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     // (f32's steps are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the
     // workgroups then need two turns; 2048 tokens of 12 heads of 64 take 114 us so, 142 in one turn, 4096 282, 389)
     const long long turns = E::RUN == 4 ? std::min(2 * want / busy, 4LL) : 0;
-    sp.parts = fit(std::max(want / busy, turns), most, 64);
+    sp.parts = fit(std::max(want / busy, turns), most, TILE_PARTS);
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * W, 0, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
