@@ -897,7 +897,7 @@ __global__ __launch_bounds__(256, HD * sizeof(typename E::T) <= 256 ? 2 : 1) voi
 // Up to ROWS rows of HD values (blockIdx.z of gridDim.z equal shares of the dimensions) out of `n` parts: part z's statistics
 // of row r are ml(z, r), its O of four dimensions o(z, r, four). Groups of threads share the parts among them, and the first
 // loads of O do not wait for the statistics: few loads wait for each other, which is what this would spend its time on
-// (1 x 4100 positions, 33 parts: 14 -> 6 us).
+// (1 x 4100 positions, 33 parts: 14 -> 7 us).
 constexpr int JOIN_MOST = 256, TILE_PARTS = 64;  // parts of a row at the most, of a prompt's tile
 template <class E, int HD, int ROWS, class Ml, class O, class At>
 __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, Ml ml, O o, At at) {
@@ -970,7 +970,7 @@ __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, 
 }
 
 // The same for 16 rows with few parts and all their dimensions: every thread adds the parts of its own runs of four, whose
-// first loads do not wait for the statistics either.
+// first loads do not wait for the statistics either. Bound: memory (512 tokens, 4 parts, 34 MB read: 8.3 us, by join 9.5).
 template <class E, int HD, class Ml, class O, class At>
 __device__ __forceinline__ void join_whole(const PagedAttendArgs &a, int n, int rows, Ml ml, O o, At at) {
     constexpr int ROWS = 16, K = 256 / ROWS, RUNS = HD / 4 / K, HELD = 4;
@@ -1119,8 +1119,7 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const long long top = (long long)p.max_page << p.page_log;
     const long long most = top <= KT * whole_steps<E>() ? 1 : top / (KT * tile_least<E>());
     Split sp{};
-    // parts for two workgroups per CU (512 tokens after 7000: 91 us, for four 98, in one part 163).
-    // (f32's steps are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the
+    // parts for two workgroups per CU (single calls, 512 tokens after 7000: 91 us, for four 98, in one part 163; f32's steps are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the
     // workgroups then need two turns; 2048 tokens of 12 heads of 64 take 114 us so, 142 in one turn, 4096 282, 389)
     const long long turns = E::RUN == 4 ? std::min(2 * want / busy, 4LL) : 0;
     sp.parts = fit(std::max(want / busy, turns), most, TILE_PARTS);
