@@ -346,7 +346,8 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
         for (int c = 0; c < S::PS; ++c) {
             const run4 w = S::weights(s, c);
             if constexpr (masked) {
-                st.add_masked([&](int d, uint32_t plus) { return v_run(c, d, plus); }, valid >> ((4 * c + g) * RUN), w, t0 + 4 * RUN * c, limit);
+                st.add_masked([&](int d, uint32_t plus) { return v_run(c, d, plus); }, valid >> ((4 * c + g) * RUN), w,
+                              t0 + 4 * RUN * c, limit);
             } else {
 #pragma unroll
                 for (int d = 0; d < S::DB; ++d) st.o[d] = mul16<E>(v[c][d], w, st.o[d]);
@@ -868,7 +869,8 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
 }
 
 template <class E, int HD, int W>
-__global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256 ? 2 : 1) void paged_tiles(PagedAttendArgs a, Split sp) {
+__global__ __launch_bounds__(64 * W, W == 8 || HD * sizeof(typename E::T) <= 256 ? 2 : 1)
+void paged_tiles(PagedAttendArgs a, Split sp) {
     __shared__ __align__(16) TileShared<E, HD> shared;
     tile_rows<E, HD, W, false>(a, sp, {(int)blockIdx.x, (int)blockIdx.y, (int)gridDim.x, (int)gridDim.y}, shared);
 }
@@ -1119,8 +1121,9 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const long long top = (long long)p.max_page << p.page_log;
     const long long most = top <= KT * whole_steps<E>() ? 1 : top / (KT * tile_least<E>());
     Split sp{};
-    // parts for two workgroups per CU (single calls, 512 tokens after 7000: 91 us, for four 98, in one part 163; f32's steps are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the
-    // workgroups then need two turns; 2048 tokens of 12 heads of 64 take 114 us so, 142 in one turn, 4096 282, 389)
+    // parts for two workgroups per CU (single calls, 512 tokens after 7000: 91 us, for four 98, in one part 163); f32's steps
+    // are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the workgroups then
+    // need two turns (2048 tokens of 12 heads of 64 114 us, 142 in one turn, 4096 282, 389)
     const long long turns = E::RUN == 4 ? std::min(2 * want / busy, 4LL) : 0;
     sp.parts = fit(std::max(want / busy, turns), most, TILE_PARTS);
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
