@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "launch.hpp"
+#include "paged_plan.hpp"
 #include "paged_wave.hpp"
 
 namespace llamd {
@@ -173,8 +174,8 @@ __device__ __forceinline__ Row prompt_row(const PagedArgs &p, int tile, const Ti
     return r;
 }
 
-// A group of sequences: its members [first, end) and the positions that they share (whole pages); none shared where a
-// group has no two members.
+// A group of sequences: its members [first, end) and the positions that they share (whole pages of a table); none shared
+// where a group has no two members.
 struct Group {
     int first, end, shared;
 };
@@ -182,7 +183,7 @@ __device__ __forceinline__ Group group_at(const PagedAttendArgs &a, int g) {
     Group x;
     x.first = min(max(a.group_at[g], 0), a.p.n_seq);
     x.end = min(max(a.group_at[g + 1], x.first), a.p.n_seq);
-    x.shared = x.end - x.first < 2 ? 0 : max(a.shared[g], 0) & ~((1 << a.p.page_log) - 1);
+    x.shared = x.end - x.first < 2 ? 0 : shared_positions(a.shared[g], a.p.page_log, a.p.max_page);
     return x;
 }
 // The group of a sequence, by itself if it is in none.

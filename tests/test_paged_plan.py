@@ -1,0 +1,32 @@
+"""The paged attention's arithmetic on numbers that lie on the device, and how much its launches take (paged_plan.hpp),
+compiled for the host: whatever the numbers, what becomes an address stays inside its buffer."""
+import subprocess
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parent.parent
+HDR = ROOT / "llamd_rs_amd" / "csrc" / "paged_plan.hpp"
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    exe = tmp_path_factory.mktemp("paged_plan") / "paged_plan"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{HDR.parent}", "-o", str(exe),
+                    str(ROOT / "tests" / "native" / "paged_plan.cpp")], check=True)
+
+    def run(lines):
+        done = subprocess.run([str(exe)], input="\n".join(lines), capture_output=True, text=True)
+        assert done.returncode == 0, done.stderr
+        return [tuple(int(x) for x in line.split()) for line in done.stdout.splitlines()]
+    return run
+
+
+def test_shared_positions_stay_in_the_table(plan):
+    """Any number on the device: whole pages, none past the table. A wave steps up to 127 positions past the shared ones, and a
+    sequence of no positions does so without a test of its length before: 2^31 - 16 shared positions would wrap."""
+    numbers = [-(1 << 31), -1, 0, 1, 15, 16, 17, 100, 4095, 4096, 1 << 30, (1 << 30) + 1, (1 << 31) - 64, (1 << 31) - 16, (1 << 31) - 1]
+    cases = [(n, log, most) for n in numbers for log in range(4, 9) for most in (1, 3, 257, 1 << (30 - log))]
+    for (n, log, most), (got,) in zip(cases, plan([f"shared {n} {log} {most}" for n, log, most in cases])):
+        assert got == min(max(n, 0), most << log) >> log << log
+        assert got + 128 < 1 << 31
