@@ -1065,7 +1065,7 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
     if (prefix) {
         int number = 0, tiles = 0;
         const Group g = group_of(a, seq, number);
-        for (int i = lane; i < number; i += WAVE) tiles += prefix_units<R>(a, group_at(a, i));
+        for (int i = lane; i < number; i += WAVE) tiles = add_tiles(tiles, prefix_units<R>(a, group_at(a, i)), sp.tiles);
         base = wave_reduce(tiles, 0, [](int x, int y) { return x + y; });
         constexpr int KT = tile_positions<E, HD>();
         parts = parts_of((readable_of(p, g.shared) + KT - 1) / KT, sp.parts, prefix_least<E>());
@@ -1073,8 +1073,7 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
     }
     const auto many = [&](int z, int r) {  // the slot of a row's 32-row block
         const long long x = first + r;
-        // (starts of groups that descend: more tiles than slots)
-        const size_t tile = (size_t)min((long long)base + x / R, (long long)sp.tiles - 1);
+        const size_t tile = (size_t)tile_of_row(base, x, R, sp.tiles);
         return (tile * p.n_kv_head + kvh) * sp.parts * (R / 32) + (size_t)z * (R / 32) + (size_t)(x % R) / 32;
     };
     const auto few = [&](int z) { return (size_t)(before + z - parts) * gridDim.y + blockIdx.y; };

@@ -14,7 +14,17 @@ int main() {
             return true;
         };
         if (!strcmp(name, "shared") && read(3)) printf("%d\n", llamd::shared_positions((int)a[0], (int)a[1], (int)a[2]));
-        else return 1;
+        else if (!strcmp(name, "join") && read(6)) {
+            // a wave counts the tiles of `groups` groups, 64 at a time, every other one of `more` tiles, and looks for a row
+            const int groups = (int)a[0], more = (int)a[1], tiles = (int)a[2], R = (int)a[3];
+            int sum = 0;
+            for (int lane = 0; lane < 64; ++lane) {
+                int mine = 0;
+                for (int i = lane; i < groups; i += 64) mine = llamd::add_tiles(mine, i % 2 ? 0 : more, tiles);
+                sum += mine;
+            }
+            printf("%d %lld\n", sum, llamd::tile_of_row(a[5] ? a[5] : sum, a[4], R, tiles));
+        } else return 1;
     }
     return 0;
 }

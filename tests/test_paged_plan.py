@@ -30,3 +30,18 @@ def test_shared_positions_stay_in_the_table(plan):
     for (n, log, most), (got,) in zip(cases, plan([f"shared {n} {log} {most}" for n, log, most in cases])):
         assert got == min(max(n, 0), most << log) >> log << log
         assert got + 128 < 1 << 31
+
+
+def test_a_row_of_a_prefix_finds_a_slot(plan):
+    """Starts of groups that go back to the first sequence again and again claim the whole batch each time: 100000 sequences
+    of 64 heads, 50000 groups of 50001 tiles, 2.5e9 in all. Sums and slots stay in their ranges; groups that make sense keep
+    their places."""
+    cases = []
+    for groups, more, tiles in ((100_000, 50_001, 150_000), (100_000, (1 << 22) - 1, (1 << 22) - 1), (3, 7, 9), (1, 1, 1), (0, 5, 5)):
+        for row in (0, 127, 128, 6_399_999, (1 << 31) - 1):
+            cases.append((groups, more, tiles, 128, row, 0))
+    for (groups, more, tiles, R, row, _), (total, tile) in zip(cases, plan([f"join {' '.join(map(str, c))}" for c in cases])):
+        assert 0 <= total <= 64 * tiles and 0 <= tile < tiles
+        if (groups + 1) // 2 * more <= tiles:
+            assert total == (groups + 1) // 2 * more and tile == min(total + row // R, tiles - 1)
+    assert plan(["join 0 0 40 128 300 11"]) == [(0, 13)]
