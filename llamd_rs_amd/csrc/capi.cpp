@@ -378,6 +378,8 @@ int llamd_fwd_end_capture(void) {
 
 int llamd_fwd_graph_launch(void) {
     if (!g_exec) return fail("graph_launch: no graph");
+    // its calls may use the library's scratch: not between the launches of another thread's call that does
+    const std::lock_guard<std::mutex> lk(lib_scratch_mutex());
     return hip_ok(hipGraphLaunch(g_exec, stream()), "graph launch") ? 0 : -1;
 }
 
