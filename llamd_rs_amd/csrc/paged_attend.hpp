@@ -1110,8 +1110,6 @@ bool room(Split &sp, size_t many, size_t few, int few_rows, int hd) {
 
 int queued() { return hipGetLastError() == hipSuccess ? 0 : -1; }
 
-int fit(long long want, long long most, long long cap) { return (int)std::max(1LL, std::min({want, most, cap})); }
-
 template <class E, int HD, int W>
 int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
@@ -1125,7 +1123,7 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     // are long, and a causal prompt's last tile has twice the steps of the mean: up to 4 parts where the workgroups then
     // need two turns (2048 tokens of 12 heads of 64 114 us, 142 in one turn, 4096 282, 389)
     const long long turns = E::RUN == 4 ? std::min(2 * want / busy, 4LL) : 0;
-    sp.parts = fit(std::max(want / busy, turns), most, TILE_PARTS);
+    sp.parts = at_least_one(std::max(want / busy, turns), most, TILE_PARTS);
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     if (sp.parts > 1 && !room(sp, (size_t)tiles * p.n_kv_head * sp.parts * W, 0, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
@@ -1142,7 +1140,7 @@ int prompt_few(const PagedAttendArgs &a, hipStream_t st) {
     const long long busy = (rows + 15) / 16 * p.n_kv_head, want = (HD <= 128 ? 3 : 2) * CUS;
     const long long most = ((long long)p.max_page << p.page_log) / FEW_STEP;
     Split sp{};
-    sp.parts = fit(want / busy, most, 128);
+    sp.parts = at_least_one(want / busy, most, 128);
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     if (sp.parts > 1 && !room(sp, 0, (size_t)tiles * p.n_kv_head * sp.parts, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);
@@ -1185,10 +1183,11 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
                                                 (long long)p.n_seq * ((top + FEW_STEP - 1) / FEW_STEP));
     long long tiles = 0, slots = 0;
     if (a.n_groups) {
-        const long long rows = (long long)p.n_seq * p.group;
-        tiles = rows / R + a.n_groups;
-        const long long busy = (rows + R - 1) / R * p.n_kv_head, want = 2 * CUS;
-        sp.parts = fit(want / busy, top / (KT * prefix_least<E>()), 64);
+        // (groups of one sequence share nothing)
+        const TilePlan plan = plan_tiles((long long)p.n_seq * p.group, std::min(a.n_groups, p.n_seq / 2), R, p.n_kv_head, 2 * CUS,
+                                         top / (KT * prefix_least<E>()), 64);
+        tiles = plan.tiles;
+        sp.parts = plan.parts;
         sp.tiles = (int)tiles;
         slots = tiles * p.n_kv_head * sp.parts * 4;
     }

@@ -20,4 +20,26 @@ constexpr long long tile_of_row(long long before, long long row, int R, int tile
     return tile < tiles ? tile : tiles - 1;
 }
 
+// How many there are of something: `want`, but no more than `most` nor `cap`, and one at least.
+constexpr int at_least_one(long long want, long long most, long long cap) {
+    const long long n = want < most ? want : most, x = n < cap ? n : cap;
+    return x < 1 ? 1 : (int)x;
+}
+
+// The tiles of R rows that there can be where `rows` rows lie in up to `pieces` pieces (sequences, groups) that each begin a
+// tile of their own, and the parts of a tile's positions that make about `want` workgroups, `most` and `cap` at the most. How
+// many pieces have rows is known on the device only: parts are for tiles that the rows fill, or for a tile per four pieces
+// if that is more, so that tiles times parts stays within a few times `want` whatever the pieces. 64 sequences of 32 heads
+// in 32 pairs: 2 parts, 166 us and 130 MB of slots, where parts for full tiles are 16, 192 us and 1 GB, and a tile per piece
+// gives one part, 164 us; but one group in a list of 32 places (64 sequences behind 15000 positions, 32 / 4 heads) takes 53
+// us this way, 98 with a tile per piece.
+struct TilePlan {
+    long long tiles;
+    int parts;
+};
+constexpr TilePlan plan_tiles(long long rows, long long pieces, int R, int n_kv_head, long long want, long long most, int cap) {
+    const long long full = (rows + R - 1) / R, some = (pieces + 3) / 4, least = full > some ? full : some;
+    return {rows / R + pieces, at_least_one(want / (least * n_kv_head), most, cap)};
+}
+
 }  // namespace llamd

@@ -24,6 +24,9 @@ int main() {
                 sum += mine;
             }
             printf("%d %lld\n", sum, llamd::tile_of_row(a[5] ? a[5] : sum, a[4], R, tiles));
+        } else if (!strcmp(name, "tiles") && read(7)) {
+            const llamd::TilePlan x = llamd::plan_tiles(a[0], a[1], (int)a[2], (int)a[3], a[4], a[5], (int)a[6]);
+            printf("%lld %d\n", x.tiles, x.parts);
         } else return 1;
     }
     return 0;

@@ -1,12 +1,16 @@
 """The paged cache's calls at their edges: numbers on the device that make no sense, an eager call beside a replayed graph, what
 the library's scratch grows to. Values against paged_reference."""
 import ctypes as C
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
 
 import paged_reference as R
-from test_gpu_paged import filled, rounded, tables, want_decode
+from test_gpu_paged import filled, rounded, shared_tables, tables, want_decode
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +71,50 @@ def test_a_replayed_graph_beside_another_threads_calls(gpu, kind):
     L.llamd_fwd_graph_destroy()
     assert len(other) == 61 and replayed
     assert all(np.array_equal(x, other[0]) for x in other) and all(np.array_equal(x, want) for x in replayed)
+
+
+# ---- the scratch ------------------------------------------------------------------
+# It never shrinks, and what other calls left would hide a call's own need: each of these runs in a process of its own.
+
+HERE = Path(__file__).resolve().parent
+MB = 1 << 20
+
+
+def alone(name, *args):
+    """Runs a function of this file in a fresh process."""
+    code = f"import test_gpu_paged_calls as t\nfrom llamd_rs_amd import rocm\nt.{name}(rocm, *{args!r})\nprint('done', flush=True)"
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(HERE), str(HERE.parent)]))
+    done = subprocess.run([sys.executable, "-c", code], cwd=HERE.parent, env=env, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and done.stdout.split()[-1:] == ["done"], done.stdout[-2000:] + done.stderr[-4000:]
+
+
+def grown(gpu, call):
+    """What a call returns, and by how many bytes the library's scratch grew in it (its other memory is freed)."""
+    before = gpu.lib().llamd_rocm_free_mem()
+    got = call()
+    return got, before - gpu.lib().llamd_rocm_free_mem()
+
+
+def pairs(gpu, n_seq, heads, width):
+    """Sequences in pairs that share two pages, in a wide table."""
+    rng = np.random.default_rng(61)
+    hd, page = 128, 32
+    group = list(range(0, n_seq + 1, 2))
+    lengths = [70 + s % 9 for s in range(n_seq)]
+    table, n_page, _ = shared_tables(rng, group, [64] * (n_seq // 2), lengths, page)
+    c, k, v = filled(gpu, rng, "bf16", table, n_page, page, heads, heads, hd, lengths)
+    q = rounded(rng.standard_normal((n_seq, heads * hd)), "bf16")
+    wide = np.full((n_seq, width // page), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    shared = [64] * (n_seq // 2)
+    got, more = grown(gpu, lambda: c.decode(q, wide, lengths, group, shared))
+    want, bound = want_decode(q, k, v, table, lengths, heads, heads, hd, hd ** -0.5, "bf16", group, shared)
+    R.check(got, want, bound)
+    # slots of 128 rows (f32 values, two statistics): 5 for each of 512 workgroups, or one per pair and head; then small things
+    assert more <= max(5 * 512, (n_seq // 2 + 2) * heads) * 128 * (hd * 4 + 8) + 8 * MB, more // MB
+
+
+@pytest.mark.parametrize("n_seq,heads,width", [(64, 32, 8192), (128, 16, 16384)])
+def test_scratch_of_many_small_groups(gpu, n_seq, heads, width):
+    """Every group has tiles of its own: parts are for the tiles that there can be, not for rows packed into full ones."""
+    alone("pairs", n_seq, heads, width)

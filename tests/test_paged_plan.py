@@ -1,5 +1,6 @@
 """The paged attention's arithmetic on numbers that lie on the device, and how much its launches take (paged_plan.hpp),
 compiled for the host: whatever the numbers, what becomes an address stays inside its buffer."""
+import random
 import subprocess
 from pathlib import Path
 
@@ -45,3 +46,24 @@ def test_a_row_of_a_prefix_finds_a_slot(plan):
         if (groups + 1) // 2 * more <= tiles:
             assert total == (groups + 1) // 2 * more and tile == min(total + row // R, tiles - 1)
     assert plan(["join 0 0 40 128 300 11"]) == [(0, 13)]
+
+
+def test_tiles_and_parts_of_any_pieces(plan):
+    """Rows cut into pieces anyhow never make more tiles than there are slots for, and slots stay within five times the
+    workgroups wanted (tiles <= full tiles + pieces <= 5 max(full tiles, pieces / 4)), or the tiles themselves where these are
+    more."""
+    rng = random.Random(5)
+    cases = []
+    for R in (16, 128):
+        for rows, pieces in ((8, 64), (1, 1), (64, 32), (2048, 512), (4096, 0), (12, 12), (100_000, 3), (1 << 20, 1 << 16)):
+            cases += [(rows, pieces, R, kv, 512, most, 64) for kv in (1, 4, 32) for most in (0, 16, 4096)]
+    for (rows, pieces, R, kv, want, most, cap), (tiles, parts) in zip(cases, plan([f"tiles {' '.join(map(str, c))}" for c in cases])):
+        assert 1 <= parts <= max(1, min(most, cap))
+        assert parts == 1 or tiles * kv * parts <= 5 * want
+        for _ in range(4):
+            cuts = sorted(rng.randrange(rows + 1) for _ in range(max(pieces, 1) - 1)) + [rows]
+            sizes = [b - a for a, b in zip([0] + cuts, cuts)]
+            if pieces:
+                assert sum(-(-n // R) for n in sizes) <= tiles
+    # 64 sequences in pairs, heads of their own; 48 sequences of 8 heads behind one prefix
+    assert plan(["tiles 64 32 128 32 512 16 64", "tiles 384 1 128 4 512 9 64"]) == [(32, 2), (4, 9)]
