@@ -1114,7 +1114,7 @@ template <class E, int HD, int W>
 int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
     constexpr int R = 32 * W, KT = tile_positions<E, HD>();
-    const long long rows = (long long)p.n_tok * p.group, tiles = rows / R + p.n_seq;
+    const long long rows = (long long)p.n_tok * p.group, tiles = rows / R + std::min(p.n_seq, p.n_tok);
     const long long busy = (rows + R - 1) / R * p.n_kv_head, want = CUS * 8 / W;
     const long long top = (long long)p.max_page << p.page_log;
     const long long most = top <= KT * whole_steps<E>() ? 1 : top / (KT * tile_least<E>());
@@ -1135,12 +1135,12 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
 template <class E, int HD>
 int prompt_few(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
-    const long long rows = (long long)p.n_tok * p.group, tiles = rows / 16 + p.n_seq;
     // as many workgroups as are resident (16 tokens after 12000 positions: 33.5 us, for 2 per CU 42, for 4 40)
-    const long long busy = (rows + 15) / 16 * p.n_kv_head, want = (HD <= 128 ? 3 : 2) * CUS;
-    const long long most = ((long long)p.max_page << p.page_log) / FEW_STEP;
+    const TilePlan plan = plan_tiles((long long)p.n_tok * p.group, std::min(p.n_seq, p.n_tok), 16, p.n_kv_head, (HD <= 128 ? 3 : 2) * CUS,
+                                     ((long long)p.max_page << p.page_log) / FEW_STEP, 128);
+    const long long tiles = plan.tiles;
     Split sp{};
-    sp.parts = at_least_one(want / busy, most, 128);
+    sp.parts = plan.parts;
     if (tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
     if (sp.parts > 1 && !room(sp, 0, (size_t)tiles * p.n_kv_head * sp.parts, 16, HD)) return -1;
     const dim3 grid((unsigned)(tiles * p.n_kv_head), sp.parts);

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 import paged_reference as R
-from test_gpu_paged import filled, rounded, shared_tables, tables, want_decode
+from test_gpu_paged import filled, rounded, shared_tables, tables, want_decode, want_prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,30 @@ def pairs(gpu, n_seq, heads, width):
 def test_scratch_of_many_small_groups(gpu, n_seq, heads, width):
     """Every group has tiles of its own: parts are for the tiles that there can be, not for rows packed into full ones."""
     alone("pairs", n_seq, heads, width)
+
+
+def few_tokens(gpu, n_seq, tokens, heads, kvh):
+    """A prompt batch of few tokens and many sequences that have none, as a captured call with places left looks."""
+    rng = np.random.default_rng(62)
+    hd, page = 128, 64
+    new = [0] * n_seq
+    for i in range(tokens):
+        new[(i * 37 + 5) % n_seq] += 1
+    lengths = [200 + 3 * s % 50 if n else 0 for s, n in enumerate(new)]
+    table, n_page = tables(rng, lengths, page)
+    wide = np.full((n_seq, 16384 // page), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    c, k, v = filled(gpu, rng, "bf16", table, n_page, page, heads, kvh, hd, lengths)
+    start = np.concatenate([[0], np.cumsum(new)])
+    q = rounded(rng.standard_normal((tokens, heads * hd)), "bf16")
+    got, more = grown(gpu, lambda: c.prompt(q, wide, lengths, start))
+    want, bound = want_prompt(q, k, v, table, lengths, start, heads, kvh, hd, hd ** -0.5, "bf16")
+    R.check(got, want, bound)
+    # slots of 16 rows: 5 for each of 768 workgroups, or one per tile and head; then small things
+    assert more <= max(5 * 768, 2 * tokens * kvh) * 16 * (hd * 4 + 8) + 8 * MB, more // MB
+
+
+@pytest.mark.parametrize("n_seq,tokens,heads,kvh", [(64, 1, 32, 4), (256, 8, 32, 32), (1000, 3, 8, 8), (40, 40, 12, 12)])
+def test_scratch_of_sequences_without_tokens(gpu, n_seq, tokens, heads, kvh):
+    """Tiles are counted for the sequences that can have tokens."""
+    alone("few_tokens", n_seq, tokens, heads, kvh)
