@@ -145,3 +145,41 @@ def few_tokens(gpu, n_seq, tokens, heads, kvh):
 def test_scratch_of_sequences_without_tokens(gpu, n_seq, tokens, heads, kvh):
     """Tiles are counted for the sequences that can have tokens."""
     alone("few_tokens", n_seq, tokens, heads, kvh)
+
+
+def moved_scratch(gpu, kind):
+    L = gpu.lib()
+    rng = np.random.default_rng(64)
+    heads, kvh, hd, page = 8, 1, 128, 16
+    lengths, start = [900, 2000, 50], [0, 20, 29, 40]
+    table, n_page = tables(rng, lengths, page)
+    c, k, v = filled(gpu, rng, kind, table, n_page, page, heads, kvh, hd, lengths)
+    q = rounded(rng.standard_normal((40, heads * hd)), kind)
+    want, bound = want_prompt(q, k, v, table, lengths, start, heads, kvh, hd, hd ** -0.5, kind)
+    b, keep = c._batch(table, lengths, start, 40)
+    dq, out = gpu.DeviceBuffer.from_array(c.encode(q)), gpu.DeviceBuffer.from_array(np.zeros(q.shape, c.dtype))
+    assert L.llamd_fwd_begin_capture() == 0
+    assert L.llamd_hip_paged_prompt(C.byref(c.pages), C.byref(b), dq.ptr, heads, hd ** -0.5, c.pages.type, out.ptr) == 0
+    assert L.llamd_fwd_end_capture() == 0
+    first = None
+    big_q = rng.standard_normal((700, heads * hd))
+    for turn, width in enumerate((3000, 9000, 3000)):
+        out.upload(np.zeros(q.shape, c.dtype))
+        assert L.llamd_fwd_graph_launch() == 0
+        got = c.decode_values(out.download(np.empty(q.shape, c.dtype)))
+        R.check(got, want, bound, turn)
+        assert first is None or np.array_equal(got, first), turn
+        first = got
+        # an eager call whose parts (44 tiles of 128 rows, 11 parts: 33 MB) need more than the captured call's (3 MB)
+        big_t, big_n = tables(rng, [width], page, 0)
+        big = gpu.PagedCache(kind, big_n, page, heads, kvh, hd)
+        _, more = grown(gpu, lambda: big.prompt(big_q, big_t, [width], [0, 700]))
+        big.close()
+        assert turn or more >= 32 * MB, more  # the scratch is another one now
+    L.llamd_fwd_graph_destroy()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_a_graph_keeps_the_scratch_that_it_captured(gpu, kind):
+    """A larger eager call replaces the library's scratch; replays go on in the one that they were captured with."""
+    alone("moved_scratch", kind)
