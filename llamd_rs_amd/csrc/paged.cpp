@@ -77,7 +77,8 @@ int describe_attend(const char *what, const llamd_hip_pages *c, const llamd_hip_
                     float scale, int out_type, void *out, PagedAttendArgs *a) {
     if (describe(what, c, b, n_head, &a->p)) return -1;
     if (!q || !out || !aligned(q) || !aligned(out)) return set_error("%s: q and out must be 16-byte aligned", what);
-    if (!(scale > 0.0f) || !isfinite(scale)) return set_error("%s: scale %g", what, (double)scale);
+    const float by = (float)(scale * 1.4426950408889634074);  // (past the largest f32: 0 scores would be NaN)
+    if (!(scale > 0.0f) || !isfinite(by)) return set_error("%s: scale %g", what, (double)scale);
     if (out_type != c->type && out_type != PT_F32)
         return set_error("%s: out_type %d (the cache's, %d, or f32)", what, out_type, c->type);
     const size_t values = (size_t)b->n_tok * n_head * c->hd;
@@ -87,7 +88,7 @@ int describe_attend(const char *what, const llamd_hip_pages *c, const llamd_hip_
     a->q = q;
     a->out = out;
     a->out_f32 = out_type == PT_F32;
-    a->scale = (float)(scale * 1.4426950408889634074);
+    a->scale = by;
     return 0;
 }
 

@@ -144,3 +144,11 @@ def test_frequencies_by_parts(n_rot, base, factor, orig):
 def test_refused_frequencies(args):
     with pytest.raises(HipError):
         rocm.rope_freqs(*args)
+
+
+@pytest.mark.parametrize("name", ["prompt", "decode"])
+def test_refused_scales_whose_exponent_of_two_is_no_number(name):
+    """Weights are powers of two of scale * log2(e) times a score: where that passes f32's range, scores of 0 would be NaN."""
+    for scale in (3e38, 2.4e38, -math.inf):
+        assert call(name, scale=scale) == -1
+        assert last_error() == "paged_%s: scale %g" % (name, np.float32(scale))
