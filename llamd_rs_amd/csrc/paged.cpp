@@ -145,12 +145,15 @@ int llamd_hip_paged_store(const llamd_hip_pages *c, const llamd_hip_batch *b, co
                          interleaved);
     if (!(eps >= 0.0f) || !isfinite(eps) || !isfinite(mscale))
         return set_error("paged_store: eps %g, mscale %g", (double)eps, (double)mscale);
+    // (the rows up to the last one's end)
+    const size_t rows = b->n_tok ? b->n_tok - 1 : 0, n_k = (rows * ld_k + kv) * 4, n_v = (rows * ld_v + kv) * 4;
+    if (meets_pages(c, k, n_k) || meets_pages(c, v, n_v)) return set_error("paged_store: k or v overlaps the pages");
     if (q) {
-        const size_t rows = b->n_tok ? b->n_tok - 1 : 0;
+        const size_t n_q = (rows * ld_q + (size_t)n_head * c->hd) * 4;
         const size_t n_out = (size_t)b->n_tok * n_head * c->hd * type_bytes(c->type);
-        if (overlap(q, (rows * ld_q + (size_t)n_head * c->hd) * 4, q_out, n_out) ||
-            overlap(k, (rows * ld_k + kv) * 4, q_out, n_out) || overlap(v, (rows * ld_v + kv) * 4, q_out, n_out))
+        if (overlap(q, n_q, q_out, n_out) || overlap(k, n_k, q_out, n_out) || overlap(v, n_v, q_out, n_out))
             return set_error("paged_store: q_out overlaps q, k or v");
+        if (meets_pages(c, q, n_q)) return set_error("paged_store: q overlaps the pages");
         if (meets_pages(c, q_out, n_out)) return set_error("paged_store: q_out overlaps the pages");
     }
     if (!b->n_seq || !b->n_tok) return 0;

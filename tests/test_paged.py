@@ -152,3 +152,11 @@ def test_refused_scales_whose_exponent_of_two_is_no_number(name):
     for scale in (3e38, 2.4e38, -math.inf):
         assert call(name, scale=scale) == -1
         assert last_error() == "paged_%s: scale %g" % (name, np.float32(scale))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=(1 << 20) + 4096), dict(k=(1 << 20) + 4096), dict(v=(2 << 20) + 4096), dict(k=(2 << 20) - 16), dict(v=(1 << 20) - 2048)])
+def test_refused_store_of_rows_that_lie_in_the_pages(kw):
+    """Pages are written while other workgroups read q, k and v."""
+    assert call("store", **kw) == -1
+    assert "overlaps the pages" in last_error()
