@@ -30,17 +30,17 @@
 namespace llamd {
 namespace {
 
-// Parts of rows: a slot has the statistics (maximum, sum) of `rows` rows and their O, four dimensions at a time:
+// Parts of rows: a slot has the statistics (maximum, sum) of its rows and their O, four dimensions at a time:
 // o[slot][HD / 4][rows].
 struct Parts {
     float4 *o;
     float2 *ml;
-    int rows;
 };
 
 // How a call is split (host).
 struct Split {
     Parts many, few;     // of paged_tiles (blocks of 32 rows) and of paged_few
+    int few_rows;        // rows of a slot of the latter: 16, or in decode a sequence's and kv head's, if fewer
     int parts;           // most parts of a row tile (prompt, prefix)
     int tiles;           // decode: tiles of shared prefixes that there are slots for
     double per_item;     // decode: 1 / (positions of all sequences' parts wanted, in steps)
@@ -548,7 +548,7 @@ __device__ __forceinline__ void few_rows(const PagedAttendArgs &a, const Split &
         l = __builtin_fmaf(stats[w][m].y, f[w], l);
     }
     const float by = parts > 1 ? 1.0f : over(l);
-    if (parts > 1 && wave == 0 && g == 0 && m < sp.few.rows) sp.few.ml[slot * sp.few.rows + m] = make_float2(top, l);
+    if (parts > 1 && wave == 0 && g == 0 && m < sp.few_rows) sp.few.ml[slot * sp.few_rows + m] = make_float2(top, l);
 #pragma unroll
     for (int j = 0; j < S::DB / 4; ++j) {
         const int d = wave * (S::DB / 4) + j;
@@ -562,7 +562,7 @@ __device__ __forceinline__ void few_rows(const PagedAttendArgs &a, const Split &
         }
         const float4 y = make_float4(x[0], x[1], x[2], x[3]);
         if (parts > 1) {
-            if (m < sp.few.rows) sp.few.o[(slot * (HD / 4) + 4 * d + g) * sp.few.rows + m] = y;
+            if (m < sp.few_rows) sp.few.o[(slot * (HD / 4) + 4 * d + g) * sp.few_rows + m] = y;
         } else if (r.at >= 0) {
             put_out<E>(a.out, a.out_f32, (size_t)r.at * HD + 16 * d + 4 * g, y);
         }
@@ -897,10 +897,10 @@ __global__ __launch_bounds__(256, HD * sizeof(typename E::T) <= 256 ? 2 : 1) voi
 
 // ---- the parts together ------------------------------------------------------------
 
-// Up to ROWS rows of HD values (blockIdx.z of gridDim.z equal shares of the dimensions) out of `n` parts: part z's statistics
-// of row r are ml(z, r), its O of four dimensions o(z, r, four). Groups of threads share the parts among them, and the first
-// loads of O do not wait for the statistics: few loads wait for each other, which is what this would spend its time on
-// (1 x 4100 positions, 33 parts: 14 -> 7 us).
+// Up to ROWS rows, 32 of their dimensions (share number blockIdx.z), out of `n` parts: part z's statistics of row r are
+// ml(z, r), its O of four dimensions o(z, r, four). Groups of threads share the parts among them, and the first loads of O do
+// not wait for the statistics: few loads wait for each other, which is what this would spend its time on (1 x 4100
+// positions, 33 parts: 14 -> 7 us).
 constexpr int JOIN_MOST = 256, TILE_PARTS = 64;  // parts of a row at the most, of a prompt's tile
 template <class E, int HD, int ROWS, class Ml, class O, class At>
 __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, Ml ml, O o, At at) {
@@ -909,18 +909,15 @@ __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, 
     __shared__ float side[K][ROWS];
     __shared__ float4 sums[GROUPS][FOURS * ROWS];
     const int r = threadIdx.x % ROWS, k = threadIdx.x / ROWS, f = k % FOURS, group = k / FOURS;
-    const int share = HD / 4 / gridDim.z, begin = blockIdx.z * share;
+    const int four = blockIdx.z * FOURS + f;
     const bool here = r < rows;
     for (int z = k; z < n; z += K) stats[z * ROWS + r] = here ? ml(z, r) : make_float2(NEG_INF, 0.0f);
     float4 held[HELD];
-    const auto hold = [&](int four) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int z = group + i * GROUPS;
-            held[i] = here && z < n ? o(z, r, four) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-    };
-    hold(begin + f);
+    for (int i = 0; i < HELD; ++i) {
+        const int z = group + i * GROUPS;
+        held[i] = here && z < n ? o(z, r, four) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
     float top = NEG_INF;
     for (int z = k; z < n; z += K) top = fmaxf(top, stats[z * ROWS + r].x);  // this thread's own writes
     side[k][r] = top;
@@ -942,33 +939,28 @@ __device__ __forceinline__ void join(const PagedAttendArgs &a, int n, int rows, 
     for (int i = 0; i < K; ++i) l += side[i][r];
     const float by = over(l);
     const long long row = here ? at(r) : -1;
-    for (int four = begin + f; four < begin + share; four += FOURS) {
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const auto add = [&](float4 x, float w) {
-            y.x = __builtin_fmaf(x.x, w, y.x);
-            y.y = __builtin_fmaf(x.y, w, y.y);
-            y.z = __builtin_fmaf(x.z, w, y.z);
-            y.w = __builtin_fmaf(x.w, w, y.w);
-        };
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&](float4 x, float w) {
+        y.x = __builtin_fmaf(x.x, w, y.x);
+        y.y = __builtin_fmaf(x.y, w, y.y);
+        y.z = __builtin_fmaf(x.z, w, y.z);
+        y.w = __builtin_fmaf(x.w, w, y.w);
+    };
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int z = group + i * GROUPS;
-            if (z < n) add(held[i], stats[z * ROWS + r].x);
-        }
-        if (four + FOURS < begin + share) hold(four + FOURS);
-        if (here) {
+    for (int i = 0; i < HELD; ++i) {
+        const int z = group + i * GROUPS;
+        if (z < n) add(held[i], stats[z * ROWS + r].x);
+    }
+    if (here) {
 #pragma unroll 8
-            for (int z = group + HELD * GROUPS; z < n; z += GROUPS) add(o(z, r, four), stats[z * ROWS + r].x);
-        }
-        sums[group][f * ROWS + r] = y;
-        __syncthreads();
-        if (row >= 0 && !group) {
+        for (int z = group + HELD * GROUPS; z < n; z += GROUPS) add(o(z, r, four), stats[z * ROWS + r].x);
+    }
+    sums[group][f * ROWS + r] = y;
+    __syncthreads();
+    if (row >= 0 && !group) {
 #pragma unroll
-            for (int i = 1; i < GROUPS; ++i) add(sums[i][f * ROWS + r], 1.0f);
-            put_out<E>(a.out, a.out_f32, (size_t)row * HD + 4 * four,
-                       make_float4(y.x * by, y.y * by, y.z * by, y.w * by));
-        }
-        __syncthreads();
+        for (int i = 1; i < GROUPS; ++i) add(sums[i][f * ROWS + r], 1.0f);
+        put_out<E>(a.out, a.out_f32, (size_t)row * HD + 4 * four, make_float4(y.x * by, y.y * by, y.z * by, y.w * by));
     }
 }
 
@@ -1077,7 +1069,7 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
         return (tile * p.n_kv_head + kvh) * sp.parts * (R / 32) + (size_t)z * (R / 32) + (size_t)(x % R) / 32;
     };
     const auto few = [&](int z) { return (size_t)(before + z - parts) * gridDim.y + blockIdx.y; };
-    const int w = sp.few.rows;
+    const int w = sp.few_rows;
     join<E, HD, ROWS>(
         a, parts + units, min(p.group - head, 16),
         [&](int z, int r) {
@@ -1103,8 +1095,7 @@ bool room(Split &sp, size_t many, size_t few, int few_rows, int hd) {
     sp.few.o = (float4 *)(p + o_many * 4);
     sp.many.ml = (float2 *)(p + (o_many + o_few) * 4);
     sp.few.ml = sp.many.ml + many * 32;
-    sp.many.rows = 32;
-    sp.few.rows = few_rows;
+    sp.few_rows = few_rows;
     return true;
 }
 

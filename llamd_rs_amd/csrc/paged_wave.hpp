@@ -199,21 +199,6 @@ template <class E, int HD> struct RowState {
         for (int j = 0; j < E::RUN; ++j) x[j] = s[c * E::RUN + j];
         return to_run<E>(x);
     }
-
-    // O to a row of HD values, of the type or f32.
-    template <class W> __device__ __forceinline__ void write_as(void *out, size_t row) const {
-        const int h = (threadIdx.x >> 5) & 1;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                put4<W>(out, row * HD + 32 * d + 2 * i + 4 * h,
-                        make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]));
-    }
-    __device__ __forceinline__ void write(void *out, bool f32, size_t row) const {
-        if (f32) write_as<ElemF32>(out, row);
-        else write_as<E>(out, row);
-    }
 };
 
 // ---- 16 rows ----------------------------------------------------------------------
