@@ -12,11 +12,12 @@
 // matrix operands. Either may have a part of a row's positions only; then O (unnormalised), the maximum and the sum
 // go to scratch and paged_join or paged_join_decode puts the parts together, in a fixed order.
 //
-// Bound and measured (32 query heads on 4 kv heads of 128, one MI355X). Long prompts: the matrix cores, 995 TFLOP/s of the
-// causal half at 8192 tokens of bf16 (552 us; a library product of 8192^3 reaches 1349, both at the clock that the power
-// leaves); f32 110 to 119 of 154. Pieces and packed prompts: the steps of a CU's tiles, 1.1 us each, and 8 us to every
-// workgroup's first product (512 tokens after 7000 81 us, 9 prompts of up to 1400 41). Decode: memory, then the chain
-// length -> table -> keys and the second launch (1 x 4100 13.0 us, 13 x 1000 in f32 20.8, 48 behind 4100 shared 26.4).
+// Bound and measured (32 query heads on 4 kv heads of 128, one MI355X). Long prompts of 16 bits: products and the softmax's
+// vector work, one after the other (8192 tokens of bf16: matrix cores busy 46% of the cycles, vector units 53%; 560 us, 980
+// TFLOP/s of the causal half, where a library product of 8192^3 reaches 1349); f32 110 to 119 of 154. Pieces and packed
+// prompts: the steps of a CU's tiles, 1.1 us each, and 8 us to every workgroup's first product (512 tokens after 7000 81 us,
+// 9 prompts of 192 to 700 tokens 41). Decode: memory, then the chain length -> table -> keys and the second launch (1 x 4100
+// 12.8 us, 13 x 1000 in f32 20.4, 48 behind 4100 shared 25.8).
 #pragma once
 
 #include <algorithm>
@@ -363,7 +364,9 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
 }
 
 // Rows of a wave of paged_tiles (32, from `limit` and `at` of their lanes) once more, 16 at a time straight from the pages,
-// every infinity or NaN in V added only where it belongs. (Inline: a call would give the kernel scratch memory, with which
+// every infinity or NaN in V added only where it belongs. Slow, since a workgroup does it alone: one such value in a tile that
+// some row sees in part makes a prompt of 4096 tokens 1128 us instead of 160, 63 of them 1545; 512 tokens after 7000 410
+// instead of 85, 9 packed prompts 175 instead of 44. (Inline: a call would give the kernel scratch memory, with which
 // workgroups start at a third of the rate, 14 us for 512 of them instead of 5.)
 template <class E, int HD>
 __device__ __forceinline__ void attend_again(const PagedAttendArgs &a, const Parts &parts, bool part, int seq, int n_kv,
@@ -1149,8 +1152,12 @@ int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
     const long long total = (long long)p.n_tok * p.group, rows = total / p.n_seq;  // and of a sequence, on average
     const long long top = (long long)p.max_page << p.page_log;
     // few rows per sequence or in all, or little work by what the table holds: 16-row tiles spread it further, but each reads
-    // its keys again (32 query and 4 kv heads: 45 tokens 6.3 us, in larger tiles 9.6; 16 after 500 positions 12.0 and 20.6,
-    // after 3000 20.9 and 22.7; 64 after 500, 1.2 M rows x positions, 16.8 and 20.6; 32 after 3000, 3.1 M, 27.9 and 20.9)
+    // its keys again (32 query and 4 kv heads of bf16: 45 tokens 6.3 us, in larger tiles 9.6; 16 after 500 positions 14.3 and
+    // 21.5, after 3000 20.8 and 22.7, after 12000 36 and 42; 64 after 500, 1.2 M rows x positions, 16.8 and 20.6; 32 after
+    // 3000, 3.1 M, 27.9 and 20.9). The wrong way at its far end: 24 after 12000 46 and 36, 16 after 30000 66 and 56. One way
+    // for the whole batch, by its mean: a long prompt among many short sequences, or in a list of mostly empty places, is
+    // taken 16 rows at a time (4096 tokens in 1024 places 939 us, in 256 165, alone 154; 2000 tokens beside 400 single ones 311,
+    // in two calls 60 and 87)
     if (rows <= 64 || total * p.n_kv_head <= 768 || total * p.n_kv_head * top <= 5 << 19) return prompt_few<E, HD>(a, st);
     // eight waves where all CUs still have work (32 query heads on 4: 4096 tokens 175 us, four waves 195; 3000 110 and 101)
     if constexpr (wide<E, HD>())
@@ -1165,8 +1172,9 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
     const int per = (p.group + 15) / 16, cols = p.n_kv_head * per;
     const long long top = (long long)p.max_page << p.page_log;
     Split sp{};
-    // parts of the sequences' own positions: 4 workgroups per CU, one part per sequence at least (64 x 2000 positions: 44 us,
-    // 2 per CU 51, 1 per CU 50); a row's should fill the GPU once where there are few columns
+    // parts of the sequences' own positions: 4 workgroups per CU, one part per sequence at least (64 x 500 to 2000 positions,
+    // 164 MB: 37.5 us, 2 per CU 44, 1 per CU 51; all of 2000, 263 MB: 52.6, 51.6, 47.5); a row's should fill the GPU once
+    // where there are few columns
     const int target = std::min(std::max(1, 4 * CUS / cols), JOIN_MOST - 66);
     sp.per_item = 1.0 / ((double)target * FEW_STEP);
     sp.per_row = 1.0 / ((double)std::max(FEW_PARTS, CUS / cols) * FEW_STEP);

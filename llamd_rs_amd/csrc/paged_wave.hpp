@@ -9,8 +9,10 @@
 // position's dimensions together, V pages a dimension's positions.
 //
 // Exponentials are powers of two: x = s * (scale * log2 e) - m. Scores, maxima, sums and O are f32. P is rounded to the
-// cache's type for the second product (half a unit in the last place of values in [0, 1], independent per position, of
-// the size of V's own rounding); the sum l adds the unrounded values.
+// cache's type for the second product (half a step relative, of the size of V's own rounding; below f16's normal range,
+// half its smallest step); the sum l adds the unrounded values. Positions of equal scores round alike, so that what this
+// takes from O does not shrink with their number: half a step (bf16 2^-8, f16 2^-11) of sum p |v| bounds it, and an f32
+// result of a 16-bit cache has it too.
 #pragma once
 
 #include "paged_util.hpp"
