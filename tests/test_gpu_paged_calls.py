@@ -31,6 +31,19 @@ def test_groups_that_share_more_than_the_table_holds(gpu, page, shared):
     assert not got[[1, 4]].any() and got[5].any()
 
 
+@pytest.mark.parametrize("heads,kvh", [(8, 2), (40, 1)])
+@pytest.mark.parametrize("lengths,group", [([700], [0, 1]), ([0], [0, 1]), ([300, 40], [0, 1, 2]), ([5, 900, 33], [0, 0, 1, 2]), ([5, 900, 33], [1, 1, 1, 1])])
+def test_groups_of_one_share_nothing(gpu, heads, kvh, lengths, group):
+    """Such groups have no tiles: every sequence reads its own table."""
+    rng = np.random.default_rng(65)
+    hd, page = 128, 16
+    table, n_page = tables(rng, lengths, page)
+    c, k, v = filled(gpu, rng, "f16", table, n_page, page, heads, kvh, hd, lengths)
+    q = rounded(rng.standard_normal((len(lengths), heads * hd)), "f16")
+    want, bound = want_decode(q, k, v, table, lengths, heads, kvh, hd, hd ** -0.5, "f16")
+    R.check(c.decode(q, table, lengths, group, [256] * (len(group) - 1)), want, bound)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_a_replayed_graph_beside_another_threads_calls(gpu, kind):
     """A graph's calls and eager ones use the same scratch: a replay from one thread falls between calls of another, never
