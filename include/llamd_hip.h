@@ -504,6 +504,76 @@ int llamd_hip_paged_decode(const llamd_hip_pages *c, const llamd_hip_batch *b, c
                            const int32_t *shared, int n_group, const void *q, int n_head, float scale,
                            int out_type, void *out);
 
+/* ---- the same over 8-bit pages ----------------------------------------------- */
+/* Not in the reference. Half the bytes of a 16-bit cache: an element is an e4m3
+ * number (OCP: 4 bits of exponent, 3 of mantissa, largest 448, no infinities)
+ * times 2^(E - 127), with one byte E, 1 to 254, for every 16 positions of a page
+ * and kv head, K and V apart.
+ *
+ * What is said above holds, with these differences. q and q_out are bf16, results
+ * bf16 or f32; products and weights are those of a bf16 cache, which holds
+ * every element exactly. paged8_store takes for 16 positions the least E with
+ * which the new ones' largest finite value fits (448 * 2^(E - 127)), or the E
+ * there where positions of the sequence before the new ones need more; where E
+ * grows, those positions' numbers are rounded again (exactly but for values below
+ * 2^-14 of the largest that fits). Each value is off by half a step: 2^-4 of itself,
+ * or 2^-10 * 2^(E - 127). Infinities are stored as NaN. What lies in the 16
+ * positions behind the new tokens is left as it was, in the E that there is now.
+ * Two sequences of one call that store into the same 16 positions of a page leave
+ * those undefined. */
+typedef struct {
+    void *k;           /* [n_page][n_head_kv][page][hd] */
+    void *v;           /* [n_page][n_head_kv][hd][page] */
+    uint8_t *k_scale;  /* [n_page][n_head_kv][page / 16], 4-byte aligned */
+    uint8_t *v_scale;
+    int n_page;
+    int page;          /* positions per page: 16, 32, 64, 128 or 256 */
+    int n_head_kv;
+    int hd;            /* 64, 128 or 256 */
+} llamd_hip_pages8;
+int llamd_hip_paged8_store(const llamd_hip_pages8 *c, const llamd_hip_batch *b, const float *q, int ld_q,
+                           const float *k, int ld_k, const float *v, int ld_v, const float *q_norm,
+                           const float *k_norm, float eps, const double *freqs, int n_rot,
+                           int interleaved, float mscale, int n_head, void *q_out);
+int llamd_hip_paged8_prompt(const llamd_hip_pages8 *c, const llamd_hip_batch *b, const void *q, int n_head,
+                            float scale, int out_type, void *out);
+int llamd_hip_paged8_decode(const llamd_hip_pages8 *c, const llamd_hip_batch *b, const int32_t *group,
+                            const int32_t *shared, int n_group, const void *q, int n_head, float scale,
+                            int out_type, void *out);
+
+/* ---- sampling -------------------------------------------------------------------- */
+/* Not in the reference (its llamd-sampling crate is empty; next tokens are
+ * argmax). One token per row of logits [n_seq][ld], of which n count (up to
+ * 2^20), by the row's rule and its random number u, uniform in [0, 1). All
+ * device pointers; asynchronous on the library stream; 0 or -1. Rules and
+ * numbers are read on the device, so a captured call follows them.
+ *
+ *   weights w = exp((x - max) / temperature)
+ *   order: x falling, of equal ones the lower id first
+ *   top_k: the first top_k in that order
+ *   top_p: of these, with S the sum of their w, those whose predecessors sum to
+ *     less than top_p * S
+ *   min_p: of these, those with w >= min_p
+ *   (the first is always kept)
+ *   ids: the first id, in rising order, at which the running sum of kept w
+ *     exceeds u times the sum of all kept w;  prob (may be NULL): its w / that sum
+ *
+ * temperature not above 0 (or NaN): the first in that order (argmax), prob 1.
+ * NaN logits count as -infinity, which is never drawn; a row of nothing else
+ * gives id -1, prob 0. +infinity: one of those that are. u below 0 takes the first
+ * id kept, u from 1 on (or NaN) the last. Weights are held to 2^-44 and added
+ * exactly, so results do not depend on timing; a weight below 2^-44 is 0. */
+typedef struct {
+    float temperature;
+    int32_t top_k;  /* 0 or less, n or more: all */
+    float top_p;    /* 1 or more, NaN: all */
+    float min_p;    /* 0 or less, NaN: all */
+} llamd_hip_sampling;
+/* how [n_seq] 16-byte aligned, u [n_seq] 8; ids and prob [n_seq] overlap nothing
+ * that the call reads. */
+int llamd_hip_sample(const float *logits, int ld, int n, int n_seq, const llamd_hip_sampling *how,
+                     const double *u, int32_t *ids, float *prob);
+
 /* ---- one MoE decode layer (R8 router -> R9 route -> R11 moe_ffn -> R12) ---- */
 /* Not in the reference as one call: DeviceModel::queue_token's MoE phases
  * (crates/llamd-runtime/src/device.rs:486-655) behind a handle.

@@ -199,6 +199,10 @@ SIGNATURES = {
     "llamd_hip_paged_store": (i32, [vp, vp, vp, i32, vp, i32, vp, i32, vp, vp, f, vp, i32, i32, f, i32, vp]),
     "llamd_hip_paged_prompt": (i32, [vp, vp, vp, i32, f, i32, vp]),
     "llamd_hip_paged_decode": (i32, [vp, vp, vp, vp, i32, vp, i32, f, i32, vp]),
+    "llamd_hip_paged8_store": (i32, [vp, vp, vp, i32, vp, i32, vp, i32, vp, vp, f, vp, i32, i32, f, i32, vp]),
+    "llamd_hip_paged8_prompt": (i32, [vp, vp, vp, i32, f, i32, vp]),
+    "llamd_hip_paged8_decode": (i32, [vp, vp, vp, vp, i32, vp, i32, f, i32, vp]),
+    "llamd_hip_sample": (i32, [vp, i32, i32, i32, vp, vp, vp, vp]),
     # host-side synthetic data (llamd_rs_amd/csrc/host/synth.cpp)
     "llamd_synth_normal": (None, [u64, f, vp, sz]),
     "llamd_synth_f32_to_f16": (u16, [f]),

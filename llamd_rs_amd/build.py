@@ -52,8 +52,9 @@ HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", f"-I{R
 
 HIP_SOURCES = ["q6k_mv.hip", "q8k.hip", "moe.hip", "moe_decode.hip", "group.hip", "norm.hip",
                "decode.hip", "noalloc.hip", "compat.hip", "paged_store.hip",
-               "paged_attend_f32.hip", "paged_attend_f16.hip", "paged_attend_bf16.hip"]
-HOST_HIP_SOURCES = ["capi.cpp", "model.cpp", "compat_abi.cpp", "paged.cpp"]  # host code that calls the HIP runtime
+               "paged_attend_f32.hip", "paged_attend_f16.hip", "paged_attend_bf16.hip",
+               "paged_attend_e4m3.hip", "paged8_store.hip", "sampling.hip"]
+HOST_HIP_SOURCES = ["capi.cpp", "model.cpp", "compat_abi.cpp", "paged.cpp", "sample.cpp"]  # host code that calls the HIP runtime
 HOST_SOURCES = ["host/layout.cpp", "host/synth.cpp", "host/gguf.cpp"]
 
 

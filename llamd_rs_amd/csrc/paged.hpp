@@ -10,8 +10,9 @@
 namespace llamd {
 
 enum PagedType { PT_F32 = 0, PT_F16 = 1, PT_BF16 = 30 };  // ggml's numbers
+constexpr int SCALE_BLOCK = 16, SCALE_LOG = 4;            // positions of 8-bit pages that share a scale
 
-// The cache and the batch (llamd_hip_pages, llamd_hip_batch), as the kernels take them.
+// The cache and the batch (llamd_hip_pages or llamd_hip_pages8, llamd_hip_batch), as the kernels take them.
 struct PagedArgs {
     void *k, *v;           // [n_page][n_kv_head][page][hd], [n_page][n_kv_head][hd][page]
     const int32_t *start;  // [n_seq + 1]; null: sequence s has token s
@@ -20,6 +21,7 @@ struct PagedArgs {
     int n_page, page_log, n_kv_head, hd;
     int n_seq, n_tok, max_page;
     int n_head, group;  // group = n_head / n_kv_head
+    uint8_t *k_scale, *v_scale;  // 8-bit pages: [n_page][n_kv_head][page / 16]
 };
 
 struct PagedStoreArgs {
@@ -51,5 +53,8 @@ int launch_paged_store(const PagedStoreArgs &a, int type, hipStream_t st);
 int launch_paged_attend_f32(const PagedAttendArgs &a, bool decode, hipStream_t st);
 int launch_paged_attend_f16(const PagedAttendArgs &a, bool decode, hipStream_t st);
 int launch_paged_attend_bf16(const PagedAttendArgs &a, bool decode, hipStream_t st);
+int launch_paged_attend_e4m3(const PagedAttendArgs &a, bool decode, hipStream_t st);
+// paged8_store.hip
+int launch_paged8_store(const PagedStoreArgs &a, hipStream_t st);
 
 }  // namespace llamd

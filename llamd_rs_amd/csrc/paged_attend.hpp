@@ -247,16 +247,27 @@ __device__ __forceinline__ int2 part_steps(int steps, int parts, int z) {
 
 // Where a kv head's pages are.
 template <class E> struct Pages {
-    const typename E::T *k, *v;
+    const typename E::P *k, *v;
     const int32_t *table;
     size_t step;  // elements between pages
     int mask;     // positions per page - 1
+    const uint8_t *k_scale, *v_scale;  // 8-bit pages: of this kv head, step >> SCALE_LOG / HD bytes between pages
 };
 template <class E, int HD>
 __device__ __forceinline__ Pages<E> pages_of(const PagedArgs &p, int seq, int kvh) {
     const size_t head = (size_t)kvh * HD << p.page_log;
-    return {(const typename E::T *)p.k + head, (const typename E::T *)p.v + head, p.table + (size_t)seq * p.max_page,
-            (size_t)p.n_kv_head * HD << p.page_log, (1 << p.page_log) - 1};
+    Pages<E> x = {(const typename E::P *)p.k + head, (const typename E::P *)p.v + head, p.table + (size_t)seq * p.max_page,
+                  (size_t)p.n_kv_head * HD << p.page_log, (1 << p.page_log) - 1};
+    if constexpr (bytes_of<E>) {
+        const size_t first = (size_t)kvh << (p.page_log - SCALE_LOG);
+        x.k_scale = p.k_scale + first;
+        x.v_scale = p.v_scale + first;
+    }
+    return x;
+}
+// Where the scale of a position of a page lies.
+template <class E> __device__ __forceinline__ size_t scale_at(const PagedArgs &p, const Pages<E> &pg, int page, int pos) {
+    return (((size_t)page * p.n_kv_head) << (p.page_log - SCALE_LOG)) + ((pos & pg.mask) >> SCALE_LOG);
 }
 
 __device__ __forceinline__ float over(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
@@ -275,20 +286,103 @@ __device__ __forceinline__ uint32_t fresh(uint32_t x) {
     return x;
 }
 
-// A row's runs for the first product of 16 rows.
+// A row's runs for the first product of 16 rows. 8-bit pages: 16 bytes of K are the runs of two steps.
 template <class E, int HD>
 __device__ __forceinline__ void load_few(run4 (&q)[HD / (4 * E::RUN)], const void *from, long long at) {
     const typename E::T *x = (const typename E::T *)from + (size_t)max(at, 0LL) * HD;
     const int g = (threadIdx.x >> 4) & 3;
 #pragma unroll
-    for (int c = 0; c < HD / (4 * E::RUN); ++c) q[c] = *(const run4 *)(x + (4 * c + g) * E::RUN);
+    for (int c = 0; c < HD / (4 * E::RUN); ++c)
+        q[c] = *(const run4 *)(x + (bytes_of<E> ? 2 * (4 * (c / 2) + g) + c % 2 : 4 * c + g) * E::RUN);
+}
+
+// Positions of a step of 16 rows.
+template <class E> constexpr int few_positions = bytes_of<E> ? 64 : 32;
+
+// 16 rows against 8-bit pages (see attend_few_runs): steps of 64 positions, position 16 g + 8 j + 4 b + i of a step in register i of
+// block b and half j of group g's lanes.
+template <int HD, int STRIDE, bool AGAIN>
+__device__ __forceinline__ void attend_few8(const PagedArgs &p, const Pages<ElemE4M3> &pg, int n_kv, int limit, int begin,
+                                            int end, const run4 (&q)[HD / 32], float scale, FewState<ElemE4M3, HD> &st) {
+    typedef ElemE4M3 E;
+    typedef FewState<E, HD> S;
+    const int all = wave_reduce(limit, 0x7FFFFFFF, [](int x, int y) { return min(x, y); });
+    const auto step = [&](auto masked, int t0) {
+        const int lane = (AGAIN ? fresh(threadIdx.x) : threadIdx.x) & 63, g = lane >> 4, m = lane & 15;
+        // the lane's page as a row of K (16 positions on per 4 rows), and as a group of positions
+        const int k0 = t0 + SCALE_BLOCK * (m >> 2), v0 = t0 + SCALE_BLOCK * g;
+        const int idk = pg.table[min(k0, n_kv - 1) >> p.page_log], idv = pg.table[min(v0, n_kv - 1) >> p.page_log];
+        const bool ok = (unsigned)idv < (unsigned)p.n_page;
+        // bit i: position t0 + i can be read
+        const unsigned long long valid = __ballot(ok && t0 + lane < n_kv);
+        if (!masked && valid != ~0ull) return false;
+        const int page = ok ? idv : 0, page_k = (unsigned)idk < (unsigned)p.n_page ? idk : 0;
+        const size_t at = scale_at(p, pg, page, v0);
+        const uint32_t ek = pg.k_scale[at], ev = pg.v_scale[at];
+        run4 k[4][HD / 64], v[S::DB];
+        const uint8_t *x = pg.k + (size_t)page_k * pg.step + (size_t)((k0 & pg.mask) + (m & 3)) * HD + g * 16;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) k[b][c] = *(const run4 *)(x + 4 * b * HD + 64 * c);
+        const uint8_t *y = pg.v + (size_t)page * pg.step + ((size_t)m << p.page_log) + (v0 & pg.mask);
+        const auto v_run = [&](int d, uint32_t plus) { return *(const run4 *)(y + (((size_t)(16 * d) << p.page_log) + plus)); };
+        if constexpr (!masked) {
+#pragma unroll
+            for (int d = 0; d < S::DB; ++d) v[d] = v_run(d, 0u);
+        }
+        v4f s[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) s[b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    s[b] = mul16<E>(widen(k[b][c][2 * h], k[b][c][2 * h + 1], 1.0f), q[2 * c + h], s[b]);
+        if constexpr (masked) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = SCALE_BLOCK * g + 4 * b + i;
+                    s[b][i] = t0 + n < limit && (valid >> n & 1) ? s[b][i] : NEG_INF;
+                }
+        }
+        // (what lies in place of a scale that is none may be anything)
+        const bool some = valid >> (SCALE_BLOCK * g) & 1;
+        // (inside f32's range: 0 scores, and masked ones, stay what they are)
+        st.softmax(s, fminf(fmaxf(scale * unit_of(some ? ek : 127u), 0x1p-126f), 0x1.fffffep127f));
+        const float unit = unit_of(some ? ev : 127u);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const run4 w = S::weights(s, j);
+            if constexpr (masked) {
+                st.add_masked(
+                    [&](int d, uint32_t plus) {
+                        const run4 r = v_run(d, plus);
+                        return widen(r[2 * j], r[2 * j + 1], unit);
+                    },
+                    (uint32_t)(valid >> (SCALE_BLOCK * g + 8 * j)), w, t0 + 8 * j, limit);
+            } else {
+#pragma unroll
+                for (int d = 0; d < S::DB; ++d) st.o[d] = mul16<E>(widen(v[d][2 * j], v[d][2 * j + 1], unit), w, st.o[d]);
+            }
+        }
+        return true;
+    };
+    int t0 = begin;
+    while (!AGAIN && t0 < end && t0 + 64 <= all && step(std::false_type{}, t0)) t0 += STRIDE;
+    for (; t0 < end; t0 += STRIDE) step(std::true_type{}, t0);
 }
 
 // 16 rows against the positions t0 .. t0 + 31 for t0 = begin, begin + STRIDE, ... below end; begin and STRIDE are multiples of
-// 32, uniform over the wave. K of a step (and V, where the registers allow) is loaded whole before the first product.
-template <class E, int HD, int STRIDE, bool AGAIN = false>
-__device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &pg, int n_kv, int limit, int begin, int end,
-                                           const run4 (&q)[HD / (4 * E::RUN)], float scale, FewState<E, HD> &st) {
+// 32 (few_positions), uniform over the wave. K of a step (and V, where the registers allow) is loaded whole before the first
+// product.
+template <class E, int HD, int STRIDE, bool AGAIN>
+__device__ __forceinline__ void attend_few_runs(const PagedArgs &p, const Pages<E> &pg, int n_kv, int limit, int begin, int end,
+                                                const run4 (&q)[HD / (4 * E::RUN)], float scale, FewState<E, HD> &st) {
     typedef typename E::T T;
     typedef FewState<E, HD> S;
     constexpr int RUN = E::RUN;
@@ -363,6 +457,13 @@ __device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &p
     for (; t0 < end; t0 += STRIDE) step(std::true_type{}, t0);
 }
 
+template <class E, int HD, int STRIDE, bool AGAIN = false>
+__device__ __forceinline__ void attend_few(const PagedArgs &p, const Pages<E> &pg, int n_kv, int limit, int begin, int end,
+                                           const run4 (&q)[HD / (4 * E::RUN)], float scale, FewState<E, HD> &st) {
+    if constexpr (bytes_of<E>) attend_few8<HD, STRIDE, AGAIN>(p, pg, n_kv, limit, begin, end, q, scale, st);
+    else attend_few_runs<E, HD, STRIDE, AGAIN>(p, pg, n_kv, limit, begin, end, q, scale, st);
+}
+
 // Rows of a wave of paged_tiles (32, from `limit` and `at` of their lanes) once more, 16 at a time straight from the pages,
 // every infinity or NaN in V added only where it belongs. Slow, since a workgroup does it alone: one such value in a tile that
 // some row sees in part makes a prompt of 4096 tokens 1128 us instead of 160, 63 of them 1545; 512 tokens after 7000 410
@@ -380,7 +481,7 @@ __device__ __forceinline__ void attend_again(const PagedAttendArgs &a, const Par
         load_few<E, HD>(q, a.q, row);
         FewState<E, HD> st;
         st.clear();
-        attend_few<E, HD, 32, true>(a.p, pages_of<E, HD>(a.p, seq, kvh), n_kv, lim, begin, end, q, a.scale, st);
+        attend_few<E, HD, few_positions<E>, true>(a.p, pages_of<E, HD>(a.p, seq, kvh), n_kv, lim, begin, end, q, a.scale, st);
         const float l = add_groups(st.l), f = over(l);
         if (part) {
             if (g == 0) parts.ml[slot * 32 + from] = make_float2(st.m, l);
@@ -399,7 +500,8 @@ __device__ __forceinline__ void attend_again(const PagedAttendArgs &a, const Par
 // Least positions of a part of paged_few: one step of each wave. A sequence has no more than FEW_PARTS parts (each costs the
 // join) unless they would have more than LONG_PART steps (1 x 9000 positions: 17 us, in 71 parts 19.4; 1 x 60000: 35 us in
 // 118 parts, in 64 43).
-constexpr int FEW_STEP = 128, FEW_PARTS = 64, LONG_PART = 4;
+template <class E> constexpr int few_step = 4 * few_positions<E>;
+constexpr int FEW_PARTS = 64, LONG_PART = 4;
 
 // A sequence's own positions in a decode batch (behind those that its group shares), cut into parts.
 struct Own {
@@ -424,7 +526,7 @@ struct DecodePlan {
     Own mine;  // of sequence `lane`
     int cut;   // positions per part, so that all parts together are about as many as the host wants
 };
-__device__ __forceinline__ DecodePlan decode_plan(const PagedAttendArgs &a, const Split &sp) {
+template <class E> __device__ __forceinline__ DecodePlan decode_plan(const PagedAttendArgs &a, const Split &sp) {
     const int lane = threadIdx.x & 63;
     DecodePlan d;
     d.mine = own_of(a, lane);
@@ -436,9 +538,9 @@ __device__ __forceinline__ DecodePlan decode_plan(const PagedAttendArgs &a, cons
         most = max(most, n);
     }
     most = wave_reduce(most, 0, [](int x, int y) { return max(x, y); });
-    // (2^31 - 128 at most: one part)
+    // (a step less than 2^31 at most: one part)
     const double row = min(most * sp.per_row, (double)LONG_PART);
-    d.cut = (int)min(max(ceil(max(wave_sum_d(sum) * sp.per_item, row)), 1.0) * FEW_STEP, 2147483520.0);
+    d.cut = (int)min(max(ceil(max(wave_sum_d(sum) * sp.per_item, row)), 1.0) * few_step<E>, 2147483648.0 - few_step<E>);
     return d;
 }
 // The sequence of part number `part` (its number within the sequence afterwards); -1: past the last.
@@ -500,7 +602,7 @@ __device__ __forceinline__ void few_rows(const PagedAttendArgs &a, const Split &
     int begin, end, parts, kvh;
     size_t slot;
     if constexpr (DECODE) {
-        const DecodePlan plan = decode_plan(a, sp);
+        const DecodePlan plan = decode_plan<E>(a, sp);
         const int cut = plan.cut;
         int unit = at.x;
         Own own;
@@ -520,19 +622,19 @@ __device__ __forceinline__ void few_rows(const PagedAttendArgs &a, const Split &
         int tile = unit;
         if (!prompt_tile<16>(p, tile, t)) return;
         r = prompt_row<16>(p, tile, t, kvh, m);
-        const int steps = (t.top + FEW_STEP - 1) / FEW_STEP;
+        const int steps = (t.top + few_step<E> - 1) / few_step<E>;
         parts = parts_of(steps, sp.parts, 1);
         if (at.y >= parts) return;
         const int2 range = part_steps(steps, parts, at.y);
-        begin = range.x * FEW_STEP;
-        end = min(range.y * FEW_STEP, t.top);
+        begin = range.x * few_step<E>;
+        end = min(range.y * few_step<E>, t.top);
         slot = (size_t)(unit * p.n_kv_head + kvh) * sp.parts + at.y;
     }
     run4 q[S::QS];
     load_few<E, HD>(q, a.q, r.at);
     S st;
     st.clear();
-    attend_few<E, HD, FEW_STEP>(p, pages_of<E, HD>(p, t.seq, kvh), t.n_kv, r.limit, begin + 32 * wave, end, q, a.scale, st);
+    attend_few<E, HD, few_step<E>>(p, pages_of<E, HD>(p, t.seq, kvh), t.n_kv, r.limit, begin + few_positions<E> * wave, end, q, a.scale, st);
 
     // the four waves' positions together: every wave adds a quarter of the dimensions
     const float mine = add_groups(st.l);
@@ -619,6 +721,10 @@ template <class E, int HD> struct TileShared {
     int least[8];
 };
 
+// The runs as they are, or of 8-bit pages the widened ones.
+template <int N, int M> __device__ __forceinline__ run4 (&of_raw(run4 (&x)[N], run4 (&)[M]))[N] { return x; }
+template <int N> __device__ __forceinline__ run4 (&of_raw(run2 (&)[N], run4 (&x)[N]))[N] { return x; }
+
 // W waves of 32 rows each. at.x: a tile and kv head, at.y: a part of its positions.
 template <class E, int HD, int W, bool PREFIX>
 __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split &sp, Place at, TileShared<E, HD> &shared) {
@@ -629,6 +735,8 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
     constexpr int SUB = KT / 32;
     constexpr int KCH = HD / RUN, VCH = KT / RUN;                 // 16-byte runs per row of a tile
     constexpr int N = KT * KCH / THREADS;                             // loads of each thread per K (V) tile
+    typedef std::conditional_t<bytes_of<E>, run2, run4> Raw;          // a run as it lies in a page
+    typedef typename E::P P;
     auto &lds = shared.lds;
     auto &least = shared.least;
     const PagedArgs &p = a.p;
@@ -683,14 +791,17 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
     const bool one_page = 1 << p.page_log >= KT;
     // (step's page: the table's entry for its position of this lane)
     const auto page_or_0 = [&](int id) { return (unsigned)id < (unsigned)p.n_page ? id : 0; };
-    const auto load_k = [&](run4 (&x)[N], int step, int id) {
+    // (8-bit pages: and the scales, of the lane's position for K, of its run for V)
+    uint32_t k_unit = 0, v_unit = 0;
+    const auto load_k = [&](Raw (&x)[N], int step, int id) {
         const int t0 = step * KT;
         const uint32_t tid = fresh(threadIdx.x);
+        if constexpr (bytes_of<E>) k_unit = g.k_scale[scale_at(p, g, page_or_0(id), t0 + (tid & (KT - 1)))];
         if (one_page) {
             const int page = page_or_0(__builtin_amdgcn_readfirstlane(id));
             const char *k = (const char *)(g.k + (size_t)page * g.step + (size_t)(t0 & g.mask) * HD);
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = *(const run4 *)(k + i * (THREADS * 16) + tid * 16);
+            for (int i = 0; i < N; ++i) x[i] = *(const Raw *)(k + i * (THREADS * sizeof(Raw)) + tid * sizeof(Raw));
         } else {
             // (a wave's 64 runs are rows of one page: 64 / KCH rows from a multiple of that)
             static_assert(64 / KCH <= 16, "a wave's runs in one page");
@@ -700,26 +811,29 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
                 const int r = (THREADS * i + 64 * wave) / KCH;
                 const char *k = (const char *)(g.k + (size_t)__builtin_amdgcn_readlane(page, r) * g.step +
                                                (size_t)((t0 + r) & g.mask) * HD);
-                x[i] = *(const run4 *)(k + (tid & 63) * 16);
+                x[i] = *(const Raw *)(k + (tid & 63) * sizeof(Raw));
             }
         }
     };
-    const auto load_v = [&](run4 (&x)[N], int step, int id) {
+    const auto load_v = [&](Raw (&x)[N], int step, int id) {
         const int t0 = step * KT;
         const uint32_t tid = fresh(threadIdx.x);
         if (one_page) {
             const int page = page_or_0(__builtin_amdgcn_readfirstlane(id));
+            if constexpr (bytes_of<E>) v_unit = g.v_scale[scale_at(p, g, page, t0 + tid % VCH * RUN)];
             const char *v = (const char *)(g.v + (size_t)page * g.step + (t0 & g.mask));
-            const uint32_t v_lane = (uint32_t)(((tid / VCH) << p.page_log) + (tid % VCH) * RUN) * (uint32_t)sizeof(T);
+            const uint32_t v_lane = (uint32_t)(((tid / VCH) << p.page_log) + (tid % VCH) * RUN) * (uint32_t)sizeof(P);
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                x[i] = *(const run4 *)(v + (size_t)i * ((THREADS / VCH * sizeof(T)) << p.page_log) + v_lane);
+                x[i] = *(const Raw *)(v + (size_t)i * ((THREADS / VCH * sizeof(P)) << p.page_log) + v_lane);
         } else {
             const int page = page_or_0(id);
             const uint32_t c = tid % VCH;
-            const T *v = g.v + (size_t)__shfl(page, c * RUN, WAVE) * g.step + ((t0 + c * RUN) & g.mask);
+            const int of_run = __shfl(page, c * RUN, WAVE);
+            if constexpr (bytes_of<E>) v_unit = g.v_scale[scale_at(p, g, of_run, t0 + c * RUN)];
+            const P *v = g.v + (size_t)of_run * g.step + ((t0 + c * RUN) & g.mask);
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = *(const run4 *)(v + ((size_t)((THREADS * i + tid) / VCH) << p.page_log));
+            for (int i = 0; i < N; ++i) x[i] = *(const Raw *)(v + ((size_t)((THREADS * i + tid) / VCH) << p.page_log));
         }
     };
     // positions of a step that can be read
@@ -727,21 +841,33 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
         return __ballot((unsigned)id < (unsigned)p.n_page && step * KT + (lane & (KT - 1)) < t.n_kv);
     };
     // the loaded runs into their buffer; V at positions that cannot be read may be anything: 0 in its place
-    const auto put_k = [&](const run4 (&x)[N], int step) {
+    // (8-bit pages: as bf16, once for all rows; widened by each wave for its own, the tile's 128 conversions per wave
+    // would cost as much as its products)
+    const auto put_k = [&](const Raw (&x)[N], int step) {
         run4 *to = lds[step & 1][0];
         const uint32_t tid = fresh(threadIdx.x);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t r = (THREADS * i + tid) / KCH;
-            to[r * KCH + ((tid % KCH) ^ k_swap(r))] = x[i];
+            run4 y;
+            if constexpr (bytes_of<E>)  // (the wave's rows have one scale)
+                y = widen(x[i][0], x[i][1], unit_of(__builtin_amdgcn_readlane(k_unit, (THREADS * i + 64 * wave) / KCH)));
+            else y = x[i];
+            to[r * KCH + ((tid % KCH) ^ k_swap(r))] = y;
         }
     };
     // (a position that a row does not attend to weighs nothing, whatever lies there; but nothing times an infinity or NaN
     // is NaN: where some row does not see all of a tile that has one, the rows are done again, attend_again)
     uint32_t bad = 0;
-    const auto put_v = [&](run4 (&x)[N], int step, unsigned long long valid) {
+    const auto put_v = [&](Raw (&raw)[N], int step, unsigned long long valid) {
         run4 *to = lds[step & 1][1];
         const uint32_t tid = fresh(threadIdx.x);
+        run4 wide_runs[bytes_of<E> ? N : 1];
+        if constexpr (bytes_of<E>) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) wide_runs[i] = widen(raw[i][0], raw[i][1], unit_of(v_unit));
+        }
+        run4 (&x)[N] = of_raw(raw, wide_runs);
         if (valid != ~0ull) {
 #pragma unroll
             for (int i = 0; i < N; ++i) x[i] = keep_elements<E>(x[i], (uint32_t)(valid >> (tid % VCH * RUN)));
@@ -759,7 +885,7 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
 
     if (range.x < range.y) {
         const int last = range.y - 1;
-        run4 kr[N], vr[N];
+        Raw kr[N], vr[N];
         load_k(kr, range.x, next);
         load_v(vr, range.x, next);
         unsigned long long valid = readable(range.x, next);
@@ -1025,7 +1151,7 @@ __global__ __launch_bounds__(256) void paged_join(PagedAttendArgs a, Split sp) {
     const PagedArgs &p = a.p;
     const int unit = blockIdx.x / p.n_kv_head, kvh = blockIdx.x % p.n_kv_head;
     constexpr bool FEW = R == 16;
-    constexpr int STEP = FEW ? FEW_STEP : tile_positions<E, HD>();
+    constexpr int STEP = FEW ? few_step<E> : tile_positions<E, HD>();
     int tile = unit;
     Tile t;
     if (!prompt_tile<R>(p, tile, t)) return;
@@ -1050,7 +1176,7 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
     const PagedArgs &p = a.p;
     const int lane = threadIdx.x & 63, seq = blockIdx.x, per = (p.group + 15) / 16;
     const int kvh = blockIdx.y / per, head = (blockIdx.y % per) * 16;
-    const DecodePlan plan = decode_plan(a, sp);
+    const DecodePlan plan = decode_plan<E>(a, sp);
     Own own;
     const int before = parts_before(a, plan, seq, own), units = own.units(plan.cut);
     const bool prefix = own.shared && own.n;
@@ -1131,7 +1257,7 @@ int prompt_few(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
     // as many workgroups as are resident (16 tokens after 12000 positions: 33.5 us, for 2 per CU 42, for 4 40)
     const TilePlan plan = plan_tiles((long long)p.n_tok * p.group, std::min(p.n_seq, p.n_tok), 16, p.n_kv_head, (HD <= 128 ? 3 : 2) * CUS,
-                                     ((long long)p.max_page << p.page_log) / FEW_STEP, 128);
+                                     ((long long)p.max_page << p.page_log) / few_step<E>, 128);
     const long long tiles = plan.tiles;
     Split sp{};
     sp.parts = plan.parts;
@@ -1176,10 +1302,10 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
     // 164 MB: 37.5 us, 2 per CU 44, 1 per CU 51; all of 2000, 263 MB: 52.6, 51.6, 47.5); a row's should fill the GPU once
     // where there are few columns
     const int target = std::min(std::max(1, 4 * CUS / cols), JOIN_MOST - 66);
-    sp.per_item = 1.0 / ((double)target * FEW_STEP);
-    sp.per_row = 1.0 / ((double)std::max(FEW_PARTS, CUS / cols) * FEW_STEP);
+    sp.per_item = 1.0 / ((double)target * few_step<E>);
+    sp.per_row = 1.0 / ((double)std::max(FEW_PARTS, CUS / cols) * few_step<E>);
     const long long items = std::min<long long>((long long)p.n_seq + target + 1,
-                                                (long long)p.n_seq * ((top + FEW_STEP - 1) / FEW_STEP));
+                                                (long long)p.n_seq * ((top + few_step<E> - 1) / few_step<E>));
     long long tiles = 0, slots = 0;
     if (a.n_groups) {
         // (groups of one sequence share nothing)
@@ -1191,7 +1317,7 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
         slots = tiles * p.n_kv_head * sp.parts * 4;
     }
     if (items * cols > 0x7FFFFFFF / 512 || cols > 65535 || tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
-    const bool join = a.n_groups || top > FEW_STEP;
+    const bool join = a.n_groups || top > few_step<E>;
     if (join && !room(sp, slots, (size_t)items * cols, std::min(p.group, 16), HD)) return -1;
     if (a.n_groups) {
         const long long nx = tiles * p.n_kv_head, grid = nx * sp.parts + items * cols;

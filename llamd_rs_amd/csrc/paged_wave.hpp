@@ -20,7 +20,6 @@
 namespace llamd {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef uint32_t run4 __attribute__((ext_vector_type(4)));  // a 16-byte run of elements
 
 template <class E> struct Mma;
 template <> struct Mma<ElemF16> {
@@ -37,6 +36,7 @@ template <> struct Mma<ElemBF16> {
     }
     static constexpr uint32_t EXP = 0x7F807F80u;
 };
+template <> struct Mma<ElemE4M3> : Mma<ElemBF16> {};
 template <> struct Mma<ElemF32> {
     static __device__ __forceinline__ v16f mul(run4 a, run4 b, v16f c) {
 #pragma unroll
@@ -205,7 +205,9 @@ template <class E, int HD> struct RowState {
 
 // ---- 16 rows ----------------------------------------------------------------------
 // The same for up to 16 rows and 32 positions with 16x16 matrix instructions, whose four groups of 16 lanes hold a run each:
-// a row's values lie in four lanes, and half the registers and columns are left unused.
+// a row's values lie in four lanes, and half the registers and columns are left unused. 8-bit pages: 64 positions, two
+// such halves j, of which group g has the runs 16 g + 8 j: then 16 bytes of V are a lane's runs of both halves, and a
+// group's scores and runs are those of one scale.
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
@@ -218,6 +220,7 @@ template <> __device__ __forceinline__ v4f mul16<ElemBF16>(run4 a, run4 b, v4f c
     typedef Mma<ElemBF16>::V V;
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
 }
+template <> __device__ __forceinline__ v4f mul16<ElemE4M3>(run4 a, run4 b, v4f c) { return mul16<ElemBF16>(a, b, c); }
 template <> __device__ __forceinline__ v4f mul16<ElemF32>(run4 a, run4 b, v4f c) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -257,13 +260,14 @@ template <class E, int HD> struct FewState {
         l = 0.0f;
     }
 
-    __device__ __forceinline__ void softmax(v4f (&s)[2], float scale) {
+    // (of 8-bit pages `scale` is the lane's: its positions' unit is in it)
+    template <int N> __device__ __forceinline__ void softmax(v4f (&s)[N], float scale) {
         float top = s[0][0];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < N; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][i]);
-        top = max_groups(top) * scale;
+        top = bytes_of<E> ? max_groups(top * scale) : max_groups(top) * scale;
         if (__any(top > m + LAZY)) {
             const float m1 = fmaxf(m, top), shrink = exp2_fast(m - against(m1));
             m = m1;
@@ -273,7 +277,7 @@ template <class E, int HD> struct FewState {
         }
         const float ref = against(m);
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < N; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[b][i] = exp2_fast(__builtin_fmaf(s[b][i], scale, -ref));
@@ -281,17 +285,17 @@ template <class E, int HD> struct FewState {
             }
     }
 
-    static __device__ __forceinline__ run4 weights(const v4f (&s)[2], int c) {
+    template <int N> static __device__ __forceinline__ run4 weights(const v4f (&s)[N], int c) {
         float x[E::RUN];
 #pragma unroll
-        for (int j = 0; j < E::RUN; ++j) x[j] = E::RUN == 8 ? s[j / 4][j % 4] : s[c][j % 4];
+        for (int j = 0; j < E::RUN; ++j) x[j] = E::RUN == 8 ? s[2 * c + j / 4][j % 4] : s[c][j % 4];
         return to_run<E>(x);
     }
 
     // One step of the second product where some of V is not to be read as it stands: of the runs v(d, 0) of the dimension
     // blocks, the elements of `keep` can be read, the others may hold anything. An infinity or NaN at a position that
     // only some rows attend to gives the others nothing, not 0 * inf: such elements are left out of the product and
-    // added one position at a time (pos0 + e) to the rows that see it.
+    // added one position at a time to the rows that see it (element e of group g: pos0 + GROUP g + e).
     template <class Load>
     __device__ __forceinline__ void add_masked(Load v, uint32_t keep, run4 p, int pos0, int limit) {
         const int g = (threadIdx.x >> 4) & 3;
@@ -310,7 +314,8 @@ template <class E, int HD> struct FewState {
         for (int e = 0; e < 4 * E::RUN; ++e) {
             const uint32_t one = (e / E::RUN == g) ? 1u << (e % E::RUN) : 0u;
             if (!__any((any & one) != 0)) continue;
-            const bool seen = pos0 + e < limit;
+            constexpr int GROUP = bytes_of<E> ? SCALE_BLOCK : E::RUN;
+            const bool seen = pos0 + GROUP * (e / E::RUN) + e % E::RUN < limit;
             uint32_t none = 0;
             asm volatile("" : "+v"(none));  // the runs are read again: held in registers throughout, they would crowd out others
 #pragma unroll

@@ -302,6 +302,45 @@ def route(logits, n_used: int) -> Routing:
     return Routing(ids, w)
 
 
+SAMPLING = np.dtype([("temperature", np.float32), ("top_k", np.int32), ("top_p", np.float32), ("min_p", np.float32)])
+
+
+def sampling_rules(n_seq: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> np.ndarray:
+    """llamd_hip_sampling [n_seq] from numbers or arrays of one per sequence."""
+    r = np.zeros(n_seq, SAMPLING)
+    for name, x in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+        if np.ndim(x) > 1 or (np.ndim(x) == 1 and len(x) != n_seq):
+            raise ValueError(f"{name}: one number, or one per sequence")
+        r[name] = x
+    return r
+
+
+def _sample_device(logits_ptr, ld: int, n: int, rules: np.ndarray, u) -> tuple[np.ndarray, np.ndarray]:
+    """(ids, probabilities) of rows of device logits."""
+    n_seq = len(rules)
+    u = np.ascontiguousarray(np.broadcast_to(np.asarray(u, np.float64), (n_seq,)))
+    ids, prob = np.empty(n_seq, np.int32), np.empty(n_seq, np.float32)
+    if not n_seq:
+        return ids, prob
+    how, du = DeviceBuffer.from_array(rules), DeviceBuffer.from_array(u)
+    di, dp = DeviceBuffer(ids.nbytes), DeviceBuffer(prob.nbytes)
+    check(lib().llamd_hip_sample(logits_ptr, ld, n, n_seq, how.ptr, du.ptr, di.ptr, dp.ptr), "sample")
+    return di.download(ids), dp.download(prob)
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> tuple[np.ndarray, np.ndarray]:
+    """A token per row of logits [n_seq, n] and the probability that it was drawn with (llamd_hip_sample): u uniform
+    numbers in [0, 1), one per row; the rule's numbers for all rows or one per row."""
+    x = np.atleast_2d(_f32(logits))
+    if np.shape(u) not in ((), (len(x),)):
+        raise ValueError("u: one number per row")
+    rules = sampling_rules(len(x), temperature, top_k, top_p, min_p)
+    if not x.size:
+        raise ValueError("no logits")
+    dx = DeviceBuffer.from_array(x)  # (held until the results are back)
+    return _sample_device(dx.ptr, x.shape[1], x.shape[1], rules, u)
+
+
 def argmax(x) -> np.ndarray:
     """Row-wise argmax, lowest index on ties."""
     x = np.atleast_2d(_f32(x))
@@ -481,6 +520,19 @@ class LmHead:
         ids = self._ids.download(np.empty(nseq, np.int32))
         return logits, ids
 
+    def sample(self, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> tuple[np.ndarray, np.ndarray]:
+        """A drawn token per sequence and its probability (sample), from logits that stay on the device."""
+        x = np.atleast_2d(_f32(x))
+        nseq = x.shape[0]
+        if x.shape[1] != self.blocks * QK_K or not 0 < nseq <= self.max_seq:
+            raise ValueError("x must be [1 <= nseq <= max_seq, k]")
+        if np.shape(u) not in ((), (nseq,)):
+            raise ValueError("u: one number per sequence")
+        rules = sampling_rules(nseq, temperature, top_k, top_p, min_p)
+        self._x.upload(x)
+        check(lib().llamd_hip_lmhead_forward(self._h, self._x.ptr, nseq, self._logits.ptr, self._ids.ptr), "lmhead_forward")
+        return _sample_device(self._logits.ptr, self.rows, self.rows, rules, u)
+
     def close(self):
         if self._h:
             lib().llamd_hip_lmhead_destroy(self._h)
@@ -497,6 +549,13 @@ class Pages(C.Structure):
     """llamd_hip_pages: a paged cache's memory. k [n_page][n_head_kv][page][hd],
     v [n_page][n_head_kv][hd][page]; type is ggml's number (PAGE_TYPES)."""
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("n_page", C.c_int),
+                ("page", C.c_int), ("n_head_kv", C.c_int), ("hd", C.c_int)]
+
+
+class Pages8(C.Structure):
+    """llamd_hip_pages8: an 8-bit paged cache's memory. k and v as in Pages, bytes; a
+    scale byte for each 16 positions of a page and kv head."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n_page", C.c_int),
                 ("page", C.c_int), ("n_head_kv", C.c_int), ("hd", C.c_int)]
 
 
@@ -521,6 +580,37 @@ def from_bf16(b) -> np.ndarray:
     return (np.ascontiguousarray(b, np.uint16).astype(np.uint32) << 16).view(np.float32)
 
 
+def _e4m3_values() -> np.ndarray:
+    b = np.arange(256)
+    e, m = b >> 3 & 15, b & 7
+    x = np.where(e, (8 + m) * 2.0 ** (e - 10.0), m * 2.0 ** -9)
+    x[127] = x[255] = np.nan
+    return np.where(b < 128, x, -x).astype(np.float32)
+
+
+_E4M3 = _e4m3_values()
+
+
+def from_e4m3(b) -> np.ndarray:
+    return _E4M3[np.asarray(b, np.uint8)]
+
+
+def to_e4m3(x) -> np.ndarray:
+    """Values of up to 448 -> e4m3 bytes, rounded to nearest even; NaN for what is larger or not finite."""
+    x = np.asarray(x, np.float64)
+    a = np.abs(np.where(np.isfinite(x), x, np.inf))
+    step = 2.0 ** (np.clip(np.frexp(np.where(np.isinf(a), 0, a))[1] - 1, -6, 8) - 3)
+    a = np.rint(np.minimum(a, 1e9) / step) * step
+    code = np.searchsorted(_E4M3[:127], a.astype(np.float32)).clip(0, 126)
+    return (np.where(a > 448, 127, code) | np.where(np.signbit(x), 128, 0)).astype(np.uint8)
+
+
+def scale_byte(top) -> np.ndarray:
+    """The scale byte of 16 positions whose largest magnitude is `top`: the least E, 1 to 254, with top <= 448 * 2^(E - 127)."""
+    m, e = np.frexp(_f32(top))  # top = m 2^e, m in [1/2, 1)
+    return np.where(_f32(top) > 0, np.clip(127 + e - 9 + (m > 0.875), 1, 254), 1).astype(np.uint8)
+
+
 def rope_freqs(n_rot: int, base: float, factor: float = 1.0, orig_ctx: int = 0, beta_fast: float = 32.0,
                beta_slow: float = 1.0) -> tuple[np.ndarray, float]:
     """(radians per position [n_rot / 2] f64, magnitude): llamd_hip_rope_freqs."""
@@ -536,6 +626,8 @@ class PagedCache:
     out. A batch is (table [n_seq, max_page], length [n_seq], start [n_seq + 1]
     or None for one token each); q and results cross as f32. A program that
     keeps its data on the device fills Pages and Batch and calls the C ABI."""
+
+    calls = "llamd_hip_paged"
 
     def __init__(self, type: str, n_page: int, page: int, n_head: int, n_head_kv: int, hd: int):
         if type not in PAGE_TYPES:
@@ -596,7 +688,7 @@ class PagedCache:
         norms = [None if w is None else DeviceBuffer.from_array(_f32(w)) for w in (q_norm, k_norm)]
         fr = None if freqs is None else DeviceBuffer.from_array(np.ascontiguousarray(freqs, np.float64))
         out = DeviceBuffer.from_array(np.zeros(q.shape, self.dtype))
-        check(lib().llamd_hip_paged_store(
+        check(getattr(lib(), self.calls + "_store")(
             C.byref(self.pages), C.byref(b), dev[0].ptr, self.n_head * hd, dev[1].ptr, kvh * hd, dev[2].ptr, kvh * hd,
             *(None if w is None else w.ptr for w in norms), eps, fr and fr.ptr,
             0 if freqs is None else 2 * len(freqs), int(interleaved), mscale, self.n_head, out.ptr), "paged_store")
@@ -618,8 +710,8 @@ class PagedCache:
     def prompt(self, q, table, length, start, scale: float | None = None, f32_out: bool = False) -> np.ndarray:
         """Causal attention of the packed tokens q [n_tok, n_head * hd]."""
         def call(b, dq, scale, number, out):
-            check(lib().llamd_hip_paged_prompt(C.byref(self.pages), C.byref(b), dq.ptr, self.n_head, scale, number,
-                                               out.ptr), "paged_prompt")
+            check(getattr(lib(), self.calls + "_prompt")(C.byref(self.pages), C.byref(b), dq.ptr, self.n_head, scale, number,
+                                                         out.ptr), "paged_prompt")
         return self._attend(call, q, table, length, start, scale, f32_out)
 
     def decode(self, q, table, length, group=None, shared=None, scale: float | None = None,
@@ -632,9 +724,9 @@ class PagedCache:
                                         for x in (group, shared)]
 
         def call(b, dq, scale, number, out):
-            check(lib().llamd_hip_paged_decode(C.byref(self.pages), C.byref(b), g and g[0].ptr, g and g[1].ptr,
-                                               0 if g is None else len(shared), dq.ptr, self.n_head, scale, number,
-                                               out.ptr), "paged_decode")
+            check(getattr(lib(), self.calls + "_decode")(C.byref(self.pages), C.byref(b), g and g[0].ptr, g and g[1].ptr,
+                                                         0 if g is None else len(shared), dq.ptr, self.n_head, scale, number,
+                                                         out.ptr), "paged_decode")
         return self._attend(call, q, table, length, None, scale, f32_out)
 
     def close(self):
@@ -642,8 +734,62 @@ class PagedCache:
         self._v.close()
 
 
+class PagedCache8(PagedCache):
+    """One layer's 8-bit paged KV cache (llamd_hip_paged8_*): e4m3 numbers with a power of two for each 16 positions
+    of a page and kv head. q and results are bf16 values."""
+
+    calls = "llamd_hip_paged8"
+
+    def __init__(self, n_page: int, page: int, n_head: int, n_head_kv: int, hd: int):
+        if min(n_page, page, n_head_kv, hd) <= 0 or page % 16:
+            raise ValueError("n_page, page, n_head_kv and hd must be positive, page a multiple of 16")
+        self.type, self.n_head, self.dtype = "bf16", n_head, np.uint16
+        self.shape_k, self.shape_v = (n_page, n_head_kv, page, hd), (n_page, n_head_kv, hd, page)
+        self.shape_scale = (n_page, n_head_kv, page // 16)
+        self._k, self._v = (DeviceBuffer.from_array(np.zeros(self.shape_k, np.uint8)) for _ in range(2))
+        self._ks, self._vs = (DeviceBuffer.from_array(np.ones(self.shape_scale, np.uint8)) for _ in range(2))
+        self.pages = Pages8(self._k.ptr, self._v.ptr, self._ks.ptr, self._vs.ptr, n_page, page, n_head_kv, hd)
+
+    def read_bytes(self) -> tuple[np.ndarray, np.ndarray, np.ndarray, np.ndarray]:
+        """(K, V, K's scales, V's scales) as they lie in memory."""
+        return tuple(b.download(np.empty(shape, np.uint8)) for b, shape in (
+            (self._k, self.shape_k), (self._v, self.shape_v), (self._ks, self.shape_scale), (self._vs, self.shape_scale)))
+
+    def write_bytes(self, k, v, k_scale, v_scale):
+        for b, x, shape in ((self._k, k, self.shape_k), (self._v, v, self.shape_v), (self._ks, k_scale, self.shape_scale),
+                            (self._vs, v_scale, self.shape_scale)):
+            if np.shape(x) != shape:
+                raise ValueError(f"pages are {self.shape_k} and {self.shape_v}, scales {self.shape_scale}")
+            b.upload(np.ascontiguousarray(x, np.uint8))
+
+    def read(self) -> tuple[np.ndarray, np.ndarray]:
+        """(K, V) pages as f32."""
+        k, v, ks, vs = self.read_bytes()
+        unit = [np.exp2(np.repeat(np.maximum(s, 1).astype(np.float32), 16, 2) - 127) for s in (ks, vs)]
+        return from_e4m3(k) * unit[0][..., None], from_e4m3(v) * unit[1][:, :, None, :]
+
+    def write(self, k, v):
+        """f32 pages; each 16 positions get the scale that their largest finite value needs."""
+        if np.shape(k) != self.shape_k or np.shape(v) != self.shape_v:
+            raise ValueError(f"pages are {self.shape_k} and {self.shape_v}")
+        n_page, kvh, page, hd = self.shape_k
+        k = _f32(k).reshape(n_page, kvh, page // 16, 16 * hd)
+        v = _f32(v).reshape(n_page, kvh, hd, page // 16, 16)
+        top = [np.where(np.isfinite(x), np.abs(x), 0).max(axis) for x, axis in ((k, 3), (v, (2, 4)))]
+        ks, vs = (scale_byte(t) for t in top)
+        unit = [np.exp2(127 - s.astype(np.float64)) for s in (ks, vs)]
+        self.write_bytes(to_e4m3(k * unit[0][..., None]).reshape(self.shape_k),
+                         to_e4m3(v * unit[1][:, :, None, :, None]).reshape(self.shape_v), ks, vs)
+
+    def close(self):
+        super().close()
+        self._ks.close()
+        self._vs.close()
+
+
 __all__ = [
-    "Pages", "Batch", "PagedCache", "PAGE_TYPES", "rope_freqs", "to_bf16", "from_bf16",
+    "Pages", "Pages8", "Batch", "PagedCache", "PagedCache8", "PAGE_TYPES", "rope_freqs", "to_bf16", "from_bf16", "to_e4m3",
+    "from_e4m3", "scale_byte", "SAMPLING", "sampling_rules", "sample",
     "BlockQ8K", "DeviceInfo", "DeviceWeights", "Q8_0Weights", "MoeLayer", "LmHead", "Routing",
     "DeviceBuffer", "available", "device_count", "device_info", "quantize_q8k_on_device",
     "swiglu_q8k_on_device", "matvec_q6k", "route", "argmax", "HipError", "HipUnavailable",
