@@ -8,19 +8,20 @@
 // neither do results, and 2^20 of them stay inside 64 bits. A weight is off by 2^-44 then, of 2^20 of them the sum by 2^-24
 // at the very worst and 2^-35 by chance; a token whose weight is below that is not drawn.
 //
-// No sort: the tokens kept are those up to one border in that order, and the draw goes by index. Four launches over the
-// row in chunks of 4096:
-//   maxima: each chunk's maximum and minimum
-//   bins: counts and weights by distance from the maximum (2048 bins), in LDS and then by integer atomics
-//   border: the bins that hold the border, found by every workgroup for itself; their tokens are listed, the weights in front
-//           of them added up by chunk
-//   draw: one workgroup per row finds the border among the listed tokens by digits of (x, index), the chunk that u falls into,
-//         and the token in it
-// Rows without top-k and top-p need no border: bins adds up their chunks. A list that is too long (most logits equal) is
-// replaced by the row itself.
+// Four launches, rows in chunks of 4096:
+//   sample_scan: maximum and minimum of each chunk, and the maxima of each 64 values
+//   sample_bins, by the row's rule:
+//     top-k of up to 1024: the k-th largest of the maxima bounds the k-th largest value from below; the tokens above the
+//       bound are listed (50 of 151936: about 55 tokens)
+//     top-p (or a larger k) alone: weights (counts) by distance from the maximum, 2048 bins, in LDS and then by integer atomics
+//     neither: there is no border, the chunks' weights are added up
+//   sample_border: rows with bins only: the bins that hold the border; their tokens are listed, the weights in front of them
+//     added up by chunk
+//   sample_draw: one workgroup per row. A small top-k's tokens are sorted, cut, and sorted by index. Else the border is found
+//     among the listed tokens by digits of (x, index), then the chunk that u falls into, and the token in it. Where a list is too
+//     short (most logits equal), the row is read in its place.
 //
-// Bound: the launches and the chain inside them for few rows; reading the row three times (once from memory) and the 64-bit
-// exponentials for many.
+// Bound: for few rows the launches and the chain of steps in each; for many the 64-bit exponentials and LDS atomics of the bins.
 #include <algorithm>
 #include <mutex>
 
@@ -33,43 +34,49 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH, BINS = 2048, PER = BINS / THREADS, LIST = 2048;
+constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH, DRAW = 1024;
+constexpr int BINS = 2048, LIST = 2048, FEW = 1024, GROUP = 64, GROUPS = CHUNK / GROUP;
 constexpr int MOST_CHUNKS = SAMPLE_MOST / CHUNK;
 static_assert(MOST_CHUNKS <= THREADS, "a thread per chunk");
 constexpr double RANGE = 44.0;  // weights below 2^-44 are 0
 
+enum Mode { GREEDY, WHOLE, SMALL, BINNED };  // the maximum alone; no border; a small top-k; top-p or a larger top-k
+
 struct Extremes {
     float top, least;  // least: of the finite values
-    int at, pad;
+    int at;            // the maximum's first index
+    int pad;
 };
-// A row's scratch.
-struct Row {
-    unsigned count[BINS];
-    u64 weight[BINS];
-    u64 sum[MOST_CHUNKS];      // of the weights in front of the border's bins
-    Extremes chunk[MOST_CHUNKS];
-    unsigned listed, pad[3];
-    uint2 list[LIST];          // (index, x's bits), in any order
+// Where the border lies.
+struct Border {
+    int k_bin;             // top-k's last token's bin; -1: there are fewer than k
+    int lo, hi;            // the bins that may hold the last token kept; lo BINS, hi below: no border
+    unsigned k_count;      // tokens in front of k_bin, and their weight
+    u64 k_weight, weight;  // weight of the tokens in front of lo
+    u64 total;             // of all; with k_bin >= 0, of the tokens up to its end
 };
-
 __device__ __forceinline__ float value(float x) { return x == x ? x + 0.0f : -INFINITY; }  // (-0 is 0)
 
-// Position in the order: x falling, then index rising.
-__device__ __forceinline__ u64 place(float x, uint32_t i) {
+// A number's bits so that they rise with it, and back.
+__device__ __forceinline__ uint32_t rising(float x) {
     const uint32_t b = __float_as_uint(x);
-    const uint32_t rising = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return (u64)~rising << 32 | i;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float of_rising(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r ^ 0x80000000u : ~r); }
 
-// A row's rule, and the distance of its logits from the maximum in powers of two.
+// Position in the order: x falling, then index rising.
+__device__ __forceinline__ u64 place(float x, uint32_t i) { return (u64)~rising(x) << 32 | i; }
+
+// A row's rule.
 struct Rule {
-    double m, c;       // maximum, log2(e) / T
-    double furthest;   // min-p's
-    double per_bin;
+    double m, c;        // maximum, log2(e) / T
+    double furthest;    // min-p's
     double p;
-    int k;             // 0: all
-    bool greedy, cut;  // the maximum alone; top-k or top-p
+    float half, scale;  // half the maximum; bins per half a unit of x
+    int k;              // 0: all
+    Mode mode;
 
+    // distance from the maximum in powers of two
     __device__ __forceinline__ double distance(float x) const { return (double)x == m ? 0.0 : (m - (double)x) * c; }
     // 2^-y as a multiple of 2^-43; 0 for NaN (an infinite temperature, and a token ruled out)
     static __device__ __forceinline__ u64 weight(double y) {
@@ -92,14 +99,39 @@ struct Rule {
         const double w = __longlong_as_double(__double_as_longlong(s) + ((long long)(43 - (int)r) << 52)) + 4503599627370496.0;
         return (u64)__double_as_longlong(w) & 0xFFFFFFFFFFFFFull;
     }
-    __device__ __forceinline__ int bin(double y) const { return min((int)(y * per_bin), BINS - 1); }
     __device__ __forceinline__ bool likely(double y) const { return y <= furthest; }
+    // Rises as x falls; BINS and more: behind the bins. (Halves: the difference of any two numbers is finite.)
+    __device__ __forceinline__ int bin(float x) const {
+        return 2.0f * half == x ? 0 : (int)fminf((half - 0.5f * x) * scale, (float)BINS);
+    }
 };
 
-// The rule of a row from its chunks' extremes. All threads of the workgroup; `at`: the maximum's first index.
+// A row's scratch; behind it the maxima of its groups of 64 values.
+struct alignas(16) Row {
+    u64 weight[BINS];
+    unsigned count[BINS];
+    u64 sum[MOST_CHUNKS];  // of the kept weights, or of those in front of the border's bins
+    Border border;
+    u64 far;               // weight of the tokens behind the bins
+    unsigned listed;
+    int best;              // the maximum's first index
+    Rule rule;
+    Extremes chunk[MOST_CHUNKS];
+    uint2 list[LIST];      // (index, x's bits), in any order
+};
+struct Rows {
+    char *base;
+    size_t step;
+    int chunks;
+    __device__ __forceinline__ Row &row(int i) const { return *(Row *)(base + (size_t)i * step); }
+    __device__ __forceinline__ float *maxima(int i) const { return (float *)(base + (size_t)i * step + sizeof(Row)); }
+};
+
+// The rule of a row from its chunks' extremes; `at`: the maximum's first index.
 __device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int number, int chunks, int &at) {
-    __shared__ float tops[4], leasts[4];
-    __shared__ int places[4];
+    constexpr int W = 4;  // waves that have chunks
+    __shared__ float tops[W], leasts[W];
+    __shared__ int places[W];
     const SampleRule how = a.how[number];
     Extremes x = {-INFINITY, INFINITY, 0x7FFFFFFF, 0};
     if ((int)threadIdx.x < chunks) x = row.chunk[threadIdx.x];
@@ -110,78 +142,120 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int
     float top = tops[0], least = leasts[0];
     at = places[0];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
+    for (int w = 1; w < W; ++w) {
         argmax_step(top, at, tops[w], places[w]);
         least = fminf(least, leasts[w]);
     }
     Rule r;
     r.m = top;
     r.c = 1.4426950408889634074 / (double)how.temperature;
-    r.greedy = !(how.temperature > 0.0f) || top == -INFINITY;
     r.furthest = how.min_p > 0.0f ? fmax(-log2((double)how.min_p), 0.0) : INFINITY;
-    const double range = fmin(r.distance(least), RANGE);  // (a least of +inf: no finite value)
-    r.per_bin = range > 0.0 ? (BINS - 1) / range : 0.0;
     r.k = how.top_k > 0 && how.top_k < a.n ? how.top_k : 0;
     r.p = how.top_p < 1.0f ? fmax((double)how.top_p, 0.0) : 1.0;  // (NaN: all)
-    r.cut = r.k || r.p < 1.0;
+    // (a bound of the k-th largest needs k groups; a quarter more leaves it some choice)
+    const bool few = r.k && r.k <= FEW && (a.n <= LIST || a.n / GROUP >= r.k + r.k / 4);
+    r.mode = !(how.temperature > 0.0f) || top == -INFINITY ? GREEDY : few ? SMALL : r.k || r.p < 1.0 ? BINNED : WHOLE;
+    // How far the bins reach, in x: to the least value, or where weights end. Top-p alone: tokens beyond log2(n / (1 - p)) + 1
+    // sum to less than half of (1 - p) S, S >= 1, and are not needed to reach p S.
+    const double reach = r.k || r.p == 1.0 ? RANGE : fmin(RANGE, log2(a.n / (1.0 - r.p)) + 1.0);
+    const double range = fmin(r.m - (double)least, reach / r.c);
+    r.half = 0.5f * top;
+    r.scale = range > 0.0 ? (float)fmin((2.0 * BINS - 1.0) / range, 3e38) : 0.0f;
     return r;
 }
 
-// f(x, index) for every logit of a chunk, 16 per thread. VEC: rows are 16-byte aligned.
-template <bool VEC, class F> __device__ __forceinline__ void each(const float *x, int n, int chunk, F f) {
-    const int first = chunk * CHUNK;
-    if (first + CHUNK <= n) {
-        float v[EACH];
-        if constexpr (VEC) {
+// A chunk's logits, 16 per thread. VEC: rows are 16-byte aligned.
+template <bool VEC> struct Chunk {
+    float v[EACH];
+    int first, n;
+
+    __device__ __forceinline__ void load(const float *x, int of_row, int chunk) {
+        first = chunk * CHUNK;
+        n = of_row;
+        if (VEC && first + CHUNK <= n) {
 #pragma unroll
             for (int j = 0; j < EACH / 4; ++j) *(float4 *)(v + 4 * j) = *(const float4 *)(x + first + (j * THREADS + threadIdx.x) * 4);
         } else {
 #pragma unroll
-            for (int j = 0; j < EACH; ++j) v[j] = x[first + j * THREADS + threadIdx.x];
+            for (int j = 0; j < EACH; ++j) v[j] = index(j) < n ? x[index(j)] : -INFINITY;
         }
-#pragma unroll
-        for (int j = 0; j < EACH; ++j)
-            f(value(v[j]), first + (VEC ? (j / 4 * THREADS + (int)threadIdx.x) * 4 + j % 4 : j * THREADS + (int)threadIdx.x));
-    } else {
-        for (int i = first + threadIdx.x; i < n; i += THREADS) f(value(x[i]), i);
     }
+    __device__ __forceinline__ int index(int j) const {
+        return first + (VEC ? (j / 4 * THREADS + (int)threadIdx.x) * 4 + j % 4 : j * THREADS + (int)threadIdx.x);
+    }
+    // f(x, index) for each; -infinity behind the row
+    template <class F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) f(value(v[j]), index(j));
+    }
+};
+
+// Sums over the wave, lane by lane.
+__device__ __forceinline__ unsigned wave_scan(unsigned x) { return (unsigned)wave_incl_sum_i((int)x); }
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 dpp64(u64 x) {
+    return (u64)(unsigned)dpp<CTRL, ROWS, ROWS == 0xF>(0, (int)(x >> 32)) << 32 | (unsigned)dpp<CTRL, ROWS, ROWS == 0xF>(0, (int)x);
+}
+__device__ __forceinline__ u64 wave_scan(u64 x) {
+    x += dpp64<DPP_ROW_SHR1, 0xF>(x);
+    x += dpp64<DPP_ROW_SHR2, 0xF>(x);
+    x += dpp64<DPP_ROW_SHR4, 0xF>(x);
+    x += dpp64<DPP_ROW_SHR8, 0xF>(x);
+    x += dpp64<DPP_BCAST15, 0xA>(x);
+    x += dpp64<DPP_BCAST31, 0xC>(x);
+    return x;
+}
+__device__ __forceinline__ u64 last_lane(u64 x) {
+    return (u64)(unsigned)readlane63((int)(x >> 32)) << 32 | (unsigned)readlane63((int)x);
 }
 
-// Inclusive sums over the threads' numbers, and all threads' sum.
-template <class T> __device__ __forceinline__ T scan(T mine, T &total) {
-    __shared__ T waves[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) {
-        const T x = __shfl_up(mine, s, 64);
-        if (lane >= s) mine += x;
-    }
-    __syncthreads();  // (a scan before this one is read)
-    if (lane == 63) waves[wave] = mine;
+// Inclusive sums over the workgroup's T threads of a count and a weight, and the sums of all.
+template <int T>
+__device__ __forceinline__ void scan(unsigned &count, u64 &weight, unsigned &counts, u64 &weights) {
+    constexpr int W = T / 64;
+    __shared__ unsigned c[W];
+    __shared__ u64 w[W];
+    const int wave = threadIdx.x >> 6;
+    count = wave_scan(count);
+    weight = wave_scan(weight);
+    __syncthreads();  // (what the scan before this one left is read)
+    if ((threadIdx.x & 63) == 63) c[wave] = count, w[wave] = weight;
     __syncthreads();
-    total = 0;
+    counts = 0;
+    weights = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) mine += waves[w];
-        total += waves[w];
+    for (int i = 0; i < W; ++i) {
+        const unsigned ci = c[i];
+        const u64 wi = w[i];
+        if (i < wave) count += ci, weight += wi;
+        counts += ci;
+        weights += wi;
     }
-    return mine;
+}
+template <int T> __device__ __forceinline__ void scan(u64 &weight, u64 &weights) {
+    unsigned none = 0, all;
+    scan<T>(none, weight, all, weights);
 }
 
-template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_maxima(SampleArgs a, Row *rows, int chunks) {
+// blockIdx.x: a row's chunk.
+template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_scan(SampleArgs a, Rows rows) {
     __shared__ float tops[4], leasts[4];
     __shared__ int places[4];
-    const int number = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-    Row &row = rows[number];
+    const int number = blockIdx.x / rows.chunks, chunk = blockIdx.x % rows.chunks;
+    Row &row = rows.row(number);
     float top = -INFINITY, least = INFINITY;
     int at = 0x7FFFFFFF;
-    each<VEC>(a.logits + (size_t)number * a.ld, a.n, chunk, [&](float x, int i) {
-        argmax_step(top, at, x, i);
-        if (x > -INFINITY) least = fminf(least, x);
+    Chunk<VEC> c;
+    c.load(a.logits + (size_t)number * a.ld, a.n, chunk);
+    c.each([&](float v, int i) {
+        argmax_step(top, at, v, i);
+        if (v > -INFINITY) least = fminf(least, v);
     });
     // what the next launches add to
-    for (int i = chunk * THREADS + threadIdx.x; i < BINS; i += chunks * THREADS) row.count[i] = 0, row.weight[i] = 0;
-    if (chunk == 0 && threadIdx.x == 0) row.listed = 0;
+    for (int i = chunk * THREADS + threadIdx.x; i < BINS; i += rows.chunks * THREADS) row.count[i] = 0, row.weight[i] = 0;
+    if (chunk == 0 && threadIdx.x == 0) row.far = 0, row.listed = 0;
+    float group = fmaxf(top, dpp<DPP_XOR1>(top, top));
+    group = fmaxf(group, dpp<DPP_XOR2>(group, group));
+    if (threadIdx.x % 4 == 0) rows.maxima(number)[chunk * GROUPS + threadIdx.x / 4] = group;
     wave_argmax(top, at, -INFINITY);
     least = wave_reduce(least, INFINITY, [](float u, float v) { return fminf(u, v); });
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top, leasts[threadIdx.x >> 6] = least, places[threadIdx.x >> 6] = at;
@@ -192,87 +266,204 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_maxima(Sam
     }
 }
 
-template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(SampleArgs a, Row *rows, int chunks) {
-    __shared__ unsigned count[BINS];
-    __shared__ u64 weight[BINS];
-    const int number = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-    Row &row = rows[number];
-    int at;
-    const Rule r = rule_of(a, row, number, chunks, at);
-    if (r.greedy) return;
+// A row's maxima of groups, as many as a wave holds: four groups in a number.
+struct Maxima {
+    static constexpr int HELD = 10;
+    float4 v[HELD];
+    const float4 *from;
+    int n;  // fours
+
+    __device__ __forceinline__ void load(const float *maxima, int groups) {
+        from = (const float4 *)maxima;
+        n = groups / 4;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int at = (threadIdx.x & 63) + 64 * i;
+            v[i] = at < n ? from[at] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        }
+    }
+};
+
+// A bound that k groups' maxima, and so k tokens, reach: as few more as a short search finds. Four bounds are counted at a
+// time, one by each wave. 0: there are fewer than k.
+__device__ __forceinline__ uint32_t bound_of(const Maxima &m, float top, int k) {
+    __shared__ int counts[4];
+    constexpr int HELD = Maxima::HELD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, enough = k + k / 4;
+    const bool fours = m.n >= enough;  // maxima of four groups where these are still enough
+    const uint32_t none = rising(-INFINITY);
+    uint32_t one[HELD], four[HELD][4], least = ~0u;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const float4 v = m.v[i];
+        four[i][0] = rising(v.x), four[i][1] = rising(v.y), four[i][2] = rising(v.z), four[i][3] = rising(v.w);
+        one[i] = max(max(four[i][0], four[i][1]), max(four[i][2], four[i][3]));
+        least = min(least, one[i] > none ? one[i] : ~0u);
+    }
+    const auto count_of = [&](uint32_t at) {
+        int count = 0;
+        if (fours) {
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) count += __popcll(__ballot(one[i] >= at));
+        } else {
+#pragma unroll
+            for (int i = 0; i < HELD; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) count += __popcll(__ballot(four[i][j] >= at));
+        }
+        for (int i = lane + 64 * HELD; i < m.n + lane; i += 64) {  // (those that are not held)
+            const float4 v = m.from[min(i, m.n - 1)];
+            const bool x = rising(v.x) >= at, y = rising(v.y) >= at, z = rising(v.z) >= at, w = rising(v.w) >= at, in = i < m.n;
+            if (fours) {
+                count += __popcll(__ballot(in && (x || y || z || w)));
+            } else {
+                count += __popcll(__ballot(in && x)) + __popcll(__ballot(in && y)) + __popcll(__ballot(in && z)) +
+                         __popcll(__ballot(in && w));
+            }
+        }
+        return count;
+    };
+    // from the least finite maximum: it is reached by so many of them
+    uint32_t lo = (uint32_t)wave_reduce((int)(least ^ 0x80000000u), 0x7FFFFFFF, [](int x, int y) { return min(x, y); }) ^ 0x80000000u;
+    uint32_t hi = rising(top) + 1;  // count(lo) >= k, count(hi) < k
+    int best = count_of(lo);
+    if (best < k) {  // (there may be less ones)
+        lo = none + 1;
+        best = count_of(lo);
+        if (best < k) return 0;
+    }
+    while (best > enough && hi - lo > 1) {
+        const uint32_t step = (hi - lo) / 5 + 1;
+        const int mine = count_of(min(lo + (wave + 1) * step, hi));
+        __syncthreads();  // (what the round before left is read)
+        if (lane == 0) counts[wave] = mine;
+        __syncthreads();
+        int reached = 0;  // bounds that k reach
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int c = counts[w];
+            if (c >= k) reached = w + 1, best = c;
+        }
+        const uint32_t was = lo;
+        if (reached) lo = min(was + reached * step, hi);
+        if (reached < 4) hi = min(was + (reached + 1) * step, hi);
+    }
+    return lo;
+}
+
+// blockIdx.x: `span` chunks of a row.
+template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(SampleArgs a, Rows rows, int span) {
+    __shared__ union {
+        struct { unsigned count[BINS]; u64 weight[BINS]; } bins;
+        uint2 list[LIST];
+    } lds;
+    __shared__ unsigned listed, first;
+    const int spans = (rows.chunks + span - 1) / span, number = blockIdx.x / spans, begin = blockIdx.x % spans * span;
+    const int end = min(begin + span, rows.chunks);
+    Row &row = rows.row(number);
     const float *x = a.logits + (size_t)number * a.ld;
-    if (!r.cut) {
-        u64 sum = 0, total;
-        each<VEC>(x, a.n, chunk, [&](float v, int) {
-            const double y = r.distance(v);
-            if (r.likely(y)) sum += r.weight(y);
-        });
-        scan(sum, total);
-        if (threadIdx.x == 0) row.sum[chunk] = total;
+    Chunk<VEC> c;
+    // (on their way while the rule is made)
+    c.load(x, a.n, begin);
+    Maxima maxima;
+    maxima.load(rows.maxima(number), rows.chunks * GROUPS);
+    int at;
+    const Rule r = rule_of(a, row, number, rows.chunks, at);
+    if (begin == 0 && threadIdx.x == 0) row.rule = r, row.best = at;
+    if (r.mode == GREEDY) return;
+    if (r.mode == WHOLE) {
+        for (int chunk = begin; chunk < end; ++chunk) {
+            u64 sum = 0, total;
+            c.each([&](float v, int) {
+                const double y = r.distance(v);
+                if (r.likely(y)) sum += r.weight(y);
+            });
+            if (chunk + 1 < end) c.load(x, a.n, chunk + 1);
+            scan<THREADS>(sum, total);
+            if (threadIdx.x == 0) row.sum[chunk] = total;
+        }
         return;
     }
-    for (int i = threadIdx.x; i < BINS; i += THREADS) count[i] = 0, weight[i] = 0;
-    __syncthreads();
-    each<VEC>(x, a.n, chunk, [&](float v, int) {
-        const double y = r.distance(v);
-        const u64 w = r.weight(y);
-        if (w) {
-            const int b = r.bin(y);
-            atomicAdd(&count[b], 1u);
-            atomicAdd(&weight[b], w);
+    if (r.mode == SMALL) {
+        if (threadIdx.x == 0) listed = 0;
+        const uint32_t bound = a.n <= LIST ? 0 : bound_of(maxima, (float)r.m, r.k);
+        const float least = bound ? of_rising(bound) : -INFINITY;
+        __syncthreads();
+        for (int chunk = begin; chunk < end; ++chunk) {
+            c.each([&](float v, int i) {
+                if (v >= least && v > -INFINITY) {
+                    const unsigned to = atomicAdd(&listed, 1u);
+                    if (to < LIST) lds.list[to] = make_uint2(i, __float_as_uint(v));
+                }
+            });
+            if (chunk + 1 < end) c.load(x, a.n, chunk + 1);
         }
-    });
+        __syncthreads();
+        if (threadIdx.x == 0) first = listed ? atomicAdd(&row.listed, listed) : 0;
+        __syncthreads();
+        for (unsigned i = threadIdx.x; i < min(listed, (unsigned)LIST); i += THREADS)
+            if (first + i < LIST) row.list[first + i] = lds.list[i];
+        return;
+    }
+    for (int i = threadIdx.x; i < BINS; i += THREADS) lds.bins.count[i] = 0, lds.bins.weight[i] = 0;
+    __syncthreads();
+    u64 far = 0;
+    for (int chunk = begin; chunk < end; ++chunk) {
+        c.each([&](float v, int) {
+            const u64 w = r.weight(r.distance(v));
+            const int b = r.bin(v);
+            if (b >= BINS) {
+                far += w;
+            } else if (w) {
+                if (r.k) atomicAdd(&lds.bins.count[b], 1u);
+                atomicAdd(&lds.bins.weight[b], w);
+            }
+        });
+        if (chunk + 1 < end) c.load(x, a.n, chunk + 1);
+    }
+    far = last_lane(wave_scan(far));
+    if ((threadIdx.x & 63) == 0 && far) atomicAdd(&row.far, far);
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += THREADS)
-        if (count[i]) {
-            atomicAdd(&row.count[i], count[i]);
-            atomicAdd(&row.weight[i], weight[i]);
+        if (lds.bins.weight[i]) {
+            if (r.k) atomicAdd(&row.count[i], lds.bins.count[i]);
+            atomicAdd(&row.weight[i], lds.bins.weight[i]);
         }
 }
 
-// Where the border lies.
-struct Border {
-    int k_bin;             // top-k's last token's bin; -1: all tokens are among the first k
-    int lo, hi;            // the bins that may hold the last token kept
-    unsigned k_count;      // tokens in front of k_bin, and their weight
-    u64 k_weight, weight;  // weight of the tokens in front of lo
-    u64 total;             // of all
-};
-__device__ __forceinline__ Border border_of(const Row &row, const Rule &r) {
+constexpr int PER = BINS / THREADS;
+__device__ __forceinline__ Border border_of(const Row &row, const Rule &r, const unsigned (&count)[PER], const u64 (&weight)[PER]) {
     __shared__ Border found;
-    unsigned count[PER], counts = 0, all;
-    u64 weight[PER], weights = 0, total;
+    unsigned c = 0, all;
+    u64 w = 0, total;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        counts += count[i] = row.count[threadIdx.x * PER + i];
-        weights += weight[i] = row.weight[threadIdx.x * PER + i];
-    }
-    const unsigned counts_before = scan(counts, all) - counts;
-    const u64 before = scan(weights, total) - weights;
-    if (threadIdx.x == 0) found = {-1, BINS, BINS, 0, 0, 0, total};  // (no border: fewer than top_k, no top-p)
+    for (int i = 0; i < PER; ++i) c += count[i], w += weight[i];
+    const unsigned mine_c = c;
+    const u64 mine_w = w;
+    scan<THREADS>(c, w, all, total);
+    c -= mine_c;
+    w -= mine_w;
+    if (threadIdx.x == 0) found = {-1, BINS, BINS - 1, 0, 0, 0, total + row.far};
     __syncthreads();
-    // the bin where f(sum in front of it) is false and f(sum with it) is true
-    if (r.k && all > (unsigned)r.k) {
-        unsigned c = counts_before;
-        u64 w = before;
+    if (r.k && all >= (unsigned)r.k) {
+        u64 in_front = w;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (c < (unsigned)r.k && c + count[i] >= (unsigned)r.k) {
                 found.k_bin = found.lo = found.hi = threadIdx.x * PER + i;
                 found.k_count = c;
-                found.k_weight = found.weight = w;
-                found.total = w + weight[i];  // (at the most, of those kept)
+                found.k_weight = found.weight = in_front;
+                found.total = in_front + weight[i];
             }
             c += count[i];
-            w += weight[i];
+            in_front += weight[i];
         }
+        __syncthreads();
     }
-    __syncthreads();
     if (r.p < 1.0) {
         // the sum that p is a share of lies between these
-        const double least = r.p * (double)(found.k_bin < 0 ? total : found.k_weight), most = r.p * (double)found.total;
+        const double least = r.p * (double)(found.k_bin < 0 ? found.total : found.k_weight), most = r.p * (double)found.total;
         __syncthreads();
-        u64 w = before;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const u64 with = w + weight[i];
@@ -286,199 +477,436 @@ __device__ __forceinline__ Border border_of(const Row &row, const Rule &r) {
     return found;
 }
 
-template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(SampleArgs a, Row *rows, int chunks) {
+// blockIdx.x: `span` chunks of a row.
+template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(SampleArgs a, Rows rows, int span) {
     __shared__ unsigned listed, first;
     __shared__ uint2 list[LIST];
-    const int number = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-    Row &row = rows[number];
-    int at;
-    const Rule r = rule_of(a, row, number, chunks, at);
-    if (r.greedy || !r.cut) return;
-    const Border b = border_of(row, r);
+    __shared__ float queues[4][CHUNK / 4];
+    const int spans = (rows.chunks + span - 1) / span, number = blockIdx.x / spans, begin = blockIdx.x % spans * span;
+    const int end = min(begin + span, rows.chunks);
+    Row &row = rows.row(number);
+    if (row.rule.mode != BINNED) return;
+    const float *x = a.logits + (size_t)number * a.ld;
+    unsigned count[PER];
+    u64 weight[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) count[i] = row.count[threadIdx.x * PER + i], weight[i] = row.weight[threadIdx.x * PER + i];
+    Chunk<VEC> c;
+    c.load(x, a.n, begin);
+    const Rule r = row.rule;
+    const Border b = border_of(row, r, count, weight);
+    if (begin == 0 && threadIdx.x == 0) row.border = b;
     if (threadIdx.x == 0) listed = 0;
     __syncthreads();
-    u64 sum = 0, total;
-    each<VEC>(a.logits + (size_t)number * a.ld, a.n, chunk, [&](float v, int i) {
-        const double y = r.distance(v);
-        const u64 w = r.weight(y);
-        if (!w) return;
-        const int bin = r.bin(y);
-        if (bin < b.lo && r.likely(y)) sum += w;
-        if ((bin >= b.lo && bin <= b.hi) || bin == b.k_bin) {
-            const unsigned to = atomicAdd(&listed, 1u);
-            if (to < LIST) list[to] = make_uint2(i, __float_as_uint(v));
+    const int lane = threadIdx.x & 63;
+    float *queue = queues[threadIdx.x >> 6];
+    for (int chunk = begin; chunk < end; ++chunk) {
+        // the values in front of the border, close together: few of a wave's 64 are, and their weights are what costs
+        int queued = 0;
+        c.each([&](float v, int i) {
+            const int bin = r.bin(v);
+            const unsigned long long in_front = __ballot(bin < b.lo);
+            if (bin < b.lo) queue[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(in_front >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in_front, 0))] = v;
+            queued += __popcll(in_front);
+            if (bin >= b.lo && (bin <= b.hi || bin == b.k_bin)) {
+                const unsigned to = atomicAdd(&listed, 1u);
+                if (to < LIST) list[to] = make_uint2(i, __float_as_uint(v));
+            }
+        });
+        if (chunk + 1 < end) c.load(x, a.n, chunk + 1);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        u64 sum = 0, total;
+        for (int i = lane; i < queued; i += 64) {
+            const double y = r.distance(queue[i]);
+            if (r.likely(y)) sum += r.weight(y);
         }
-    });
-    scan(sum, total);
-    if (threadIdx.x == 0) {
-        row.sum[chunk] = total;
-        first = listed ? atomicAdd(&row.listed, listed) : 0;
+        scan<THREADS>(sum, total);
+        if (threadIdx.x == 0) row.sum[chunk] = total;
     }
+    __syncthreads();
+    if (threadIdx.x == 0) first = listed ? atomicAdd(&row.listed, listed) : 0;
     __syncthreads();
     for (unsigned i = threadIdx.x; i < min(listed, (unsigned)LIST); i += THREADS)
         if (first + i < LIST) row.list[first + i] = list[i];
 }
 
-// The border's tokens: from the list, or where that is too short, from the row.
-template <class F> __device__ __forceinline__ void each_listed(const SampleArgs &a, const Row &row, const Rule &r, const float *x, F f) {
-    if (row.listed <= LIST) {
-        for (unsigned i = threadIdx.x; i < row.listed; i += THREADS) {
-            const float v = __uint_as_float(row.list[i].y);
-            const double y = r.distance(v);
-            f(v, row.list[i].x, y, r.weight(y));
-        }
+// ---- the last launch: one workgroup of 1024 per row ---------------------------------------
+
+// Tokens of the border's bins.
+struct Listed {
+    u64 at[LIST], weight[LIST];
+    uint16_t bin[LIST];
+    unsigned n;
+};
+
+// f(place, weight) for those of bins [lo, hi]: from the list, or where that is too short, from the row (then from all tokens).
+template <class F>
+__device__ __forceinline__ void each_listed(const Listed &list, const Rule &r, const float *x, int n, int lo, int hi, F f) {
+    if (list.n <= LIST) {
+        for (unsigned i = threadIdx.x; i < list.n; i += DRAW)
+            if (list.bin[i] >= lo && list.bin[i] <= hi) f(list.at[i], list.weight[i]);
     } else {
-        for (int i = threadIdx.x; i < a.n; i += THREADS) {
+        for (int i = threadIdx.x; i < n; i += DRAW) {
             const float v = value(x[i]);
-            const double y = r.distance(v);
-            const u64 w = r.weight(y);
-            if (w) f(v, (uint32_t)i, y, w);
+            const int bin = r.bin(v);
+            if (bin < lo || bin > hi) continue;
+            const u64 w = r.weight(r.distance(v));
+            if (w) f(place(v, i), w);
         }
     }
 }
 
-// The last place of bins [lo, hi] to keep: that of the first token with which it is done(tokens up to it, their weight),
-// counted from `count` and `weight`, or one between it and the bins' next; `weight` becomes that weight. By digits of 8 bits of
-// the place, the highest first.
+// The place of the first token of bins [lo, hi] with which it is done(tokens up to it, their weight), counted from `count` and
+// `weight`; `weight` becomes that weight. By digits of 8 bits of the place, from the highest that differs.
 template <class Done>
-__device__ __forceinline__ u64 last_place(const SampleArgs &a, const Row &row, const Rule &r, const float *x, int lo, int hi,
+__device__ __forceinline__ u64 last_place(const Listed &list, const Rule &r, const float *x, int n, int lo, int hi,
                                           unsigned count, u64 &weight, Done done) {
     __shared__ unsigned counts[256];
-    __shared__ u64 weights[256];
+    __shared__ u64 weights[256], highest[256], least, most;
     __shared__ struct { unsigned digit, count, here; u64 weight, mine; } next;
-    u64 prefix = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        counts[threadIdx.x] = 0;
-        weights[threadIdx.x] = 0;
+    if (threadIdx.x == 0) least = ~0ull, most = 0;
+    __syncthreads();
+    u64 a = ~0ull, b = 0;
+    each_listed(list, r, x, n, lo, hi, [&](u64 at, u64) { a = min(a, at), b = max(b, at); });
+    if (b) atomicMin(&least, a), atomicMax(&most, b);
+    __syncthreads();
+    const u64 differ = least ^ most;
+    u64 prefix = most;
+    int shift = differ ? max(56 - (int)__builtin_clzll(differ), 0) : 0, known = shift + 8;  // bits of the prefix that are known
+    for (;;) {
+        if (threadIdx.x < 256) counts[threadIdx.x] = 0, weights[threadIdx.x] = 0, highest[threadIdx.x] = 0;
         __syncthreads();
-        each_listed(a, row, r, x, [&](float v, uint32_t i, double y, u64 w) {
-            const int bin = r.bin(y);
-            const u64 at = place(v, i);
-            if (bin < lo || bin > hi || (shift < 56 && at >> (shift + 8) != prefix >> (shift + 8))) return;
-            atomicAdd(&counts[at >> shift & 255], 1u);
-            atomicAdd(&weights[at >> shift & 255], w);
+        each_listed(list, r, x, n, lo, hi, [&](u64 at, u64 w) {
+            if (known < 64 && (at ^ prefix) >> known) return;
+            const int digit = at >> shift & 255;
+            atomicAdd(&counts[digit], 1u);
+            atomicAdd(&weights[digit], w);
+            atomicMax(&highest[digit], at);
         });
         __syncthreads();
-        unsigned all;
-        u64 total;
-        const unsigned c = counts[threadIdx.x], upto = scan(c, all) + count;
-        const u64 w = weights[threadIdx.x], with = scan(w, total) + weight;
         // the first digit with which it is done; if rounding leaves none, the last that there is
-        const bool here = c && done(upto, with);
-        const bool none = c && upto == all + count && !done(upto, with);
-        if ((here && !(upto - c > count && done(upto - c, with - w))) || none)
-            next = {threadIdx.x, upto - c, c, with - w, w};
+        if (threadIdx.x < 64) {
+            unsigned c[4], cs = 0;
+            u64 w[4], ws = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cs += c[i] = counts[4 * threadIdx.x + i], ws += w[i] = weights[4 * threadIdx.x + i];
+            unsigned before = wave_scan(cs);
+            const unsigned all = (unsigned)readlane63((int)before);
+            u64 in_front = wave_scan(ws) - ws;
+            before -= cs;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned upto = before + c[i];
+                const bool is = done(count + upto, weight + in_front + w[i]);
+                const bool was = before && done(count + before, weight + in_front);
+                if (c[i] && !was && (is || upto == all))
+                    next = {4 * threadIdx.x + i, count + before, c[i], weight + in_front, w[i]};
+                before = upto;
+                in_front += w[i];
+            }
+        }
         __syncthreads();
-        prefix |= (u64)next.digit << shift;
         count = next.count;
         weight = next.weight;
-        const unsigned here_count = next.here;
-        const u64 mine = next.mine;
-        __syncthreads();
-        if (here_count == 1 || shift == 0) {
-            weight += mine;
-            return prefix | ((1ull << shift) - 1);
+        prefix = highest[next.digit];
+        if (next.here == 1 || shift == 0) {
+            weight += next.mine;
+            return prefix;
         }
+        known = shift;
+        shift = max(shift - 8, 0);
+        __syncthreads();
     }
-    return prefix;
 }
 
-__global__ __launch_bounds__(THREADS) void sample_draw(SampleArgs a, Row *rows, int chunks) {
-    __shared__ u64 sums[MOST_CHUNKS];
+// The running sum that the token's exceeds: u times all, at most all but one.
+__device__ __forceinline__ u64 target_of(double u, u64 total) {
+    const double want = u * (double)total;
+    return want > 0.0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : u == u ? 0 : total - 1;
+}
+
+// The token drawn: one per thread that may be, `before` the kept weights in front of it.
+__device__ __forceinline__ void drawn(const SampleArgs &a, int number, u64 target, u64 before, u64 w, u64 total, int at) {
+    if (before <= target && before + w > target) {
+        a.ids[number] = at;
+        if (a.prob) a.prob[number] = (float)((double)w / (double)total);
+    }
+}
+
+// Listed tokens in order, by bins of their bits: a token's place is its bin's beginning and those in front of it in the bin.
+constexpr int CELLS = 2048, PER_CELL = CELLS / DRAW, CROWD = 64;
+struct Ordered {
+    unsigned begin[CELLS + 1];  // the cells' first tokens
+    u64 weight[CELLS];          // the weight in front of them
+    u64 at[LIST], own[LIST];    // places and weights, cell by cell
+    unsigned least, most, crowd;
+};
+constexpr int HELD = LIST / DRAW;
+struct Token {
+    u64 at, w;        // place and weight; at ~0: none
+    unsigned before;  // listed tokens in front of it, and their weight
+    u64 weight;
+};
+// False: a cell has so many (equal logits) that this would take longer than last_place.
+__device__ __forceinline__ bool order(Ordered &o, Token (&t)[HELD]) {
+    unsigned least = ~0u, most = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (t[i].at != ~0ull) {
+            least = min(least, (unsigned)(t[i].at >> 32));
+            most = max(most, (unsigned)(t[i].at >> 32));
+        }
+    least = ~(unsigned)wave_reduce((int)(~least ^ 0x80000000u), (int)0x80000000, [](int x, int y) { return max(x, y); }) ^ 0x80000000u;
+    most = (unsigned)wave_reduce((int)(most ^ 0x80000000u), (int)0x80000000, [](int x, int y) { return max(x, y); }) ^ 0x80000000u;
+    if (threadIdx.x == 0) o.least = ~0u, o.most = 0, o.crowd = 0;
+    for (int i = threadIdx.x; i < CELLS; i += DRAW) o.begin[i] = 0, o.weight[i] = 0;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) atomicMin(&o.least, least), atomicMax(&o.most, most);
+    __syncthreads();
+    least = o.least;
+    const unsigned range = o.most - least;
+    const int shift = range ? max(32 - (int)__builtin_clz(range) - 11, 0) : 0;
+    int cell[HELD];
+    unsigned slot[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (t[i].at != ~0ull) {
+            cell[i] = (int)(((unsigned)(t[i].at >> 32) - least) >> shift);
+            slot[i] = atomicAdd(&o.begin[cell[i]], 1u);
+            atomicAdd(&o.weight[cell[i]], t[i].w);
+        }
+    __syncthreads();
+    unsigned count[PER_CELL], c = 0, all;
+    u64 weight[PER_CELL], w = 0, total;
+#pragma unroll
+    for (int i = 0; i < PER_CELL; ++i) {
+        c += count[i] = o.begin[threadIdx.x * PER_CELL + i];
+        w += weight[i] = o.weight[threadIdx.x * PER_CELL + i];
+        if (count[i] > CROWD) o.crowd = 1;
+    }
+    const unsigned mine_c = c;
+    const u64 mine_w = w;
+    scan<DRAW>(c, w, all, total);
+    c -= mine_c;
+    w -= mine_w;
+#pragma unroll
+    for (int i = 0; i < PER_CELL; ++i) {
+        o.begin[threadIdx.x * PER_CELL + i] = c;
+        o.weight[threadIdx.x * PER_CELL + i] = w;
+        c += count[i];
+        w += weight[i];
+    }
+    if (threadIdx.x == DRAW - 1) o.begin[CELLS] = c;
+    __syncthreads();
+    if (o.crowd) return false;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (t[i].at != ~0ull) {
+            const unsigned to = o.begin[cell[i]] + slot[i];
+            o.at[to] = t[i].at;
+            o.own[to] = t[i].w;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (t[i].at != ~0ull) {
+            const unsigned first = o.begin[cell[i]], end = o.begin[cell[i] + 1];
+            t[i].before = first;
+            t[i].weight = o.weight[cell[i]];
+            for (unsigned j = first; j < end; ++j)
+                if (o.at[j] < t[i].at) ++t[i].before, t[i].weight += o.own[j];
+        }
+    return true;
+}
+
+template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleArgs a, Rows rows) {
+    __shared__ u64 sums[MOST_CHUNKS], highest, of_k;
     __shared__ struct { int chunk; u64 before; } hit;
+    __shared__ unsigned in_front, near;
+    __shared__ union {
+        Ordered ordered;
+        Listed list;
+        struct { u64 w[LIST]; uint32_t at[LIST]; } near;
+    } lds;
     const int number = blockIdx.x;
-    const Row &row = rows[number];
+    const Row &row = rows.row(number);
     const float *x = a.logits + (size_t)number * a.ld;
-    int best;
-    const Rule r = rule_of(a, row, number, chunks, best);
-    if (r.greedy) {
+    // (everything that the steps below may want, in one trip to memory)
+    const Rule r = row.rule;
+    const unsigned listed = row.listed;
+    const double u = a.u[number];
+    Border b = row.border;
+    const u64 of_chunk = row.sum[threadIdx.x & (MOST_CHUNKS - 1)];
+    uint2 of_list[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) of_list[i] = row.list[threadIdx.x + i * DRAW];
+    if (r.mode == GREEDY) {
         if (threadIdx.x == 0) {
             const bool some = r.m != -INFINITY;
-            a.ids[number] = some ? best : -1;
+            a.ids[number] = some ? row.best : -1;
             if (a.prob) a.prob[number] = some ? 1.0f : 0.0f;
         }
         return;
     }
-    int lo = BINS, hi = BINS;  // tokens of bins in front of lo are kept, and of bins up to hi those up to the place `last`
+    // tokens in front of bin b.lo are kept, and of bins up to b.hi those up to the place `last`
     u64 last = 0;
-    if ((int)threadIdx.x < chunks) sums[threadIdx.x] = row.sum[threadIdx.x];
-    if (r.cut) {
-        const Border b = border_of(row, r);
-        u64 all = b.total;
-        lo = b.lo;
-        hi = b.hi;
-        if (b.k_bin >= 0) {
-            all = b.k_weight;
-            last = last_place(a, row, r, x, b.k_bin, b.k_bin, b.k_count, all,
-                              [&](unsigned c, u64) { return c >= (unsigned)r.k; });
+    if (r.mode == WHOLE) b = {-1, BINS + 1, BINS, 0, 0, 0, 0};
+    if (r.mode == SMALL) b = {0, 0, BINS, 0, 0, 0, 0};
+    const int k_end = r.mode == SMALL ? b.hi : b.k_bin;  // bins k_bin .. k_end hold top-k's last token
+    if ((int)threadIdx.x < rows.chunks) sums[threadIdx.x] = r.mode == SMALL ? 0 : of_chunk;
+    Token t[HELD];
+    int bin[HELD];
+    bool keep[HELD], small = false;
+    if (r.mode != WHOLE) {
+        if (threadIdx.x == 0) highest = 0, of_k = 0, in_front = 0, near = 0;
+        unsigned front = 0;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const bool is = listed <= LIST && threadIdx.x + i * DRAW < listed;
+            const float v = __uint_as_float(of_list[i].y);
+            t[i] = {is ? place(v, of_list[i].x) : ~0ull, is ? r.weight(r.distance(v)) : 0, 0, 0};
+            bin[i] = is ? r.bin(v) : BINS + 1;
+            front += bin[i] < b.k_bin;
+            keep[i] = false;
         }
-        if (r.p < 1.0) {
+        if (listed <= LIST && order(lds.ordered, t)) {
+            // S: the weight of the first k
+            u64 all = b.total;
+            if (b.k_bin >= 0) {
+                front = wave_scan(front);
+                if ((threadIdx.x & 63) == 63 && front) atomicAdd(&in_front, front);
+                __syncthreads();
+                u64 w = 0;
+#pragma unroll
+                for (int i = 0; i < HELD; ++i) {
+                    keep[i] = bin[i] < b.k_bin || (bin[i] <= k_end && b.k_count + (t[i].before - in_front) < (unsigned)r.k);
+                    if (keep[i] && bin[i] >= b.k_bin) w += t[i].w;
+                }
+                w = last_lane(wave_scan(w));
+                if ((threadIdx.x & 63) == 0 && w) atomicAdd(&of_k, w);
+                __syncthreads();
+                all = b.k_weight + of_k;
+            } else {
+#pragma unroll
+                for (int i = 0; i < HELD; ++i) keep[i] = bin[i] <= BINS;
+            }
             const double share = r.p * (double)all;
-            u64 w = b.weight;
-            last = last_place(a, row, r, x, b.lo, b.hi, 0, w, [&](unsigned, u64 s) { return (double)s >= share; });
+            u64 top = 0;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                const u64 before = b.weight + t[i].weight;
+                keep[i] = keep[i] && bin[i] <= b.hi && (r.p == 1.0 || (double)before < share || !before);
+                if (keep[i]) top = max(top, t[i].at);
+            }
+            if (top) atomicMax(&highest, top);
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                keep[i] = keep[i] && t[i].w && r.likely(r.distance(of_rising(~(uint32_t)(t[i].at >> 32))));
+                if (keep[i]) atomicAdd(&sums[(uint32_t)t[i].at / CHUNK], t[i].w);
+            }
+            __syncthreads();
+            last = highest;
+            small = r.mode == SMALL;
+        } else {
+            if (threadIdx.x == 0) lds.list.n = listed;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < HELD; ++i)
+                if (t[i].at != ~0ull) {
+                    lds.list.at[threadIdx.x + i * DRAW] = t[i].at;
+                    lds.list.weight[threadIdx.x + i * DRAW] = t[i].w;
+                    lds.list.bin[threadIdx.x + i * DRAW] = (uint16_t)bin[i];
+                }
+            __syncthreads();
+            u64 all = b.total;
+            if (b.k_bin >= 0) {
+                all = b.k_weight;
+                last = last_place(lds.list, r, x, a.n, b.k_bin, k_end, b.k_count, all,
+                                  [&](unsigned c, u64) { return c >= (unsigned)r.k; });
+            }
+            if (r.p < 1.0) {
+                const double share = r.p * (double)all;
+                u64 w = b.weight;
+                last = last_place(lds.list, r, x, a.n, b.lo, b.hi, 0, w, [&](unsigned, u64 s) { return (double)s >= share; });
+            }
+            each_listed(lds.list, r, x, a.n, b.lo, b.hi, [&](u64 at, u64 w) {
+                if (at <= last && r.likely(r.distance(of_rising(~(uint32_t)(at >> 32))))) atomicAdd(&sums[(uint32_t)at / CHUNK], w);
+            });
         }
-        __syncthreads();
-        each_listed(a, row, r, x, [&](float v, uint32_t i, double y, u64 w) {
-            const int bin = r.bin(y);
-            if (bin >= lo && bin <= hi && place(v, i) <= last && r.likely(y)) atomicAdd(&sums[i / CHUNK], w);
-        });
     }
     __syncthreads();
     u64 total;
-    const u64 mine = (int)threadIdx.x < chunks ? sums[threadIdx.x] : 0, upto = scan(mine, total);
-    // the running sum that is exceeded: u times all, at most all but one
-    const double u = a.u[number], want = u * (double)total;
-    const u64 target = want > 0.0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : u == u ? 0 : total - 1;
+    const u64 mine = (int)threadIdx.x < rows.chunks ? sums[threadIdx.x] : 0;
+    u64 upto = mine;
+    scan<DRAW>(upto, total);
+    const u64 target = target_of(u, total);
     if (upto > target && upto - mine <= target) hit = {(int)threadIdx.x, upto - mine};
     __syncthreads();
-    const int first = hit.chunk * CHUNK + threadIdx.x * EACH;
-    u64 before = hit.before, w[EACH], sum = 0;
+    if (small) {
+        // all kept tokens are at hand: those of the chunk
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
+        for (int i = 0; i < HELD; ++i)
+            if (keep[i] && (int)((uint32_t)t[i].at / CHUNK) == hit.chunk) {
+                const unsigned to = atomicAdd(&near, 1u);
+                lds.near.at[to] = (uint32_t)t[i].at;
+                lds.near.w[to] = t[i].w;
+            }
+        __syncthreads();
+        for (unsigned i = threadIdx.x; i < near; i += DRAW) {
+            u64 before = hit.before;
+            for (unsigned j = 0; j < near; ++j) before += lds.near.at[j] < lds.near.at[i] ? lds.near.w[j] : 0;
+            drawn(a, number, target, before, lds.near.w[i], total, (int)lds.near.at[i]);
+        }
+        return;
+    }
+    constexpr int MINE = CHUNK / DRAW;
+    const int first = hit.chunk * CHUNK + threadIdx.x * MINE;
+    u64 w[MINE], sum = 0;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
         w[j] = 0;
         if (first + j < a.n) {
             const float v = value(x[first + j]);
             const double y = r.distance(v);
             w[j] = r.likely(y) ? r.weight(y) : 0;
-            if (w[j]) {
-                const int bin = r.bin(y);
-                if (bin >= lo && (bin > hi || place(v, first + j) > last)) w[j] = 0;
-            }
+            const int in = r.bin(v);
+            if (in >= b.lo && (in > b.hi || place(v, first + j) > last)) w[j] = 0;
         }
         sum += w[j];
     }
-    u64 here;
-    before += scan(sum, here) - sum;
+    u64 before = sum, here;
+    const u64 chunks_before = hit.before;
+    scan<DRAW>(before, here);
+    before += chunks_before - sum;
     if (before <= target && before + sum > target) {
 #pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-            if (before <= target && before + w[j] > target) {
-                a.ids[number] = first + j;
-                if (a.prob) a.prob[number] = (float)((double)w[j] / (double)total);
-            }
+        for (int j = 0; j < MINE; ++j) {
+            drawn(a, number, target, before, w[j], total, first + j);
             before += w[j];
         }
     }
 }
 
+template <bool VEC> void launch(const SampleArgs &a, const Rows &rows, int n, hipStream_t st) {
+    const dim3 block(THREADS);
+    const int span = std::max(1, n * rows.chunks / 768), spans = (rows.chunks + span - 1) / span;
+    hipLaunchKernelGGL((sample_scan<VEC>), dim3(n * rows.chunks), block, 0, st, a, rows);
+    hipLaunchKernelGGL((sample_bins<VEC>), dim3(n * spans), block, 0, st, a, rows, span);
+    hipLaunchKernelGGL((sample_border<VEC>), dim3(n * spans), block, 0, st, a, rows, span);
+    hipLaunchKernelGGL((sample_draw<VEC>), dim3(n), dim3(DRAW), 0, st, a, rows);
+}
+
 }  // namespace
 
-int launch_sample(const SampleArgs &a, int rows, hipStream_t st) {
-    const int chunks = (a.n + CHUNK - 1) / CHUNK;
+int launch_sample(const SampleArgs &a, int n, hipStream_t st) {
+    Rows rows;
+    rows.chunks = (a.n + CHUNK - 1) / CHUNK;
+    rows.step = sizeof(Row) + (size_t)rows.chunks * GROUPS * sizeof(float);
     const std::lock_guard<std::mutex> lk(lib_scratch_mutex());
-    Row *scratch = (Row *)lib_scratch((size_t)rows * sizeof(Row));
-    if (!scratch) return -1;
-    const dim3 grid((unsigned)(rows * chunks)), block(THREADS);
-    if (((uintptr_t)a.logits & 15) == 0 && a.ld % 4 == 0) {
-        hipLaunchKernelGGL((sample_maxima<true>), grid, block, 0, st, a, scratch, chunks);
-        hipLaunchKernelGGL((sample_bins<true>), grid, block, 0, st, a, scratch, chunks);
-        hipLaunchKernelGGL((sample_border<true>), grid, block, 0, st, a, scratch, chunks);
-    } else {
-        hipLaunchKernelGGL((sample_maxima<false>), grid, block, 0, st, a, scratch, chunks);
-        hipLaunchKernelGGL((sample_bins<false>), grid, block, 0, st, a, scratch, chunks);
-        hipLaunchKernelGGL((sample_border<false>), grid, block, 0, st, a, scratch, chunks);
-    }
-    hipLaunchKernelGGL(sample_draw, dim3(rows), block, 0, st, a, scratch, chunks);
+    rows.base = (char *)lib_scratch(n * rows.step);
+    if (!rows.base) return -1;
+    if (((uintptr_t)a.logits & 15) == 0 && a.ld % 4 == 0) launch<true>(a, rows, n, st);
+    else launch<false>(a, rows, n, st);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
