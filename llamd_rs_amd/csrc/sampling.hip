@@ -34,9 +34,9 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH, DRAW = 1024;
+constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH, DRAW = 1024, PIECE = 512;
 constexpr int BINS = 2048, LIST = 2048, FEW = 1024, GROUP = 64, GROUPS = CHUNK / GROUP;
-constexpr int MOST_CHUNKS = SAMPLE_MOST / CHUNK;
+constexpr int MOST_CHUNKS = SAMPLE_MOST / CHUNK, MOST_PIECES = SAMPLE_MOST / PIECE;
 static_assert(MOST_CHUNKS <= THREADS, "a thread per chunk");
 constexpr double RANGE = 44.0;  // weights below 2^-44 are 0
 
@@ -110,7 +110,7 @@ struct Rule {
 struct alignas(16) Row {
     u64 weight[BINS];
     unsigned count[BINS];
-    u64 sum[MOST_CHUNKS];  // of the kept weights, or of those in front of the border's bins
+    u64 sum[MOST_PIECES];  // of the kept weights of 512 values, or of those in front of the border's bins
     Border border;
     u64 far;               // weight of the tokens behind the bins
     unsigned listed;
@@ -164,24 +164,25 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int
     return r;
 }
 
-// A chunk's logits, 16 per thread. VEC: rows are 16-byte aligned.
-template <bool VEC> struct Chunk {
+// EACH logits for each of T threads, those from `first` on. VEC: rows are 16-byte aligned.
+template <bool VEC, int T, int EACH> struct Values {
     float v[EACH];
     int first, n;
 
-    __device__ __forceinline__ void load(const float *x, int of_row, int chunk) {
-        first = chunk * CHUNK;
+    __device__ __forceinline__ void load(const float *x, int of_row, int from) {
+        first = from;
         n = of_row;
-        if (VEC && first + CHUNK <= n) {
+        if (VEC && first + T * EACH <= n) {
 #pragma unroll
-            for (int j = 0; j < EACH / 4; ++j) *(float4 *)(v + 4 * j) = *(const float4 *)(x + first + (j * THREADS + threadIdx.x) * 4);
+            for (int j = 0; j < EACH / 4; ++j) *(float4 *)(v + 4 * j) = *(const float4 *)(x + index(4 * j));
         } else {
 #pragma unroll
             for (int j = 0; j < EACH; ++j) v[j] = index(j) < n ? x[index(j)] : -INFINITY;
         }
     }
     __device__ __forceinline__ int index(int j) const {
-        return first + (VEC ? (j / 4 * THREADS + (int)threadIdx.x) * 4 + j % 4 : j * THREADS + (int)threadIdx.x);
+        const int t = threadIdx.x % T;
+        return first + (VEC ? (j / 4 * T + t) * 4 + j % 4 : j * T + t);
     }
     // f(x, index) for each; -infinity behind the row
     template <class F> __device__ __forceinline__ void each(F f) const {
@@ -244,8 +245,8 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_scan(Sampl
     Row &row = rows.row(number);
     float top = -INFINITY, least = INFINITY;
     int at = 0x7FFFFFFF;
-    Chunk<VEC> c;
-    c.load(a.logits + (size_t)number * a.ld, a.n, chunk);
+    Values<VEC, THREADS, EACH> c;
+    c.load(a.logits + (size_t)number * a.ld, a.n, chunk * CHUNK);
     c.each([&](float v, int i) {
         argmax_step(top, at, v, i);
         if (v > -INFINITY) least = fminf(least, v);
@@ -351,37 +352,51 @@ __device__ __forceinline__ uint32_t bound_of(const Maxima &m, float top, int k) 
     return lo;
 }
 
-// blockIdx.x: `span` chunks of a row.
-template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(SampleArgs a, Rows rows, int span) {
+// f(values, piece) for this wave's pieces of a row: every `waves`-th from `wave` on, the next one on its way.
+template <bool VEC> using Piece = Values<VEC, 64, PIECE / 64>;
+template <bool VEC, class F>
+__device__ __forceinline__ void each_piece(Piece<VEC> &now, const float *x, int n, int wave, int waves, F f) {
+    const int pieces = (n + PIECE - 1) / PIECE;
+#pragma unroll 1
+    for (int piece = wave; piece < pieces; piece += waves) {
+        Piece<VEC> next;
+        next.load(x, n, min(piece + waves, pieces - 1) * PIECE);
+        f(now, piece);
+        now = next;
+    }
+}
+
+// blockIdx.x: one of a row's `parts` workgroups.
+template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(SampleArgs a, Rows rows, int parts) {
     __shared__ union {
         struct { unsigned count[BINS]; u64 weight[BINS]; } bins;
         uint2 list[LIST];
     } lds;
     __shared__ unsigned listed, first;
-    const int spans = (rows.chunks + span - 1) / span, number = blockIdx.x / spans, begin = blockIdx.x % spans * span;
-    const int end = min(begin + span, rows.chunks);
+    const int number = blockIdx.x / parts, part = blockIdx.x % parts;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (THREADS / 64) + (threadIdx.x >> 6)), waves = parts * (THREADS / 64);
     Row &row = rows.row(number);
     const float *x = a.logits + (size_t)number * a.ld;
-    Chunk<VEC> c;
     // (on their way while the rule is made)
-    c.load(x, a.n, begin);
+    Piece<VEC> c;
+    c.load(x, a.n, wave * PIECE);
     Maxima maxima;
-    maxima.load(rows.maxima(number), rows.chunks * GROUPS);
+    const int k = a.how[number].top_k;
+    if (k > 0 && k <= FEW) maxima.load(rows.maxima(number), rows.chunks * GROUPS);
     int at;
     const Rule r = rule_of(a, row, number, rows.chunks, at);
-    if (begin == 0 && threadIdx.x == 0) row.rule = r, row.best = at;
+    if (part == 0 && threadIdx.x == 0) row.rule = r, row.best = at;
     if (r.mode == GREEDY) return;
     if (r.mode == WHOLE) {
-        for (int chunk = begin; chunk < end; ++chunk) {
-            u64 sum = 0, total;
+        each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int piece) {
+            u64 sum = 0;
             c.each([&](float v, int) {
                 const double y = r.distance(v);
                 if (r.likely(y)) sum += r.weight(y);
             });
-            if (chunk + 1 < end) c.load(x, a.n, chunk + 1);
-            scan<THREADS>(sum, total);
-            if (threadIdx.x == 0) row.sum[chunk] = total;
-        }
+            sum = last_lane(wave_scan(sum));
+            if (lane == 0) row.sum[piece] = sum;
+        });
         return;
     }
     if (r.mode == SMALL) {
@@ -389,15 +404,14 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
         const uint32_t bound = a.n <= LIST ? 0 : bound_of(maxima, (float)r.m, r.k);
         const float least = bound ? of_rising(bound) : -INFINITY;
         __syncthreads();
-        for (int chunk = begin; chunk < end; ++chunk) {
+        each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int) {
             c.each([&](float v, int i) {
                 if (v >= least && v > -INFINITY) {
                     const unsigned to = atomicAdd(&listed, 1u);
                     if (to < LIST) lds.list[to] = make_uint2(i, __float_as_uint(v));
                 }
             });
-            if (chunk + 1 < end) c.load(x, a.n, chunk + 1);
-        }
+        });
         __syncthreads();
         if (threadIdx.x == 0) first = listed ? atomicAdd(&row.listed, listed) : 0;
         __syncthreads();
@@ -408,7 +422,7 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
     for (int i = threadIdx.x; i < BINS; i += THREADS) lds.bins.count[i] = 0, lds.bins.weight[i] = 0;
     __syncthreads();
     u64 far = 0;
-    for (int chunk = begin; chunk < end; ++chunk) {
+    each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int) {
         c.each([&](float v, int) {
             const u64 w = r.weight(r.distance(v));
             const int b = r.bin(v);
@@ -419,10 +433,9 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
                 atomicAdd(&lds.bins.weight[b], w);
             }
         });
-        if (chunk + 1 < end) c.load(x, a.n, chunk + 1);
-    }
+    });
     far = last_lane(wave_scan(far));
-    if ((threadIdx.x & 63) == 0 && far) atomicAdd(&row.far, far);
+    if (lane == 0 && far) atomicAdd(&row.far, far);
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += THREADS)
         if (lds.bins.weight[i]) {
@@ -477,13 +490,13 @@ __device__ __forceinline__ Border border_of(const Row &row, const Rule &r, const
     return found;
 }
 
-// blockIdx.x: `span` chunks of a row.
-template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(SampleArgs a, Rows rows, int span) {
+// blockIdx.x: one of a row's `parts` workgroups.
+template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(SampleArgs a, Rows rows, int parts) {
     __shared__ unsigned listed, first;
     __shared__ uint2 list[LIST];
-    __shared__ float queues[4][CHUNK / 4];
-    const int spans = (rows.chunks + span - 1) / span, number = blockIdx.x / spans, begin = blockIdx.x % spans * span;
-    const int end = min(begin + span, rows.chunks);
+    __shared__ float queues[THREADS / 64][PIECE];
+    const int number = blockIdx.x / parts, part = blockIdx.x % parts;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (THREADS / 64) + (threadIdx.x >> 6)), waves = parts * (THREADS / 64);
     Row &row = rows.row(number);
     if (row.rule.mode != BINNED) return;
     const float *x = a.logits + (size_t)number * a.ld;
@@ -491,16 +504,15 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(Sam
     u64 weight[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) count[i] = row.count[threadIdx.x * PER + i], weight[i] = row.weight[threadIdx.x * PER + i];
-    Chunk<VEC> c;
-    c.load(x, a.n, begin);
+    Piece<VEC> c;
+    c.load(x, a.n, wave * PIECE);
     const Rule r = row.rule;
     const Border b = border_of(row, r, count, weight);
-    if (begin == 0 && threadIdx.x == 0) row.border = b;
+    if (part == 0 && threadIdx.x == 0) row.border = b;
     if (threadIdx.x == 0) listed = 0;
     __syncthreads();
-    const int lane = threadIdx.x & 63;
     float *queue = queues[threadIdx.x >> 6];
-    for (int chunk = begin; chunk < end; ++chunk) {
+    each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int piece) {
         // the values in front of the border, close together: few of a wave's 64 are, and their weights are what costs
         int queued = 0;
         c.each([&](float v, int i) {
@@ -513,16 +525,16 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(Sam
                 if (to < LIST) list[to] = make_uint2(i, __float_as_uint(v));
             }
         });
-        if (chunk + 1 < end) c.load(x, a.n, chunk + 1);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-        u64 sum = 0, total;
+        u64 sum = 0;
         for (int i = lane; i < queued; i += 64) {
             const double y = r.distance(queue[i]);
             if (r.likely(y)) sum += r.weight(y);
         }
-        scan<THREADS>(sum, total);
-        if (threadIdx.x == 0) row.sum[chunk] = total;
-    }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        if (queued) sum = last_lane(wave_scan(sum));
+        if (lane == 0) row.sum[piece] = sum;
+    });
     __syncthreads();
     if (threadIdx.x == 0) first = listed ? atomicAdd(&row.listed, listed) : 0;
     __syncthreads();
@@ -720,8 +732,8 @@ __device__ __forceinline__ bool order(Ordered &o, Token (&t)[HELD]) {
 }
 
 template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleArgs a, Rows rows) {
-    __shared__ u64 sums[MOST_CHUNKS], highest, of_k;
-    __shared__ struct { int chunk; u64 before; } hit;
+    __shared__ u64 sums[MOST_PIECES], highest, of_k;
+    __shared__ struct { int piece; u64 before; } hit;
     __shared__ unsigned in_front, near;
     __shared__ union {
         Ordered ordered;
@@ -736,7 +748,11 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
     const unsigned listed = row.listed;
     const double u = a.u[number];
     Border b = row.border;
-    const u64 of_chunk = row.sum[threadIdx.x & (MOST_CHUNKS - 1)];
+    constexpr int MINE = MOST_PIECES / DRAW;
+    const int pieces = (a.n + PIECE - 1) / PIECE;
+    u64 of_piece[MINE];
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) of_piece[j] = row.sum[threadIdx.x * MINE + j];
     uint2 of_list[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) of_list[i] = row.list[threadIdx.x + i * DRAW];
@@ -753,7 +769,11 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
     if (r.mode == WHOLE) b = {-1, BINS + 1, BINS, 0, 0, 0, 0};
     if (r.mode == SMALL) b = {0, 0, BINS, 0, 0, 0, 0};
     const int k_end = r.mode == SMALL ? b.hi : b.k_bin;  // bins k_bin .. k_end hold top-k's last token
-    if ((int)threadIdx.x < rows.chunks) sums[threadIdx.x] = r.mode == SMALL ? 0 : of_chunk;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        const int piece = threadIdx.x * MINE + j;
+        sums[piece] = piece < pieces && r.mode != SMALL ? of_piece[j] : 0;
+    }
     Token t[HELD];
     int bin[HELD];
     bool keep[HELD], small = false;
@@ -802,7 +822,7 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
                 keep[i] = keep[i] && t[i].w && r.likely(r.distance(of_rising(~(uint32_t)(t[i].at >> 32))));
-                if (keep[i]) atomicAdd(&sums[(uint32_t)t[i].at / CHUNK], t[i].w);
+                if (keep[i]) atomicAdd(&sums[(uint32_t)t[i].at / PIECE], t[i].w);
             }
             __syncthreads();
             last = highest;
@@ -830,23 +850,30 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
                 last = last_place(lds.list, r, x, a.n, b.lo, b.hi, 0, w, [&](unsigned, u64 s) { return (double)s >= share; });
             }
             each_listed(lds.list, r, x, a.n, b.lo, b.hi, [&](u64 at, u64 w) {
-                if (at <= last && r.likely(r.distance(of_rising(~(uint32_t)(at >> 32))))) atomicAdd(&sums[(uint32_t)at / CHUNK], w);
+                if (at <= last && r.likely(r.distance(of_rising(~(uint32_t)(at >> 32))))) atomicAdd(&sums[(uint32_t)at / PIECE], w);
             });
         }
     }
     __syncthreads();
     u64 total;
-    const u64 mine = (int)threadIdx.x < rows.chunks ? sums[threadIdx.x] : 0;
+    u64 mine = 0;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) mine += of_piece[j] = sums[threadIdx.x * MINE + j];
     u64 upto = mine;
     scan<DRAW>(upto, total);
     const u64 target = target_of(u, total);
-    if (upto > target && upto - mine <= target) hit = {(int)threadIdx.x, upto - mine};
+    upto -= mine;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        if (upto <= target && upto + of_piece[j] > target) hit = {(int)threadIdx.x * MINE + j, upto};
+        upto += of_piece[j];
+    }
     __syncthreads();
     if (small) {
-        // all kept tokens are at hand: those of the chunk
+        // all kept tokens are at hand: those of the piece
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
-            if (keep[i] && (int)((uint32_t)t[i].at / CHUNK) == hit.chunk) {
+            if (keep[i] && (int)((uint32_t)t[i].at / PIECE) == hit.piece) {
                 const unsigned to = atomicAdd(&near, 1u);
                 lds.near.at[to] = (uint32_t)t[i].at;
                 lds.near.w[to] = t[i].w;
@@ -859,40 +886,27 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
         }
         return;
     }
-    constexpr int MINE = CHUNK / DRAW;
-    const int first = hit.chunk * CHUNK + threadIdx.x * MINE;
-    u64 w[MINE], sum = 0;
-#pragma unroll
-    for (int j = 0; j < MINE; ++j) {
-        w[j] = 0;
-        if (first + j < a.n) {
-            const float v = value(x[first + j]);
-            const double y = r.distance(v);
-            w[j] = r.likely(y) ? r.weight(y) : 0;
-            const int in = r.bin(v);
-            if (in >= b.lo && (in > b.hi || place(v, first + j) > last)) w[j] = 0;
-        }
-        sum += w[j];
+    // the piece's values, one per thread
+    const int at = hit.piece * PIECE + threadIdx.x;
+    u64 w = 0;
+    if (threadIdx.x < PIECE && at < a.n) {
+        const float v = value(x[at]);
+        const double y = r.distance(v);
+        const int in = r.bin(v);
+        if (r.likely(y) && (in < b.lo || (in <= b.hi && place(v, at) <= last))) w = r.weight(y);
     }
-    u64 before = sum, here;
-    const u64 chunks_before = hit.before;
+    u64 before = w, here;
     scan<DRAW>(before, here);
-    before += chunks_before - sum;
-    if (before <= target && before + sum > target) {
-#pragma unroll
-        for (int j = 0; j < MINE; ++j) {
-            drawn(a, number, target, before, w[j], total, first + j);
-            before += w[j];
-        }
-    }
+    drawn(a, number, target, hit.before + before - w, w, total, at);
 }
 
 template <bool VEC> void launch(const SampleArgs &a, const Rows &rows, int n, hipStream_t st) {
     const dim3 block(THREADS);
-    const int span = std::max(1, n * rows.chunks / 768), spans = (rows.chunks + span - 1) / span;
+    // workgroups of a row: four for each CU in all, a piece for each wave at least
+    const int pieces = (a.n + PIECE - 1) / PIECE, parts = std::max(1, std::min((pieces + 3) / 4, 1024 / n));
     hipLaunchKernelGGL((sample_scan<VEC>), dim3(n * rows.chunks), block, 0, st, a, rows);
-    hipLaunchKernelGGL((sample_bins<VEC>), dim3(n * spans), block, 0, st, a, rows, span);
-    hipLaunchKernelGGL((sample_border<VEC>), dim3(n * spans), block, 0, st, a, rows, span);
+    hipLaunchKernelGGL((sample_bins<VEC>), dim3(n * parts), block, 0, st, a, rows, parts);
+    hipLaunchKernelGGL((sample_border<VEC>), dim3(n * parts), block, 0, st, a, rows, parts);
     hipLaunchKernelGGL((sample_draw<VEC>), dim3(n), dim3(DRAW), 0, st, a, rows);
 }
 
