@@ -34,9 +34,9 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH, WIDE = 512, DRAW = 1024;
+constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH, DRAW = 1024, PIECE = 512;
 constexpr int BINS = 2048, LIST = 2048, FEW = 1024, GROUP = 64, GROUPS = CHUNK / GROUP;
-constexpr int MOST_CHUNKS = SAMPLE_MOST / CHUNK, UNIT = 256, MOST_SPANS = 2048;
+constexpr int MOST_CHUNKS = SAMPLE_MOST / CHUNK, MOST_PIECES = SAMPLE_MOST / PIECE;
 static_assert(MOST_CHUNKS <= THREADS, "a thread per chunk");
 constexpr double RANGE = 44.0;  // weights below 2^-44 are 0
 
@@ -54,8 +54,6 @@ struct Border {
     unsigned k_count;      // tokens in front of k_bin, and their weight
     u64 k_weight, weight;  // weight of the tokens in front of lo
     u64 total;             // of all; with k_bin >= 0, of the tokens up to its end
-    // the least values of the bins in front of lo, up to hi, in front of k_bin and up to it; NaN: there are none
-    float in_front, upto_hi, above_k, upto_k;
 };
 __device__ __forceinline__ float value(float x) { return x == x ? x + 0.0f : -INFINITY; }  // (-0 is 0)
 
@@ -69,24 +67,21 @@ __device__ __forceinline__ float of_rising(uint32_t r) { return __uint_as_float(
 // Position in the order: x falling, then index rising.
 __device__ __forceinline__ u64 place(float x, uint32_t i) { return (u64)~rising(x) << 32 | i; }
 
-// A row's rule. A token's distance z from the maximum is in bins: 2^-(z / g) is its weight, BINS of them to the end of the
-// weights or the least value, whichever is nearer.
+// A row's rule.
 struct Rule {
-    double m, per;         // maximum, z per unit of x
-    double inverse, step;  // 1 / g, ln(2) / g
-    double end, furthest;  // z where weights end, and min-p's
+    double m, c;        // maximum, log2(e) / T
+    double furthest;    // min-p's
     double p;
-    int k;                 // 0: all
+    float half, scale;  // half the maximum; bins per half a unit of x
+    int k;              // 0: all
     Mode mode;
-    bool infinite;         // the maximum is: those that are weigh 1, the others nothing
 
-    __device__ __forceinline__ double distance(float x) const {
-        if (infinite) return x == INFINITY ? 0.0 : INFINITY;
-        return (m - (double)x) * per;
-    }
-    // The weight of a bin's middle, in 2^-43
-    __device__ __forceinline__ double middle(int bin) const {
-        const double y = bin * inverse, r = rint(y), f = (r - y) * 0.69314718055994530942;  // |f| <= ln(2) / 2
+    // distance from the maximum in powers of two
+    __device__ __forceinline__ double distance(float x) const { return (double)x == m ? 0.0 : (m - (double)x) * c; }
+    // 2^-y as a multiple of 2^-43; 0 for NaN (an infinite temperature, and a token ruled out)
+    static __device__ __forceinline__ u64 weight(double y) {
+        if (!(y < RANGE)) return 0;
+        const double r = rint(y), f = (r - y) * 0.69314718055994530942;  // |f| <= ln(2) / 2
         // e^f by its series: the next term is below 2^-46
         double s = 1.0 / 39916800.0;
         s = fma(s, f, 1.0 / 3628800.0);
@@ -100,39 +95,27 @@ struct Rule {
         s = fma(s, f, 0.5);
         s = fma(s, f, 1.0);
         s = fma(s, f, 1.0);
-        return __longlong_as_double(__double_as_longlong(s) + ((long long)(43 - (int)r) << 52));
-    }
-    // A token's bin (BINS: it weighs nothing; also for NaN), and its weight from the bin's: whole multiples of 2^-43
-    static constexpr double ROUND = 6755399441055744.0;  // 1.5 2^52: whole numbers in the last places
-    __device__ __forceinline__ int bin(double z) const { return z < end ? (int)__double_as_longlong(z + ROUND) : BINS; }
-    __device__ __forceinline__ u64 weight(double z, double middle) const {
-        // at most half a bin off: u <= ln(2) / 2 / 46, the next term is below 2^-51
-        const double u = ((z + ROUND) - ROUND - z) * step;
-        double s = 1.0 / 120.0;
-        s = fma(s, u, 1.0 / 24.0);
-        s = fma(s, u, 1.0 / 6.0);
-        s = fma(s, u, 0.5);
-        s = fma(s, u, 1.0);
-        const double w = fma(middle * u, s, middle) + 4503599627370496.0;
+        // times 2^(43 - r), rounded to a whole number in the last places of 2^52
+        const double w = __longlong_as_double(__double_as_longlong(s) + ((long long)(43 - (int)r) << 52)) + 4503599627370496.0;
         return (u64)__double_as_longlong(w) & 0xFFFFFFFFFFFFFull;
     }
-    __device__ __forceinline__ u64 weight(double z) const {
-        const int b = bin(z);
-        return b < BINS ? weight(z, middle(b)) : 0;
+    __device__ __forceinline__ bool likely(double y) const { return y <= furthest; }
+    // Rises as x falls; BINS and more: behind the bins. (Halves: the difference of any two numbers is finite.)
+    __device__ __forceinline__ int bin(float x) const {
+        return 2.0f * half == x ? 0 : (int)fminf((half - 0.5f * x) * scale, (float)BINS);
     }
-    __device__ __forceinline__ bool likely(double z) const { return z <= furthest; }
 };
 
 // A row's scratch; behind it the maxima of its groups of 64 values.
 struct alignas(16) Row {
     u64 weight[BINS];
     unsigned count[BINS];
-    u64 sum[MOST_SPANS];   // of the kept weights of a wave's span, or of those in front of the border's bins
+    u64 sum[MOST_PIECES];  // of the kept weights of 512 values, or of those in front of the border's bins
     Border border;
-    unsigned listed, pad;
+    u64 far;               // weight of the tokens behind the bins
+    unsigned listed;
     int best;              // the maximum's first index
     Rule rule;
-    double middle[BINS];   // the weights of the bins' middles
     Extremes chunk[MOST_CHUNKS];
     uint2 list[LIST];      // (index, x's bits), in any order
 };
@@ -154,7 +137,7 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int
     if ((int)threadIdx.x < chunks) x = row.chunk[threadIdx.x];
     wave_argmax(x.top, x.at, -INFINITY);
     x.least = wave_reduce(x.least, INFINITY, [](float u, float v) { return fminf(u, v); });
-    if ((threadIdx.x & 63) == 0 && threadIdx.x < 64 * W) tops[threadIdx.x >> 6] = x.top, leasts[threadIdx.x >> 6] = x.least, places[threadIdx.x >> 6] = x.at;
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = x.top, leasts[threadIdx.x >> 6] = x.least, places[threadIdx.x >> 6] = x.at;
     __syncthreads();
     float top = tops[0], least = leasts[0];
     at = places[0];
@@ -164,20 +147,20 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int
         least = fminf(least, leasts[w]);
     }
     Rule r;
-    r.infinite = top == INFINITY;
     r.m = top;
-    const double c = 1.4426950408889634074 / (double)how.temperature;
+    r.c = 1.4426950408889634074 / (double)how.temperature;
+    r.furthest = how.min_p > 0.0f ? fmax(-log2((double)how.min_p), 0.0) : INFINITY;
     r.k = how.top_k > 0 && how.top_k < a.n ? how.top_k : 0;
     r.p = how.top_p < 1.0f ? fmax((double)how.top_p, 0.0) : 1.0;  // (NaN: all)
     // (a bound of the k-th largest needs k groups; a quarter more leaves it some choice)
     const bool few = r.k && r.k <= FEW && (a.n <= LIST || a.n / GROUP >= r.k + r.k / 4);
     r.mode = !(how.temperature > 0.0f) || top == -INFINITY ? GREEDY : few ? SMALL : r.k || r.p < 1.0 ? BINNED : WHOLE;
-    const double range = fmin((r.m - (double)least) * c, RANGE), g = (BINS - 1) / fmax(range, 1e-30);
-    r.per = c * g;
-    r.inverse = 1.0 / g;
-    r.step = 0.69314718055994530942 / g;
-    r.end = fmin(RANGE * g, BINS - 0.5);  // (nothing lies behind the least value)
-    r.furthest = how.min_p > 0.0f ? fmax(-log2((double)how.min_p), 0.0) * g : INFINITY;
+    // How far the bins reach, in x: to the least value, or where weights end. Top-p alone: tokens beyond log2(n / (1 - p)) + 1
+    // sum to less than half of (1 - p) S, S >= 1, and are not needed to reach p S.
+    const double reach = r.k || r.p == 1.0 ? RANGE : fmin(RANGE, log2(a.n / (1.0 - r.p)) + 1.0);
+    const double range = fmin(r.m - (double)least, reach / r.c);
+    r.half = 0.5f * top;
+    r.scale = range > 0.0 ? (float)fmin((2.0 * BINS - 1.0) / range, 3e38) : 0.0f;
     return r;
 }
 
@@ -204,7 +187,7 @@ template <bool VEC, int T, int EACH> struct Values {
     // f(x, index) for each; -infinity behind the row
     template <class F> __device__ __forceinline__ void each(F f) const {
 #pragma unroll
-        for (int j = 0; j < EACH; ++j) f(v[j], index(j));
+        for (int j = 0; j < EACH; ++j) f(value(v[j]), index(j));
     }
 };
 
@@ -270,7 +253,7 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_scan(Sampl
     });
     // what the next launches add to
     for (int i = chunk * THREADS + threadIdx.x; i < BINS; i += rows.chunks * THREADS) row.count[i] = 0, row.weight[i] = 0;
-    if (chunk == 0 && threadIdx.x == 0) row.listed = 0;
+    if (chunk == 0 && threadIdx.x == 0) row.far = 0, row.listed = 0;
     float group = fmaxf(top, dpp<DPP_XOR1>(top, top));
     group = fmaxf(group, dpp<DPP_XOR2>(group, group));
     if (threadIdx.x % 4 == 0) rows.maxima(number)[chunk * GROUPS + threadIdx.x / 4] = group;
@@ -302,11 +285,10 @@ struct Maxima {
     }
 };
 
-// A bound that k groups' maxima, and so k tokens, reach: as few more as a short search finds. Eight bounds are counted at a
+// A bound that k groups' maxima, and so k tokens, reach: as few more as a short search finds. Four bounds are counted at a
 // time, one by each wave. 0: there are fewer than k.
 __device__ __forceinline__ uint32_t bound_of(const Maxima &m, float top, int k) {
-    constexpr int W = WIDE / 64;
-    __shared__ int counts[W];
+    __shared__ int counts[4];
     constexpr int HELD = Maxima::HELD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, enough = k + k / 4;
     const bool fours = m.n >= enough;  // maxima of four groups where these are still enough
@@ -352,71 +334,52 @@ __device__ __forceinline__ uint32_t bound_of(const Maxima &m, float top, int k) 
         if (best < k) return 0;
     }
     while (best > enough && hi - lo > 1) {
-        const uint32_t step = (hi - lo) / (W + 1) + 1;
+        const uint32_t step = (hi - lo) / 5 + 1;
         const int mine = count_of(min(lo + (wave + 1) * step, hi));
         __syncthreads();  // (what the round before left is read)
         if (lane == 0) counts[wave] = mine;
         __syncthreads();
         int reached = 0;  // bounds that k reach
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
+        for (int w = 0; w < 4; ++w) {
             const int c = counts[w];
             if (c >= k) reached = w + 1, best = c;
         }
         const uint32_t was = lo;
         if (reached) lo = min(was + reached * step, hi);
-        if (reached < W) hi = min(was + (reached + 1) * step, hi);
+        if (reached < 4) hi = min(was + (reached + 1) * step, hi);
     }
     return lo;
 }
 
-// Values of a row's span, units of 256 for `waves` waves, as even as they go.
-__host__ __device__ constexpr int span_units(int n, int waves) { return ((n + UNIT - 1) / UNIT + waves - 1) / waves; }
-template <bool VEC> struct Span {
-    static constexpr int AHEAD = 6;  // on their way (with one, memory's latency is what these kernels wait for)
-    Values<VEC, 64, UNIT / 64> v[AHEAD];
-    const float *x;
-    int n, first, end;
-
-    __device__ __forceinline__ void load(int i, int from) {
-        if (from < end) v[i].load(x, n, from);
-    }
-    __device__ __forceinline__ void begin(const float *row, int of_row, int wave, int waves) {
-        const int units = span_units(of_row, waves);
-        x = row, n = of_row;
-        first = wave * units * UNIT;
-        end = min(first + units * UNIT, n);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) load(i, first + i * UNIT);
-    }
-    // f(x, index) for each, done() after every unit
-    template <class F, class Done> __device__ __forceinline__ void each(F f, Done done) {
+// f(values, piece) for this wave's pieces of a row: every `waves`-th from `wave` on, the next one on its way.
+template <bool VEC> using Piece = Values<VEC, 64, PIECE / 64>;
+template <bool VEC, class F>
+__device__ __forceinline__ void each_piece(Piece<VEC> &now, const float *x, int n, int wave, int waves, F f) {
+    const int pieces = (n + PIECE - 1) / PIECE;
 #pragma unroll 1
-        for (int from = first; from < end; from += AHEAD * UNIT) {
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                if (from + i * UNIT < end) v[i].each(f), done();
-                load(i, from + (i + AHEAD) * UNIT);
-            }
-        }
+    for (int piece = wave; piece < pieces; piece += waves) {
+        Piece<VEC> next;
+        next.load(x, n, min(piece + waves, pieces - 1) * PIECE);
+        f(now, piece);
+        now = next;
     }
-    template <class F> __device__ __forceinline__ void each(F f) { each(f, [] {}); }
-};
+}
 
 // blockIdx.x: one of a row's `parts` workgroups.
-template <bool VEC> __global__ __launch_bounds__(WIDE, 4) void sample_bins(SampleArgs a, Rows rows, int parts) {
+template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(SampleArgs a, Rows rows, int parts) {
     __shared__ union {
-        struct { unsigned count[BINS]; u64 weight[BINS]; double middle[BINS]; } bins;
+        struct { unsigned count[BINS]; u64 weight[BINS]; } bins;
         uint2 list[LIST];
     } lds;
     __shared__ unsigned listed, first;
     const int number = blockIdx.x / parts, part = blockIdx.x % parts;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (WIDE / 64) + (threadIdx.x >> 6)), waves = parts * (WIDE / 64);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (THREADS / 64) + (threadIdx.x >> 6)), waves = parts * (THREADS / 64);
     Row &row = rows.row(number);
     const float *x = a.logits + (size_t)number * a.ld;
     // (on their way while the rule is made)
-    Span<VEC> c;
-    c.begin(x, a.n, wave, waves);
+    Piece<VEC> c;
+    c.load(x, a.n, wave * PIECE);
     Maxima maxima;
     const int k = a.how[number].top_k;
     if (k > 0 && k <= FEW) maxima.load(rows.maxima(number), rows.chunks * GROUPS);
@@ -424,73 +387,76 @@ template <bool VEC> __global__ __launch_bounds__(WIDE, 4) void sample_bins(Sampl
     const Rule r = rule_of(a, row, number, rows.chunks, at);
     if (part == 0 && threadIdx.x == 0) row.rule = r, row.best = at;
     if (r.mode == GREEDY) return;
+    if (r.mode == WHOLE) {
+        each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int piece) {
+            u64 sum = 0;
+            c.each([&](float v, int) {
+                const double y = r.distance(v);
+                if (r.likely(y)) sum += r.weight(y);
+            });
+            sum = last_lane(wave_scan(sum));
+            if (lane == 0) row.sum[piece] = sum;
+        });
+        return;
+    }
     if (r.mode == SMALL) {
         if (threadIdx.x == 0) listed = 0;
         const uint32_t bound = a.n <= LIST ? 0 : bound_of(maxima, (float)r.m, r.k);
         const float least = bound ? of_rising(bound) : -INFINITY;
         __syncthreads();
-        c.each([&](float v, int i) {
-            if (v >= least && v > -INFINITY) {
-                const unsigned to = atomicAdd(&listed, 1u);
-                if (to < LIST) lds.list[to] = make_uint2(i, __float_as_uint(v));
-            }
+        each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int) {
+            c.each([&](float v, int i) {
+                if (v >= least && v > -INFINITY) {
+                    const unsigned to = atomicAdd(&listed, 1u);
+                    if (to < LIST) lds.list[to] = make_uint2(i, __float_as_uint(v));
+                }
+            });
         });
         __syncthreads();
         if (threadIdx.x == 0) first = listed ? atomicAdd(&row.listed, listed) : 0;
         __syncthreads();
-        for (unsigned i = threadIdx.x; i < min(listed, (unsigned)LIST); i += WIDE)
+        for (unsigned i = threadIdx.x; i < min(listed, (unsigned)LIST); i += THREADS)
             if (first + i < LIST) row.list[first + i] = lds.list[i];
         return;
     }
-    for (int i = threadIdx.x; i < BINS; i += WIDE) {
-        const double middle = r.middle(i);
-        lds.bins.count[i] = 0;
-        lds.bins.weight[i] = 0;
-        lds.bins.middle[i] = middle;
-        if (part == 0) row.middle[i] = middle;
-    }
+    for (int i = threadIdx.x; i < BINS; i += THREADS) lds.bins.count[i] = 0, lds.bins.weight[i] = 0;
     __syncthreads();
-    if (r.mode == WHOLE) {
-        u64 sum = 0;
+    u64 far = 0;
+    each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int) {
         c.each([&](float v, int) {
-            const double z = r.distance(v);
-            const int b = r.bin(z);
-            if (b < BINS && r.likely(z)) sum += r.weight(z, lds.bins.middle[b]);
+            const u64 w = r.weight(r.distance(v));
+            const int b = r.bin(v);
+            if (b >= BINS) {
+                far += w;
+            } else if (w) {
+                if (r.k) atomicAdd(&lds.bins.count[b], 1u);
+                atomicAdd(&lds.bins.weight[b], w);
+            }
         });
-        sum = last_lane(wave_scan(sum));
-        if (lane == 0) row.sum[wave] = sum;
-        return;
-    }
-    c.each([&](float v, int) {
-        const double z = r.distance(v);
-        const int b = r.bin(z);
-        if (b < BINS) {
-            if (r.k) atomicAdd(&lds.bins.count[b], 1u);
-            atomicAdd(&lds.bins.weight[b], r.weight(z, lds.bins.middle[b]));
-        }
     });
+    far = last_lane(wave_scan(far));
+    if (lane == 0 && far) atomicAdd(&row.far, far);
     __syncthreads();
-    for (int i = threadIdx.x; i < BINS; i += WIDE)
-        if (lds.bins.weight[i] || (r.k && lds.bins.count[i])) {
+    for (int i = threadIdx.x; i < BINS; i += THREADS)
+        if (lds.bins.weight[i]) {
             if (r.k) atomicAdd(&row.count[i], lds.bins.count[i]);
             atomicAdd(&row.weight[i], lds.bins.weight[i]);
         }
 }
 
-constexpr int PER = BINS / WIDE;
-__device__ __forceinline__ Border border_of(const Rule &r, const unsigned (&count)[PER], const u64 (&weight)[PER]) {
+constexpr int PER = BINS / THREADS;
+__device__ __forceinline__ Border border_of(const Row &row, const Rule &r, const unsigned (&count)[PER], const u64 (&weight)[PER]) {
     __shared__ Border found;
-    __shared__ float edges[4];
     unsigned c = 0, all;
     u64 w = 0, total;
 #pragma unroll
     for (int i = 0; i < PER; ++i) c += count[i], w += weight[i];
     const unsigned mine_c = c;
     const u64 mine_w = w;
-    scan<WIDE>(c, w, all, total);
+    scan<THREADS>(c, w, all, total);
     c -= mine_c;
     w -= mine_w;
-    if (threadIdx.x == 0) found = {-1, BINS, BINS - 1, 0, 0, 0, total, 0, 0, 0, 0};
+    if (threadIdx.x == 0) found = {-1, BINS, BINS - 1, 0, 0, 0, total + row.far};
     __syncthreads();
     if (r.k && all >= (unsigned)r.k) {
         u64 in_front = w;
@@ -521,51 +487,16 @@ __device__ __forceinline__ Border border_of(const Rule &r, const unsigned (&coun
         }
         __syncthreads();
     }
-    // The least values, one by each of four waves: near the one that the middle's distance says, or else of all numbers up to
-    // the maximum a 65th at a time.
-    Border b = found;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int upto = wave == 0 ? b.lo - 1 : wave == 1 ? b.hi : wave == 2 ? b.k_bin - 1 : b.k_bin;
-    const uint32_t past = rising((float)r.m) + 1, none = rising(-INFINITY);
-    uint32_t low = none, high = past;  // the first's bin is past `upto`, that of high and those above is not
-    const auto is_in = [&](uint32_t at) { return r.bin(r.distance(of_rising(at))) <= upto; };
-    if (upto < 0) low = past - 1;
-    else if (wave < 4 && r.per > 0.0) {
-        const uint32_t guess = rising((float)(r.m - (upto + 0.5) / r.per));
-        const uint32_t from = min(max(guess, none + 33) - 32, past - 1), mid = min(from + lane, past - 1);
-        const unsigned long long mask = __ballot(is_in(mid));
-        if (mask && !(mask & 1)) {
-            high = min(from + __builtin_ctzll(mask), past - 1);
-            low = high - 1;
-        }
-    }
-    while (wave < 4 && high - low > 1) {
-        const uint32_t step = (high - low) / 65 + 1, mid = min(low + (lane + 1) * step, high);
-        const unsigned long long mask = __ballot(mid == high || is_in(mid));
-        const int below = mask ? __builtin_ctzll(mask) : 64;  // of the 64, past `upto`
-        const uint32_t from = low;
-        low = below ? min(from + below * step, high) : from;
-        high = below < 64 ? min(from + (below + 1) * step, high) : high;
-        if (low == high) low = high - 1;
-    }
-    if (lane == 0 && wave < 4) edges[wave] = high == past ? __builtin_nanf("") : of_rising(high);
-    __syncthreads();
-    b.in_front = edges[0];
-    b.upto_hi = edges[1];
-    b.above_k = edges[2];
-    b.upto_k = b.k_bin < 0 ? __builtin_nanf("") : edges[3];
-    return b;
+    return found;
 }
 
 // blockIdx.x: one of a row's `parts` workgroups.
-template <bool VEC> __global__ __launch_bounds__(WIDE, 4) void sample_border(SampleArgs a, Rows rows, int parts) {
+template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(SampleArgs a, Rows rows, int parts) {
     __shared__ unsigned listed, first;
     __shared__ uint2 list[LIST];
-    constexpr int QUEUE = 512;
-    __shared__ float queues[WIDE / 64][QUEUE + UNIT + 1];
-    __shared__ double middles[BINS];
+    __shared__ float queues[THREADS / 64][PIECE];
     const int number = blockIdx.x / parts, part = blockIdx.x % parts;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (WIDE / 64) + (threadIdx.x >> 6)), waves = parts * (WIDE / 64);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (THREADS / 64) + (threadIdx.x >> 6)), waves = parts * (THREADS / 64);
     Row &row = rows.row(number);
     if (row.rule.mode != BINNED) return;
     const float *x = a.logits + (size_t)number * a.ld;
@@ -573,52 +504,41 @@ template <bool VEC> __global__ __launch_bounds__(WIDE, 4) void sample_border(Sam
     u64 weight[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) count[i] = row.count[threadIdx.x * PER + i], weight[i] = row.weight[threadIdx.x * PER + i];
-    Span<VEC> c;
-    c.begin(x, a.n, wave, waves);
+    Piece<VEC> c;
+    c.load(x, a.n, wave * PIECE);
     const Rule r = row.rule;
-    const Border b = border_of(r, count, weight);
+    const Border b = border_of(row, r, count, weight);
     if (part == 0 && threadIdx.x == 0) row.border = b;
     if (threadIdx.x == 0) listed = 0;
-    for (int i = threadIdx.x; i < b.lo; i += WIDE) middles[i] = row.middle[i];
     __syncthreads();
     float *queue = queues[threadIdx.x >> 6];
-    // The values in front of the border, close together: few of a wave's 64 are, and their weights are what costs.
-    int queued = 0;
-    u64 sum = 0;
-    const auto add_up = [&](int n) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-        for (int i = lane; i < n; i += 64) {
-            const double z = r.distance(queue[i]);
-            if (r.likely(z)) sum += r.weight(z, middles[min(r.bin(z), BINS - 1)]);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    };
-    const bool tops = b.k_bin > b.hi;
-    c.each([&](float v, int i) {
-        const bool is = v >= b.in_front;
-        const unsigned long long mask = __ballot(is);
-        const int to = queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-        queue[is ? to : QUEUE + UNIT] = v;  // (the last place is nobody's)
-        queued += __popcll(mask);
-        if (__any(!is && (v >= b.upto_hi || (tops && v >= b.upto_k)))) {
-            if (!is && (v >= b.upto_hi || (v >= b.upto_k && !(v >= b.above_k)))) {
+    each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int piece) {
+        // the values in front of the border, close together: few of a wave's 64 are, and their weights are what costs
+        int queued = 0;
+        c.each([&](float v, int i) {
+            const int bin = r.bin(v);
+            const unsigned long long in_front = __ballot(bin < b.lo);
+            if (bin < b.lo) queue[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(in_front >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in_front, 0))] = v;
+            queued += __popcll(in_front);
+            if (bin >= b.lo && (bin <= b.hi || bin == b.k_bin)) {
                 const unsigned to = atomicAdd(&listed, 1u);
                 if (to < LIST) list[to] = make_uint2(i, __float_as_uint(v));
             }
+        });
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        u64 sum = 0;
+        for (int i = lane; i < queued; i += 64) {
+            const double y = r.distance(queue[i]);
+            if (r.likely(y)) sum += r.weight(y);
         }
-    }, [&]() {
-        if (queued >= QUEUE) {
-            add_up(queued);
-            queued = 0;
-        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        if (queued) sum = last_lane(wave_scan(sum));
+        if (lane == 0) row.sum[piece] = sum;
     });
-    add_up(queued);
-    sum = last_lane(wave_scan(sum));
-    if (lane == 0) row.sum[wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) first = listed ? atomicAdd(&row.listed, listed) : 0;
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < min(listed, (unsigned)LIST); i += WIDE)
+    for (unsigned i = threadIdx.x; i < min(listed, (unsigned)LIST); i += THREADS)
         if (first + i < LIST) row.list[first + i] = list[i];
 }
 
@@ -640,10 +560,9 @@ __device__ __forceinline__ void each_listed(const Listed &list, const Rule &r, c
     } else {
         for (int i = threadIdx.x; i < n; i += DRAW) {
             const float v = value(x[i]);
-            const double z = r.distance(v);
-            const int bin = r.bin(z);
+            const int bin = r.bin(v);
             if (bin < lo || bin > hi) continue;
-            const u64 w = r.weight(z);
+            const u64 w = r.weight(r.distance(v));
             if (w) f(place(v, i), w);
         }
     }
@@ -657,7 +576,7 @@ __device__ __forceinline__ u64 last_place(const Listed &list, const Rule &r, con
     __shared__ unsigned counts[256];
     __shared__ u64 weights[256], highest[256], least, most;
     __shared__ struct { unsigned digit, count, here; u64 weight, mine; } next;
-    if (threadIdx.x == 0) least = ~0ull, most = 0, next = {0, count, 1, weight, 0};
+    if (threadIdx.x == 0) least = ~0ull, most = 0;
     __syncthreads();
     u64 a = ~0ull, b = 0;
     each_listed(list, r, x, n, lo, hi, [&](u64 at, u64) { a = min(a, at), b = max(b, at); });
@@ -812,9 +731,9 @@ __device__ __forceinline__ bool order(Ordered &o, Token (&t)[HELD]) {
     return true;
 }
 
-template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleArgs a, Rows rows, int waves) {
-    __shared__ u64 sums[MOST_SPANS], highest, of_k;
-    __shared__ struct { int span; u64 before; } hit;
+template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleArgs a, Rows rows) {
+    __shared__ u64 sums[MOST_PIECES], highest, of_k;
+    __shared__ struct { int piece; u64 before; } hit;
     __shared__ unsigned in_front, near;
     __shared__ union {
         Ordered ordered;
@@ -829,11 +748,11 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
     const unsigned listed = row.listed;
     const double u = a.u[number];
     Border b = row.border;
-    constexpr int MINE = MOST_SPANS / DRAW;
-    const int span = span_units(a.n, waves) * UNIT;
-    u64 of_span[MINE];
+    constexpr int MINE = MOST_PIECES / DRAW;
+    const int pieces = (a.n + PIECE - 1) / PIECE;
+    u64 of_piece[MINE];
 #pragma unroll
-    for (int j = 0; j < MINE; ++j) of_span[j] = row.sum[threadIdx.x * MINE + j];
+    for (int j = 0; j < MINE; ++j) of_piece[j] = row.sum[threadIdx.x * MINE + j];
     uint2 of_list[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) of_list[i] = row.list[threadIdx.x + i * DRAW];
@@ -847,28 +766,26 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
     }
     // tokens in front of bin b.lo are kept, and of bins up to b.hi those up to the place `last`
     u64 last = 0;
-    if (r.mode == WHOLE) b = {-1, BINS + 1, BINS, 0, 0, 0, 0, 0, 0, 0, 0};
-    if (r.mode == SMALL) b = {0, 0, BINS, 0, 0, 0, 0, 0, 0, 0, 0};
+    if (r.mode == WHOLE) b = {-1, BINS + 1, BINS, 0, 0, 0, 0};
+    if (r.mode == SMALL) b = {0, 0, BINS, 0, 0, 0, 0};
     const int k_end = r.mode == SMALL ? b.hi : b.k_bin;  // bins k_bin .. k_end hold top-k's last token
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
-        const int i = threadIdx.x * MINE + j;
-        sums[i] = i < waves && r.mode != SMALL ? of_span[j] : 0;
+        const int piece = threadIdx.x * MINE + j;
+        sums[piece] = piece < pieces && r.mode != SMALL ? of_piece[j] : 0;
     }
     Token t[HELD];
     int bin[HELD];
     bool keep[HELD], small = false;
-    if (threadIdx.x == 0) hit = {0, 0};
     if (r.mode != WHOLE) {
         if (threadIdx.x == 0) highest = 0, of_k = 0, in_front = 0, near = 0;
         unsigned front = 0;
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
             const bool is = listed <= LIST && threadIdx.x + i * DRAW < listed;
-            const float v = value(__uint_as_float(of_list[i].y));
-            const double z = r.distance(v);
-            t[i] = {is ? place(v, of_list[i].x) : ~0ull, is ? r.weight(z) : 0, 0, 0};
-            bin[i] = is ? r.bin(z) : BINS + 1;
+            const float v = __uint_as_float(of_list[i].y);
+            t[i] = {is ? place(v, of_list[i].x) : ~0ull, is ? r.weight(r.distance(v)) : 0, 0, 0};
+            bin[i] = is ? r.bin(v) : BINS + 1;
             front += bin[i] < b.k_bin;
             keep[i] = false;
         }
@@ -905,7 +822,7 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
                 keep[i] = keep[i] && t[i].w && r.likely(r.distance(of_rising(~(uint32_t)(t[i].at >> 32))));
-                if (keep[i]) atomicAdd(&sums[(uint32_t)t[i].at / span], t[i].w);
+                if (keep[i]) atomicAdd(&sums[(uint32_t)t[i].at / PIECE], t[i].w);
             }
             __syncthreads();
             last = highest;
@@ -933,7 +850,7 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
                 last = last_place(lds.list, r, x, a.n, b.lo, b.hi, 0, w, [&](unsigned, u64 s) { return (double)s >= share; });
             }
             each_listed(lds.list, r, x, a.n, b.lo, b.hi, [&](u64 at, u64 w) {
-                if (at <= last && r.likely(r.distance(of_rising(~(uint32_t)(at >> 32))))) atomicAdd(&sums[(uint32_t)at / span], w);
+                if (at <= last && r.likely(r.distance(of_rising(~(uint32_t)(at >> 32))))) atomicAdd(&sums[(uint32_t)at / PIECE], w);
             });
         }
     }
@@ -941,23 +858,22 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
     u64 total;
     u64 mine = 0;
 #pragma unroll
-    for (int j = 0; j < MINE; ++j) mine += of_span[j] = sums[threadIdx.x * MINE + j];
+    for (int j = 0; j < MINE; ++j) mine += of_piece[j] = sums[threadIdx.x * MINE + j];
     u64 upto = mine;
     scan<DRAW>(upto, total);
-    if (!total) return;  // (never: the maximum weighs 1)
     const u64 target = target_of(u, total);
     upto -= mine;
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
-        if (upto <= target && upto + of_span[j] > target) hit = {(int)threadIdx.x * MINE + j, upto};
-        upto += of_span[j];
+        if (upto <= target && upto + of_piece[j] > target) hit = {(int)threadIdx.x * MINE + j, upto};
+        upto += of_piece[j];
     }
     __syncthreads();
     if (small) {
-        // all kept tokens are at hand: those of the span
+        // all kept tokens are at hand: those of the piece
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
-            if (keep[i] && (int)((uint32_t)t[i].at / span) == hit.span) {
+            if (keep[i] && (int)((uint32_t)t[i].at / PIECE) == hit.piece) {
                 const unsigned to = atomicAdd(&near, 1u);
                 lds.near.at[to] = (uint32_t)t[i].at;
                 lds.near.w[to] = t[i].w;
@@ -970,34 +886,28 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
         }
         return;
     }
-    // the span's values, one per thread at a time, up to those that pass the target
-    u64 so_far = hit.before;
-    const int first = hit.span * span, end = min(first + span, a.n);
-    for (int from = first; from < end && so_far <= target; from += DRAW) {
-        const int at = from + threadIdx.x;
-        u64 w = 0;
-        if (at < end) {
-            const float v = value(x[at]);
-            const double z = r.distance(v);
-            const int in = r.bin(z);
-            if (r.likely(z) && (in < b.lo || (in <= b.hi && place(v, at) <= last))) w = r.weight(z);
-        }
-        u64 before = w, here;
-        scan<DRAW>(before, here);
-        drawn(a, number, target, so_far + before - w, w, total, at);
-        so_far += here;
+    // the piece's values, one per thread
+    const int at = hit.piece * PIECE + threadIdx.x;
+    u64 w = 0;
+    if (threadIdx.x < PIECE && at < a.n) {
+        const float v = value(x[at]);
+        const double y = r.distance(v);
+        const int in = r.bin(v);
+        if (r.likely(y) && (in < b.lo || (in <= b.hi && place(v, at) <= last))) w = r.weight(y);
     }
+    u64 before = w, here;
+    scan<DRAW>(before, here);
+    drawn(a, number, target, hit.before + before - w, w, total, at);
 }
 
 template <bool VEC> void launch(const SampleArgs &a, const Rows &rows, int n, hipStream_t st) {
     const dim3 block(THREADS);
-    // workgroups of a row: two for each CU in all, two units for each wave at least
-    constexpr int W = WIDE / 64;
-    const int parts = std::max(1, std::min({(a.n / UNIT + 2 * W - 1) / (2 * W), 512 / n, MOST_SPANS / W}));
+    // workgroups of a row: four for each CU in all, a piece for each wave at least
+    const int pieces = (a.n + PIECE - 1) / PIECE, parts = std::max(1, std::min((pieces + 3) / 4, 1024 / n));
     hipLaunchKernelGGL((sample_scan<VEC>), dim3(n * rows.chunks), block, 0, st, a, rows);
-    hipLaunchKernelGGL((sample_bins<VEC>), dim3(n * parts), dim3(WIDE), 0, st, a, rows, parts);
-    hipLaunchKernelGGL((sample_border<VEC>), dim3(n * parts), dim3(WIDE), 0, st, a, rows, parts);
-    hipLaunchKernelGGL((sample_draw<VEC>), dim3(n), dim3(DRAW), 0, st, a, rows, parts * W);
+    hipLaunchKernelGGL((sample_bins<VEC>), dim3(n * parts), block, 0, st, a, rows, parts);
+    hipLaunchKernelGGL((sample_border<VEC>), dim3(n * parts), block, 0, st, a, rows, parts);
+    hipLaunchKernelGGL((sample_draw<VEC>), dim3(n), dim3(DRAW), 0, st, a, rows);
 }
 
 }  // namespace

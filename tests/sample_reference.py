@@ -1,8 +1,8 @@
 """Sampling restated in extended precision, one row at a time.
 
 The kernel holds weights to 2^-44 of the largest (one) and adds them exactly, and forms u W and p S in 64 bits: a running sum is
-off from its value by at most n (2^-44 + 2^-46) + 2^-52 W: half a multiple, the weights' own 64-bit arithmetic (bins of up to
-2047, whose rounding is 2^-53 of that, by ln(2) / 46 in the exponent: 2^-47; the series 2^-46), and the borders. A choice that lies within twice that of its border may go either way: `choices` gives every token that it may be."""
+off from its value by at most n (2^-44 + 2^-51) + 2^-52 W, the last for the borders and for weights' own 64-bit arithmetic
+(2^-51 of a weight). A choice that lies within twice that of its border may go either way: `choices` gives every token that it may be."""
 import numpy as np
 
 LD = np.longdouble
