@@ -576,7 +576,7 @@ __device__ __forceinline__ u64 last_place(const Listed &list, const Rule &r, con
     __shared__ unsigned counts[256];
     __shared__ u64 weights[256], highest[256], least, most;
     __shared__ struct { unsigned digit, count, here; u64 weight, mine; } next;
-    if (threadIdx.x == 0) least = ~0ull, most = 0;
+    if (threadIdx.x == 0) least = ~0ull, most = 0, next = {0, count, 1, weight, 0};  // (a digit is always found)
     __syncthreads();
     u64 a = ~0ull, b = 0;
     each_listed(list, r, x, n, lo, hi, [&](u64 at, u64) { a = min(a, at), b = max(b, at); });
@@ -861,6 +861,13 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
     for (int j = 0; j < MINE; ++j) mine += of_piece[j] = sums[threadIdx.x * MINE + j];
     u64 upto = mine;
     scan<DRAW>(upto, total);
+    if (!total) {  // (the maximum is kept and weighs 2^43: no row comes here, and none reads behind its end for want of a piece)
+        if (threadIdx.x == 0) {
+            a.ids[number] = -1;
+            if (a.prob) a.prob[number] = 0.0f;
+        }
+        return;
+    }
     const u64 target = target_of(u, total);
     upto -= mine;
 #pragma unroll
