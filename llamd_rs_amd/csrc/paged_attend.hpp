@@ -43,6 +43,7 @@ struct Split {
     Parts many, few;     // of paged_tiles (blocks of 32 rows) and of paged_few
     int few_rows;        // rows of a slot of the latter: 16, or in decode a sequence's and kv head's, if fewer
     int parts;           // most parts of a row tile (prompt, prefix)
+    int fine;            // parts of a shared prefix of 8-bit pages that may be short (prefix_parts); parts at the most
     int tiles;           // decode: tiles of shared prefixes that there are slots for
     double per_item;     // decode: 1 / (positions of all sequences' parts wanted, in steps)
     double per_row;      // decode: 1 / (parts of a sequence, in steps, while they are short)
@@ -711,6 +712,13 @@ template <class E> __host__ __device__ constexpr int tile_least() { return E::RU
 // the most tiles that a prompt's rows are not split for: the join costs as much (512 tokens 22 us, in two parts 27; 1024 33,
 // in four 41).
 template <class E> __host__ __device__ constexpr int prefix_least() { return E::RUN == 8 ? 8 : 1; }
+// 8-bit pages: up to Split::fine parts of 4 steps at least (8 sequences behind 7800 positions 20.3 us, by 8 steps 24.2; 64
+// behind 1300 21.6 and 28.0; 20 behind 8700, heads of 256, 32.0 and 42.3).
+constexpr int SHORT_PREFIX = 4;
+template <class E> __device__ __forceinline__ int prefix_parts(const Split &sp, int steps) {
+    const int parts = parts_of(steps, sp.parts, prefix_least<E>());
+    return bytes_of<E> ? max(parts, parts_of(steps, sp.fine, SHORT_PREFIX)) : parts;
+}
 template <class E> __host__ __device__ constexpr int whole_steps() { return E::RUN == 8 ? 16 : 1; }
 template <class E> __device__ __forceinline__ int prompt_parts(int steps, int most) {
     return steps <= whole_steps<E>() ? 1 : parts_of(steps, most, tile_least<E>());
@@ -754,8 +762,7 @@ __device__ __forceinline__ void tile_rows(const PagedAttendArgs &a, const Split 
         if (!prompt_tile_by_size<R, KT == 64 ? 6 : 5>(p, unit, at.nx / p.n_kv_head, unit, tile, t)) return;
         row = prompt_row<R>(p, tile, t, kvh, 32 * wave + m);
     }
-    const int steps = (t.top + KT - 1) / KT, parts = PREFIX ? parts_of(steps, sp.parts, prefix_least<E>())
-                                                    : prompt_parts<E>(steps, sp.parts);
+    const int steps = (t.top + KT - 1) / KT, parts = PREFIX ? prefix_parts<E>(sp, steps) : prompt_parts<E>(steps, sp.parts);
     if (at.y >= parts) return;
     const int2 range = part_steps(steps, parts, at.y);
     const Pages<E> g = pages_of<E, HD>(p, t.seq, kvh);
@@ -1189,7 +1196,7 @@ __global__ __launch_bounds__(256) void paged_join_decode(PagedAttendArgs a, Spli
         for (int i = lane; i < number; i += WAVE) tiles = add_tiles(tiles, prefix_units<R>(a, group_at(a, i)), sp.tiles);
         base = wave_reduce(tiles, 0, [](int x, int y) { return x + y; });
         constexpr int KT = tile_positions<E, HD>();
-        parts = parts_of((readable_of(p, g.shared) + KT - 1) / KT, sp.parts, prefix_least<E>());
+        parts = prefix_parts<E>(sp, (readable_of(p, g.shared) + KT - 1) / KT);
         first = (long long)(seq - g.first) * p.group + head;
     }
     const auto many = [&](int z, int r) {  // the slot of a row's 32-row block
@@ -1314,6 +1321,14 @@ int decode_as(const PagedAttendArgs &a, hipStream_t st) {
         tiles = plan.tiles;
         sp.parts = plan.parts;
         sp.tiles = (int)tiles;
+        // short parts in two fifths of the places, two workgroups per CU, that the sequences' own positions leave: past that
+        // two tiles share a CU (4 kv heads, 48 sequences behind 4100: 8 parts 26.5 us, 10 25.5, 12 24.4, 14 26.4, 16 28.6;
+        // behind 3900 26.4, 23.9, 26.3, 27.5, 28.8; 32 behind 4100 25.7, 24.5, 23.0, 22.6, 23.0; where nothing is left,
+        // 12 kv heads of 64 and 64 sequences behind 3600, 7 parts 25.8 us, 11 26.6)
+        const long long filled = std::max(((long long)p.n_seq * p.group + R - 1) / R, (long long)std::min(a.n_groups, p.n_seq / 2));
+        sp.fine = bytes_of<E> && tiles ? at_least_one((2LL * CUS - (long long)p.n_seq * cols) * 2 / (5 * filled * p.n_kv_head),
+                                                      top / (KT * SHORT_PREFIX), 64) : 1;
+        sp.parts = std::max(sp.parts, sp.fine);
         slots = tiles * p.n_kv_head * sp.parts * 4;
     }
     if (items * cols > 0x7FFFFFFF / 512 || cols > 65535 || tiles * p.n_kv_head > 0x7FFFFFFF / 512) return -1;
