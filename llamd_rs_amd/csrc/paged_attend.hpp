@@ -1259,11 +1259,14 @@ int prompt_tiles(const PagedAttendArgs &a, hipStream_t st) {
     return queued();
 }
 
+// Workgroups of paged_few that are resident at once.
+template <int HD> constexpr int few_resident() { return (HD <= 128 ? 3 : 2) * CUS; }
+
 template <class E, int HD>
 int prompt_few(const PagedAttendArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
     // as many workgroups as are resident (16 tokens after 12000 positions: 33.5 us, for 2 per CU 42, for 4 40)
-    const TilePlan plan = plan_tiles((long long)p.n_tok * p.group, std::min(p.n_seq, p.n_tok), 16, p.n_kv_head, (HD <= 128 ? 3 : 2) * CUS,
+    const TilePlan plan = plan_tiles((long long)p.n_tok * p.group, std::min(p.n_seq, p.n_tok), 16, p.n_kv_head, few_resident<HD>(),
                                      ((long long)p.max_page << p.page_log) / few_step<E>, 128);
     const long long tiles = plan.tiles;
     Split sp{};
@@ -1292,6 +1295,12 @@ int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
     // taken 16 rows at a time (4096 tokens in 1024 places 939 us, in 256 165, alone 154; 2000 tokens beside 400 single ones 311,
     // in two calls 60 and 87)
     if (rows <= 64 || total * p.n_kv_head <= 768 || total * p.n_kv_head * top <= 5 << 19) return prompt_few<E, HD>(a, st);
+    // 8-bit pages, whose 16-row steps are 64 positions: also where tiles would not be split and the 16-row ones are resident
+    // at once with some to spare (256 tokens after 500 positions 15.8 us, in larger tiles 25.0; 9 x 40 after 900 18.6 and 30.6;
+    // 16 query and 8 kv heads: 512 tokens 11.4 and 18.6; heads of 256: 9 x 100 after 900 38.9 and 55.7). Beyond: 9 x 100 after
+    // 900 of 16 and 8 heads, 584 tiles, 31.8 and 32.4; 400 tokens, 800 tiles, 19.2 and 17.1; 128 tokens after 1500 25.2 and 20.6
+    if (bytes_of<E> && top <= tile_positions<E, HD>() * whole_steps<E>() && total * p.n_kv_head <= 16 * few_resident<HD>() * 3 / 4)
+        return prompt_few<E, HD>(a, st);
     // eight waves where all CUs still have work (32 query heads on 4: 4096 tokens 175 us, four waves 195; 3000 110 and 101)
     if constexpr (wide<E, HD>())
         if (rows >= 1024 && total * p.n_kv_head >= 512 * 256) return prompt_tiles<E, HD, 8>(a, st);
