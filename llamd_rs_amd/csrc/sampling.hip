@@ -919,15 +919,27 @@ template <bool VEC> void launch(const SampleArgs &a, const Rows &rows, int n, hi
 
 }  // namespace
 
+// Rows at a time: a row's scratch is 61 KB and more, and so many fill the GPU.
+constexpr int MOST_ROWS = 1024;
+
 int launch_sample(const SampleArgs &a, int n, hipStream_t st) {
     Rows rows;
     rows.chunks = (a.n + CHUNK - 1) / CHUNK;
     rows.step = sizeof(Row) + (size_t)rows.chunks * GROUPS * sizeof(float);
     const std::lock_guard<std::mutex> lk(lib_scratch_mutex());
-    rows.base = (char *)lib_scratch(n * rows.step);
+    rows.base = (char *)lib_scratch(std::min(n, MOST_ROWS) * rows.step);
     if (!rows.base) return -1;
-    if (((uintptr_t)a.logits & 15) == 0 && a.ld % 4 == 0) launch<true>(a, rows, n, st);
-    else launch<false>(a, rows, n, st);
+    for (int first = 0; first < n; first += MOST_ROWS) {
+        SampleArgs x = a;
+        x.logits += (size_t)first * a.ld;
+        x.how += first;
+        x.u += first;
+        x.ids += first;
+        if (x.prob) x.prob += first;
+        const int here = std::min(n - first, MOST_ROWS);
+        if (((uintptr_t)x.logits & 15) == 0 && a.ld % 4 == 0) launch<true>(x, rows, here, st);
+        else launch<false>(x, rows, here, st);
+    }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

@@ -249,6 +249,23 @@ def test_prompt_long(gpu, heads, kvh, hd, page, new, old):
     R.check(c.prompt(q, table, lengths, start, scale=0.1), want, bound)
 
 
+@pytest.mark.parametrize("heads,kvh,hd,page,new,old", [
+    (32, 4, 128, 64, [256], [500]), (8, 2, 128, 16, [90, 300, 1, 77], [600, 0, 700, 333]), (8, 2, 256, 64, [100, 33, 90], [900, 871, 4]),
+    (12, 12, 64, 32, [512], [0]), (2, 2, 64, 128, [1000], [24])])
+def test_prompt_of_a_turn(gpu, heads, kvh, hd, page, new, old):
+    """Many rows after contexts of up to 1024 positions, as many as run at once and a few more."""
+    rng = np.random.default_rng(24)
+    lengths = [a + b for a, b in zip(new, old)]
+    table, n_page = tables(rng, lengths, page)
+    start = np.concatenate([[0], np.cumsum(new)])
+    c, k, v = filled(gpu, rng, table, n_page, page, heads, kvh, hd, lengths)
+    q = rounded(rng.standard_normal((start[-1] + 3, heads * hd)) * 1.5, "bf16")
+    want, bound = want_prompt(q, k, v, table, lengths, start, heads, kvh, hd, hd ** -0.5, "bf16")
+    got = c.prompt(q, table, lengths, start)
+    R.check(got, want, bound)
+    assert not got[-3:].any()
+
+
 def test_f32_results(gpu):
     rng = np.random.default_rng(23)
     table, n_page = tables(rng, [90, 4], 16)
@@ -391,6 +408,32 @@ def test_decode_shared_prefix(gpu, heads, kvh, hd, page, group, shared, lengths)
     # the same batch without the groups
     want, bound = want_decode(q, k, v, table, lengths, heads, kvh, hd, hd ** -0.5, "bf16")
     R.check(c.decode(q, table, lengths), want, bound)
+
+
+@pytest.mark.parametrize("heads,kvh,hd,page,group,shared,lengths", [
+    (32, 4, 128, 64, [0, 8], [4100], [4101 + 37 * i for i in range(8)]),
+    (8, 2, 256, 64, [1, 4], [2600], [5, 2601, 2600, 2900]),
+    (8, 1, 64, 16, [0, 3, 6], [1500, 600], [1500, 1501, 1700, 601, 900, 650])])
+def test_decode_long_shared_prefix(gpu, heads, kvh, hd, page, group, shared, lengths):
+    """Few tiles of long prefixes, cut into short parts; the same call again gives the same bits."""
+    rng = np.random.default_rng(35)
+    table, n_page, copies = shared_tables(rng, group, shared, lengths, page)
+    c, _, _ = filled(gpu, rng, table, n_page, page, heads, kvh, hd, lengths)
+    b = [x.copy() for x in c.read_bytes()]
+    for to, of, _ in copies:
+        for x in b:
+            x[to] = x[of]
+    for x in (b[0], b[1]):
+        x[x & 127 == 127] = 3
+    for x in (b[2], b[3]):
+        x[(x < 100) | (x > 150)] = 120
+    c.write_bytes(*b)
+    k, v = c.read()
+    q = rounded(rng.standard_normal((len(lengths), heads * hd)) * 1.5, "bf16")
+    want, bound = want_decode(q, k, v, table, lengths, heads, kvh, hd, hd ** -0.5, "bf16", group, shared)
+    got = c.decode(q, table, lengths, group, shared)
+    R.check(got, want, bound)
+    assert np.array_equal(got, c.decode(q, table, lengths, group, shared))
 
 
 def test_decode_missing_pages_and_nan_that_a_member_does_not_see(gpu):

@@ -51,6 +51,12 @@ def test_many_rows(gpu):
     check(gpu, x, rules, rng.random(300))
 
 
+def test_more_rows_than_go_at_a_time(gpu):
+    rng = np.random.default_rng(22)
+    x = logits(rng, 2049, 41)
+    check(gpu, x, [RULES[i % len(RULES)] for i in range(2049)], rng.random(2049))
+
+
 @pytest.mark.parametrize("ends", [[0.0, 1.0 - 2.0 ** -53, 1.0, 2.0, -1.0, np.nan, np.inf, -np.inf]])
 def test_random_numbers_at_their_ends(gpu, ends):
     rng = np.random.default_rng(3)
