@@ -512,7 +512,7 @@ int llamd_hip_paged_decode(const llamd_hip_pages *c, const llamd_hip_batch *b, c
  *
  * What is said above holds, with these differences. q and q_out are bf16, results
  * bf16 or f32; products and weights are those of a bf16 cache, which holds
- * every element exactly. paged8_store takes for 16 positions the least E with
+ * every element exactly (of V, where E is 10 or more). paged8_store takes for 16 positions the least E with
  * which the new ones' largest finite value fits (448 * 2^(E - 127)), or the E
  * there where positions of the sequence before the new ones need more; where E
  * grows, those positions' numbers are rounded again (exactly but for values below

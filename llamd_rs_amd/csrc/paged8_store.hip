@@ -13,6 +13,10 @@
 // from the length to the block's scale. One launch: queries as in paged_store.hip, a wave per token; and a workgroup per 16
 // positions, kv head, and K or V, since the unit is the largest of them all: HD / 8 lanes hold a token's head, the 16 tokens'
 // values stay in registers between the maximum and the rounding. V's bytes are turned in LDS.
+//
+// Measured (one MI355X): 8000 tokens of 32 query and 4 kv heads of 128, 238 MB, 52.1 us (4.6 TB/s, a large copy's rate is 4.7); 5
+// prompts of 16 and 8 heads, 52 MB, 14.1 us; one token 7.1 us, of which the kernel 5.2 (of a 16-bit cache
+// 4.0). The values' loads beside the page's number, and V's old bytes before the norm: 7.3, 14.6 and 53.2.
 #include <algorithm>
 
 #include "paged_store.hpp"
@@ -212,8 +216,10 @@ int store_as(const PagedStoreArgs &a, hipStream_t st) {
     const PagedArgs &p = a.p;
     // 16-position blocks of all sequences: a whole one per 16 tokens, and two that are not
     const long long blocks = std::min((long long)p.n_tok / POS + 2LL * p.n_seq, (long long)p.n_tok);
-    // four waves per token while that leaves CUs idle otherwise
-    const int waves = a.n_rot % 8 ? 0 : p.n_tok < 2048 ? 4 : 1;
+    // four waves per token while one's chain of heads takes longer than the tokens take the GPU (one and four, 4 kv heads of 128: 32
+    // heads, 500 tokens 7.3 and 7.2 us, 700 7.7 and 9.0, 1900 12.9 and 16.0; 128 heads, 1 token 13.7 and 7.3, 500 16.3 and 11.0,
+    // 2000 44.2 and 42.6; the wrong way at 64 heads, 1000 tokens, 12.4 and 13.5, and at 128, 2900, 63.8 and 58.8)
+    const int waves = a.n_rot % 8 ? 0 : p.n_tok < p.n_head * HD / 8 ? 4 : 1;
     const int tokens = !a.x[0] ? 0 : waves == 1 ? (p.n_tok + 3) / 4 : p.n_tok;
     const long long grid = tokens + 2 * blocks * p.n_kv_head;
     if (grid > 0x7FFFFFFF / 256) return -1;

@@ -12,12 +12,18 @@
 // matrix operands. Either may have a part of a row's positions only; then O (unnormalised), the maximum and the sum
 // go to scratch and paged_join or paged_join_decode puts the parts together, in a fixed order.
 //
+// 8-bit pages (e4m3 numbers with a power of two for each 16 positions): q, weights and products are bf16's. tile_rows widens K and V
+// once for all rows, on their way into LDS; few_rows widens them in registers, K without its scale, which goes to the scores: 16
+// bytes of a row are two steps' operands, so that a step is 64 positions.
+//
 // Bound and measured (32 query heads on 4 kv heads of 128, one MI355X). Long prompts of 16 bits: products and the softmax's
 // vector work, one after the other (8192 tokens of bf16: matrix cores busy 46% of the cycles, vector units 53%; 560 us, 980
 // TFLOP/s of the causal half, where a library product of 8192^3 reaches 1349); f32 110 to 119 of 154. Pieces and packed
 // prompts: the steps of a CU's tiles, 1.1 us each, and 8 us to every workgroup's first product (512 tokens after 7000 81 us,
 // 9 prompts of 192 to 700 tokens 41). Decode: memory, then the chain length -> table -> keys and the second launch (1 x 4100
-// 12.8 us, 13 x 1000 in f32 20.4, 48 behind 4100 shared 25.8).
+// 12.8 us, 13 x 1000 in f32 20.4, 48 behind 4100 shared 25.8). 8-bit pages: 8192 tokens 575 us (956 TFLOP/s), 512 after
+// 7000 84, 9 packed prompts 40.6; decode 1 x 4100 12.3, 61 x 500 to 2000 (79 MB) 28.3, of these 23 at 3.4 TB/s and the join 5.4,
+// 48 behind 4100 shared 25.4.
 #pragma once
 
 #include <algorithm>

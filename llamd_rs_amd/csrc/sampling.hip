@@ -8,20 +8,24 @@
 // neither do results, and 2^20 of them stay inside 64 bits. A weight is off by 2^-44 then, of 2^20 of them the sum by 2^-24
 // at the very worst and 2^-35 by chance; a token whose weight is below that is not drawn.
 //
-// Four launches, rows in chunks of 4096:
-//   sample_scan: maximum and minimum of each chunk, and the maxima of each 64 values
-//   sample_bins, by the row's rule:
+// Four launches; the host does not see the rules, so all four whatever they are:
+//   sample_scan, chunks of 4096: maximum and minimum of each, and the maxima of each 64 values
+//   sample_bins, pieces of 512 values per wave, by the row's rule:
 //     top-k of up to 1024: the k-th largest of the maxima bounds the k-th largest value from below; the tokens above the
 //       bound are listed (50 of 151936: about 55 tokens)
 //     top-p (or a larger k) alone: weights (counts) by distance from the maximum, 2048 bins, in LDS and then by integer atomics
-//     neither: there is no border, the chunks' weights are added up
+//     neither: there is no border, the pieces' weights are added up
 //   sample_border: rows with bins only: the bins that hold the border; their tokens are listed, the weights in front of them
-//     added up by chunk
+//     added up by piece (gathered in LDS first: of a wave's 64 values few are in front, and their exponentials are what costs)
 //   sample_draw: one workgroup per row. A small top-k's tokens are sorted, cut, and sorted by index. Else the border is found
-//     among the listed tokens by digits of (x, index), then the chunk that u falls into, and the token in it. Where a list is too
+//     among the listed tokens by digits of (x, index), then the piece that u falls into, and the token in it. Where a list is too
 //     short (most logits equal), the row is read in its place.
+// Why bins and lists, not a sort: a row is read three times whatever the rule, and nothing but the lists is ever ordered.
 //
-// Bound: for few rows the launches and the chain of steps in each; for many the 64-bit exponentials and LDS atomics of the bins.
+// Bound and measured (one MI355X). Few rows: the launches, 2.6 us each, and the chain of steps in sample_draw (1 x 151936, top-k 50
+// and top-p 0.9: 14.9 us, of these 3.6 + 6.7 + 1.7 for the first three; 13 rows of 32001 with rules of their own 27.6). Many rows:
+// 64 x 151936 with top-p 62 us, 3 x 39 MB read: scan 9.0 us (4.3 TB/s), bins 25.8 and border 20.0 (both the 64-bit exponentials, about
+// 35 vector operations a token, and their prologue of dependent loads), draw 10.6.
 #include <algorithm>
 #include <mutex>
 
@@ -152,7 +156,8 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int
     r.furthest = how.min_p > 0.0f ? fmax(-log2((double)how.min_p), 0.0) : INFINITY;
     r.k = how.top_k > 0 && how.top_k < a.n ? how.top_k : 0;
     r.p = how.top_p < 1.0f ? fmax((double)how.top_p, 0.0) : 1.0;  // (NaN: all)
-    // (a bound of the k-th largest needs k groups; a quarter more leaves it some choice)
+    // (a bound of the k-th largest needs k groups; a quarter more leaves it some choice. By list and by bins, 151936 logits, top-k
+    // with top-p: 50 14.7 and 24.1 us, 600 22.7 and 24.5, 1000 25.1 and 24.7, in 64 rows 50 26.8 and 58.9, 1000 40.3 and 61.5)
     const bool few = r.k && r.k <= FEW && (a.n <= LIST || a.n / GROUP >= r.k + r.k / 4);
     r.mode = !(how.temperature > 0.0f) || top == -INFINITY ? GREEDY : few ? SMALL : r.k || r.p < 1.0 ? BINNED : WHOLE;
     // How far the bins reach, in x: to the least value, or where weights end. Top-p alone: tokens beyond log2(n / (1 - p)) + 1
@@ -374,7 +379,8 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
     } lds;
     __shared__ unsigned listed, first;
     const int number = blockIdx.x / parts, part = blockIdx.x % parts;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (THREADS / 64) + (threadIdx.x >> 6)), waves = parts * (THREADS / 64);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (THREADS / 64) + (threadIdx.x >> 6));
+    const int waves = parts * (THREADS / 64);
     Row &row = rows.row(number);
     const float *x = a.logits + (size_t)number * a.ld;
     // (on their way while the rule is made)
@@ -496,7 +502,8 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(Sam
     __shared__ uint2 list[LIST];
     __shared__ float queues[THREADS / 64][PIECE];
     const int number = blockIdx.x / parts, part = blockIdx.x % parts;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (THREADS / 64) + (threadIdx.x >> 6)), waves = parts * (THREADS / 64);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(part * (THREADS / 64) + (threadIdx.x >> 6));
+    const int waves = parts * (THREADS / 64);
     Row &row = rows.row(number);
     if (row.rule.mode != BINNED) return;
     const float *x = a.logits + (size_t)number * a.ld;
@@ -518,7 +525,8 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(Sam
         c.each([&](float v, int i) {
             const int bin = r.bin(v);
             const unsigned long long in_front = __ballot(bin < b.lo);
-            if (bin < b.lo) queue[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(in_front >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in_front, 0))] = v;
+            const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(in_front >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in_front, 0));
+            if (bin < b.lo) queue[queued + before] = v;
             queued += __popcll(in_front);
             if (bin >= b.lo && (bin <= b.hi || bin == b.k_bin)) {
                 const unsigned to = atomicAdd(&listed, 1u);
@@ -646,6 +654,9 @@ __device__ __forceinline__ void drawn(const SampleArgs &a, int number, u64 targe
 }
 
 // Listed tokens in order, by bins of their bits: a token's place is its bin's beginning and those in front of it in the bin.
+// CROWD: tokens of a cell from which on it is done by digits (last_place) instead. By cells and by digits: top-p alone, 1 row 26.7 and
+// 34.9 us, 64 rows 62.2 and 68.3; logits of 16 bits, whose border's cell holds hundreds of equal ones: with this limit 33.1 and 73.2,
+// with a limit of 1024 41.2 and 86.7, always by digits 36.7 and 72.5.
 constexpr int CELLS = 2048, PER_CELL = CELLS / DRAW, CROWD = 64;
 struct Ordered {
     unsigned begin[CELLS + 1];  // the cells' first tokens
@@ -732,9 +743,8 @@ __device__ __forceinline__ bool order(Ordered &o, Token (&t)[HELD]) {
 }
 
 // A row whose small top-k has left few tokens: every token is compared with every other, by LANES lanes, first for its place in
-// the order, then for its place among the kept ones' ids. Three barriers instead of the fifteen of the general way (1 x 151936,
-// top-k 10, 50 and 100 with top-p: 13.9, 14.9 and 16.7 us, else 18.4, 19.7 and 20.2; up to 256 tokens with 4 lanes each: top-k 190
-// 20.4 to 21.1, else 19.7).
+// the order, then for its place among the kept ones' ids. Few barriers (1 x 151936, top-k 10, 50 and 100 with top-p: 13.9,
+// 14.9 and 16.7 us, by order() 18.4, 19.7 and 20.2; up to 256 tokens with 4 lanes each: top-k 190 20.4 to 21.1, by order() 19.7).
 constexpr int LANES = 8, PAIRS = DRAW / LANES;
 struct Few {
     ulonglong2 token[PAIRS];  // (place, weight), then (id, kept weight)
@@ -966,7 +976,8 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
 
 template <bool VEC> void launch(const SampleArgs &a, const Rows &rows, int n, hipStream_t st) {
     const dim3 block(THREADS);
-    // workgroups of a row: four for each CU in all, a piece for each wave at least
+    // workgroups of a row: four for each CU in all, a piece for each wave at least (64 x 151936 with top-p 62.2 us, two for each CU
+    // 69.3; more cost their prologues, and the bins' atomics: sample_bins 25 us, with six 28, with eight 31)
     const int pieces = (a.n + PIECE - 1) / PIECE, parts = std::max(1, std::min((pieces + 3) / 4, 1024 / n));
     hipLaunchKernelGGL((sample_scan<VEC>), dim3(n * rows.chunks), block, 0, st, a, rows);
     hipLaunchKernelGGL((sample_bins<VEC>), dim3(n * parts), block, 0, st, a, rows, parts);
@@ -994,6 +1005,7 @@ int launch_sample(const SampleArgs &a, int n, hipStream_t st) {
         x.ids += first;
         if (x.prob) x.prob += first;
         const int here = std::min(n - first, MOST_ROWS);
+        // (four logits to a load where all rows allow it: 64 x 151936 62.2 us, one at a time 64.0)
         if (((uintptr_t)x.logits & 15) == 0 && a.ld % 4 == 0) launch<true>(x, rows, here, st);
         else launch<false>(x, rows, here, st);
     }
