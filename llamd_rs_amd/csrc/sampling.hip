@@ -28,6 +28,7 @@
 // 35 vector operations a token, and their prologue of dependent loads), draw 10.6.
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "common.hpp"
 #include "launch.hpp"
@@ -59,7 +60,8 @@ struct Border {
     u64 k_weight, weight;  // weight of the tokens in front of lo
     u64 total;             // of all; with k_bin >= 0, of the tokens up to its end
 };
-__device__ __forceinline__ float value(float x) { return x == x ? x + 0.0f : -INFINITY; }  // (-0 is 0)
+// NaN as -infinity (the greater of a NaN and a number is the number).
+__device__ __forceinline__ float value(float x) { return fmaxf(x, -INFINITY); }
 
 // A number's bits so that they rise with it, and back.
 __device__ __forceinline__ uint32_t rising(float x) {
@@ -68,8 +70,15 @@ __device__ __forceinline__ uint32_t rising(float x) {
 }
 __device__ __forceinline__ float of_rising(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r ^ 0x80000000u : ~r); }
 
-// Position in the order: x falling, then index rising.
-__device__ __forceinline__ u64 place(float x, uint32_t i) { return (u64)~rising(x) << 32 | i; }
+// Position in the order: x falling, then index rising. (-0 is 0.)
+__device__ __forceinline__ u64 place(float x, uint32_t i) { return (u64)~rising(x + 0.0f) << 32 | i; }
+
+// s g + c. (Left to the compiler, c is copied first, one move for each of the polynomial's steps: 64 rows 59.8 us.)
+__device__ __forceinline__ double step(double s, double g, double c) {
+    double x;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(x) : "v"(s), "v"(g), "s"(c));
+    return x;
+}
 
 // A row's rule.
 struct Rule {
@@ -80,33 +89,44 @@ struct Rule {
     int k;              // 0: all
     Mode mode;
 
-    // distance from the maximum in powers of two
-    __device__ __forceinline__ double distance(float x) const { return (double)x == m ? 0.0 : (m - (double)x) * c; }
-    // 2^-y as a multiple of 2^-43; 0 for NaN (an infinite temperature, and a token ruled out)
+    bool infinite;      // the maximum is
+
+    // Distance from the maximum in powers of two. INF: `infinite`, where only the maximum's equals are not infinitely far.
+    template <bool INF> __device__ __forceinline__ double distance_as(float x) const {
+        return INF ? (x == INFINITY ? 0.0 : INFINITY) : (m - (double)x) * c;
+    }
+    __device__ __forceinline__ double distance(float x) const { return infinite ? distance_as<true>(x) : distance_as<false>(x); }
+    // 2^-y as a multiple of 2^-43, to the nearest; 0 for NaN (an infinite temperature, and a token ruled out)
     static __device__ __forceinline__ u64 weight(double y) {
-        if (!(y < RANGE)) return 0;
-        const double r = rint(y), f = (r - y) * 0.69314718055994530942;  // |f| <= ln(2) / 2
-        // e^f by its series: the next term is below 2^-46
-        double s = 1.0 / 39916800.0;
-        s = fma(s, f, 1.0 / 3628800.0);
-        s = fma(s, f, 1.0 / 362880.0);
-        s = fma(s, f, 1.0 / 40320.0);
-        s = fma(s, f, 1.0 / 5040.0);
-        s = fma(s, f, 1.0 / 720.0);
-        s = fma(s, f, 1.0 / 120.0);
-        s = fma(s, f, 1.0 / 24.0);
-        s = fma(s, f, 1.0 / 6.0);
-        s = fma(s, f, 0.5);
-        s = fma(s, f, 1.0);
-        s = fma(s, f, 1.0);
-        // times 2^(43 - r), rounded to a whole number in the last places of 2^52
-        const double w = __longlong_as_double(__double_as_longlong(s) + ((long long)(43 - (int)r) << 52)) + 4503599627370496.0;
+        y = fmin(y, 64.0);
+        constexpr double ROUND = 0x1.8p52;  // what is added to it is rounded to a whole number, which its low word then holds
+        const double whole = ROUND - y, g = (whole - ROUND) + y;  // -rint(y); |g| <= 1/2
+        // 2^(43 - g): the polynomial through 2^-g at the 11 Chebyshev points of [-1/2, 1/2], off by 2^-51 of it at most
+        double s = step(0x1p43 * 0x1.e6063f7217bc6p-28, g, 0x1p43 * -0x1.b675bca4eeebbp-24);
+        s = step(s, g, 0x1p43 * 0x1.62bfd47773353p-20);
+        s = step(s, g, 0x1p43 * -0x1.ffcb54062e698p-17);
+        s = step(s, g, 0x1p43 * 0x1.430913096fd9fp-13);
+        s = step(s, g, 0x1p43 * -0x1.5d87fe9d7a584p-10);
+        s = step(s, g, 0x1p43 * 0x1.3b2ab6fba1ddap-7);
+        s = step(s, g, 0x1p43 * -0x1.c6b08d703ce49p-5);
+        s = step(s, g, 0x1p43 * 0x1.ebfbdff82c598p-3);
+        s = step(s, g, 0x1p43 * -0x1.62e42fefa3a19p-1);
+        s = step(s, g, 0x1p43);
+        // times 2^-rint(y), rounded to a whole number in the last places of 2^52
+        const int exponent = __double2hiint(s) + (int)((unsigned)__double2loint(whole) << 20);
+        const double w = __hiloint2double(exponent, __double2loint(s)) + 0x1p52;
         return (u64)__double_as_longlong(w) & 0xFFFFFFFFFFFFFull;
     }
     __device__ __forceinline__ bool likely(double y) const { return y <= furthest; }
     // Rises as x falls; BINS and more: behind the bins. (Halves: the difference of any two numbers is finite.)
-    __device__ __forceinline__ int bin(float x) const {
-        return 2.0f * half == x ? 0 : (int)fminf((half - 0.5f * x) * scale, (float)BINS);
+    template <bool INF> __device__ __forceinline__ int bin_as(float x) const {
+        return INF ? (x == INFINITY ? 0 : BINS) : (int)fminf((half - 0.5f * x) * scale, (float)BINS);
+    }
+    __device__ __forceinline__ int bin(float x) const { return infinite ? bin_as<true>(x) : bin_as<false>(x); }
+    // f<infinite>()
+    template <class F> __device__ __forceinline__ void by_kind(F f) const {
+        if (__builtin_amdgcn_readfirstlane(infinite)) f(std::true_type{});
+        else f(std::false_type{});
     }
 };
 
@@ -152,6 +172,7 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int
     }
     Rule r;
     r.m = top;
+    r.infinite = top == INFINITY;
     r.c = 1.4426950408889634074 / (double)how.temperature;
     r.furthest = how.min_p > 0.0f ? fmax(-log2((double)how.min_p), 0.0) : INFINITY;
     r.k = how.top_k > 0 && how.top_k < a.n ? how.top_k : 0;
@@ -193,6 +214,11 @@ template <bool VEC, int T, int EACH> struct Values {
     template <class F> __device__ __forceinline__ void each(F f) const {
 #pragma unroll
         for (int j = 0; j < EACH; ++j) f(value(v[j]), index(j));
+    }
+    // The same where NaN may be NaN: it has no weight, and lies behind the bins.
+    template <class F> __device__ __forceinline__ void each_raw(F f) const {
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) f(v[j], index(j));
     }
 };
 
@@ -396,9 +422,11 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
     if (r.mode == WHOLE) {
         each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int piece) {
             u64 sum = 0;
-            c.each([&](float v, int) {
-                const double y = r.distance(v);
-                if (r.likely(y)) sum += r.weight(y);
+            r.by_kind([&](auto inf) {
+                c.each_raw([&](float v, int) {
+                    const double y = r.template distance_as<inf>(v);
+                    sum += r.likely(y) ? r.weight(y) : 0;
+                });
             });
             sum = last_lane(wave_scan(sum));
             if (lane == 0) row.sum[piece] = sum;
@@ -429,15 +457,17 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
     __syncthreads();
     u64 far = 0;
     each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int) {
-        c.each([&](float v, int) {
-            const u64 w = r.weight(r.distance(v));
-            const int b = r.bin(v);
-            if (b >= BINS) {
-                far += w;
-            } else if (w) {
-                if (r.k) atomicAdd(&lds.bins.count[b], 1u);
-                atomicAdd(&lds.bins.weight[b], w);
-            }
+        r.by_kind([&](auto inf) {
+            c.each_raw([&](float v, int) {
+                const u64 w = r.weight(r.template distance_as<inf>(v));
+                const int b = r.template bin_as<inf>(v);
+                if (b >= BINS) {
+                    far += w;
+                } else if (w) {
+                    if (r.k) atomicAdd(&lds.bins.count[b], 1u);
+                    atomicAdd(&lds.bins.weight[b], w);
+                }
+            });
         });
     });
     far = last_lane(wave_scan(far));
@@ -522,16 +552,18 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_border(Sam
     each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int piece) {
         // the values in front of the border, close together: few of a wave's 64 are, and their weights are what costs
         int queued = 0;
-        c.each([&](float v, int i) {
-            const int bin = r.bin(v);
-            const unsigned long long in_front = __ballot(bin < b.lo);
-            const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(in_front >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in_front, 0));
-            if (bin < b.lo) queue[queued + before] = v;
-            queued += __popcll(in_front);
-            if (bin >= b.lo && (bin <= b.hi || bin == b.k_bin)) {
-                const unsigned to = atomicAdd(&listed, 1u);
-                if (to < LIST) list[to] = make_uint2(i, __float_as_uint(v));
-            }
+        r.by_kind([&](auto inf) {
+            c.each_raw([&](float v, int i) {
+                const int bin = r.template bin_as<inf>(v);
+                const unsigned long long in_front = __ballot(bin < b.lo);
+                const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(in_front >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in_front, 0));
+                if (bin < b.lo) queue[queued + before] = v;
+                queued += __popcll(in_front);
+                if (bin >= b.lo && (bin <= b.hi || bin == b.k_bin)) {
+                    const unsigned to = atomicAdd(&listed, 1u);
+                    if (to < LIST) list[to] = make_uint2(i, __float_as_uint(v));
+                }
+            });
         });
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         u64 sum = 0;
