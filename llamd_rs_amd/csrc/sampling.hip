@@ -130,6 +130,14 @@ struct Rule {
     }
 };
 
+// A row's rule as far as it does not depend on the logits (sample_scan finds it while they are on their way; by every workgroup
+// of sample_bins, the logarithms and divisions are a part of its vector instructions).
+struct Wanted {
+    double c, furthest, p, reach;  // reach: of the bins, in x
+    int k;
+    Mode mode;
+};
+
 // A row's scratch; behind it the maxima of its groups of 64 values.
 struct alignas(16) Row {
     u64 weight[BINS];
@@ -140,6 +148,7 @@ struct alignas(16) Row {
     unsigned listed;
     int best;              // the maximum's first index
     Rule rule;
+    Wanted wanted;
     Extremes chunk[MOST_CHUNKS];
     uint2 list[LIST];      // (index, x's bits), in any order
 };
@@ -151,12 +160,31 @@ struct Rows {
     __device__ __forceinline__ float *maxima(int i) const { return (float *)(base + (size_t)i * step + sizeof(Row)); }
 };
 
+// What a row's rule is before its logits are seen.
+__device__ __forceinline__ Wanted wanted_of(const SampleArgs &a, int number) {
+    const SampleRule how = a.how[number];
+    Wanted r;
+    r.c = 1.4426950408889634074 / (double)how.temperature;
+    r.furthest = how.min_p > 0.0f ? fmax(-log2((double)how.min_p), 0.0) : INFINITY;
+    r.k = how.top_k > 0 && how.top_k < a.n ? how.top_k : 0;
+    r.p = how.top_p < 1.0f ? fmax((double)how.top_p, 0.0) : 1.0;  // (NaN: all)
+    // (a bound of the k-th largest needs k groups; a quarter more leaves it some choice. By list and by bins, 151936 logits, top-k
+    // with top-p: 50 14.7 and 24.1 us, 600 22.7 and 24.5, 1000 25.1 and 24.7, in 64 rows 50 26.8 and 58.9, 1000 40.3 and 61.5)
+    const bool few = r.k && r.k <= FEW && (a.n <= LIST || a.n / GROUP >= r.k + r.k / 4);
+    r.mode = !(how.temperature > 0.0f) ? GREEDY : few ? SMALL : r.k || r.p < 1.0 ? BINNED : WHOLE;
+    // How far the bins reach, in x: to the least value, or where weights end. Top-p alone: tokens beyond log2(n / (1 - p)) + 1
+    // sum to less than half of (1 - p) S, S >= 1, and are not needed to reach p S.
+    const double reach = r.k || r.p == 1.0 ? RANGE : fmin(RANGE, log2(a.n / (1.0 - r.p)) + 1.0);
+    r.reach = reach / r.c;
+    return r;
+}
+
 // The rule of a row from its chunks' extremes; `at`: the maximum's first index.
-__device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int number, int chunks, int &at) {
+__device__ __forceinline__ Rule rule_of(const Row &row, int chunks, int &at) {
     constexpr int W = 4;  // waves that have chunks
     __shared__ float tops[W], leasts[W];
     __shared__ int places[W];
-    const SampleRule how = a.how[number];
+    const Wanted wanted = row.wanted;
     Extremes x = {-INFINITY, INFINITY, 0x7FFFFFFF, 0};
     if ((int)threadIdx.x < chunks) x = row.chunk[threadIdx.x];
     wave_argmax(x.top, x.at, -INFINITY);
@@ -173,18 +201,12 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs &a, const Row &row, int
     Rule r;
     r.m = top;
     r.infinite = top == INFINITY;
-    r.c = 1.4426950408889634074 / (double)how.temperature;
-    r.furthest = how.min_p > 0.0f ? fmax(-log2((double)how.min_p), 0.0) : INFINITY;
-    r.k = how.top_k > 0 && how.top_k < a.n ? how.top_k : 0;
-    r.p = how.top_p < 1.0f ? fmax((double)how.top_p, 0.0) : 1.0;  // (NaN: all)
-    // (a bound of the k-th largest needs k groups; a quarter more leaves it some choice. By list and by bins, 151936 logits, top-k
-    // with top-p: 50 14.7 and 24.1 us, 600 22.7 and 24.5, 1000 25.1 and 24.7, in 64 rows 50 26.8 and 58.9, 1000 40.3 and 61.5)
-    const bool few = r.k && r.k <= FEW && (a.n <= LIST || a.n / GROUP >= r.k + r.k / 4);
-    r.mode = !(how.temperature > 0.0f) || top == -INFINITY ? GREEDY : few ? SMALL : r.k || r.p < 1.0 ? BINNED : WHOLE;
-    // How far the bins reach, in x: to the least value, or where weights end. Top-p alone: tokens beyond log2(n / (1 - p)) + 1
-    // sum to less than half of (1 - p) S, S >= 1, and are not needed to reach p S.
-    const double reach = r.k || r.p == 1.0 ? RANGE : fmin(RANGE, log2(a.n / (1.0 - r.p)) + 1.0);
-    const double range = fmin(r.m - (double)least, reach / r.c);
+    r.c = wanted.c;
+    r.furthest = wanted.furthest;
+    r.k = wanted.k;
+    r.p = wanted.p;
+    r.mode = top == -INFINITY ? GREEDY : wanted.mode;
+    const double range = fmin(r.m - (double)least, wanted.reach);
     r.half = 0.5f * top;
     r.scale = range > 0.0 ? (float)fmin((2.0 * BINS - 1.0) / range, 3e38) : 0.0f;
     return r;
@@ -278,9 +300,10 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_scan(Sampl
     int at = 0x7FFFFFFF;
     Values<VEC, THREADS, EACH> c;
     c.load(a.logits + (size_t)number * a.ld, a.n, chunk * CHUNK);
-    c.each([&](float v, int i) {
-        argmax_step(top, at, v, i);
-        if (v > -INFINITY) least = fminf(least, v);
+    if (chunk == 0 && threadIdx.x == 0) row.wanted = wanted_of(a, number);
+    c.each_raw([&](float v, int i) {  // (a thread's indices rise)
+        if (v > top) top = v, at = i;
+        least = fminf(least, v > -INFINITY ? v : INFINITY);
     });
     // what the next launches add to
     for (int i = chunk * THREADS + threadIdx.x; i < BINS; i += rows.chunks * THREADS) row.count[i] = 0, row.weight[i] = 0;
@@ -416,7 +439,7 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
     const int k = a.how[number].top_k;
     if (k > 0 && k <= FEW) maxima.load(rows.maxima(number), rows.chunks * GROUPS);
     int at;
-    const Rule r = rule_of(a, row, number, rows.chunks, at);
+    const Rule r = rule_of(row, rows.chunks, at);
     if (part == 0 && threadIdx.x == 0) row.rule = r, row.best = at;
     if (r.mode == GREEDY) return;
     if (r.mode == WHOLE) {
