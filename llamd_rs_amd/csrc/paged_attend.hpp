@@ -21,9 +21,9 @@
 // TFLOP/s of the causal half, where a library product of 8192^3 reaches 1349); f32 110 to 119 of 154. Pieces and packed
 // prompts: the steps of a CU's tiles, 1.1 us each, and 8 us to every workgroup's first product (512 tokens after 7000 81 us,
 // 9 prompts of 192 to 700 tokens 41). Decode: memory, then the chain length -> table -> keys and the second launch (1 x 4100
-// 12.8 us, 13 x 1000 in f32 20.4, 48 behind 4100 shared 25.8). 8-bit pages: 8192 tokens 575 us (956 TFLOP/s), 512 after
-// 7000 84, 9 packed prompts 40.6; decode 1 x 4100 12.3, 61 x 500 to 2000 (79 MB) 28.3, of these 23 at 3.4 TB/s and the join 5.4,
-// 48 behind 4100 shared 25.4.
+// 12.8 us, 13 x 1000 in f32 20.4, 48 behind 4100 shared 25.8). 8-bit pages: 8192 tokens 562 to 594 us (925 to 978 TFLOP/s), 512
+// after 7000 83 to 86, 9 packed prompts 40.3; decode 1 x 4100 12.3, 61 x 500 to 2000 (79 MB) 28.3, of these 23 at 3.4 TB/s and
+// the join 5.4, 48 behind 4100 shared 25.4.
 #pragma once
 
 #include <algorithm>
@@ -641,7 +641,8 @@ __device__ __forceinline__ void few_rows(const PagedAttendArgs &a, const Split &
     load_few<E, HD>(q, a.q, r.at);
     S st;
     st.clear();
-    attend_few<E, HD, few_step<E>>(p, pages_of<E, HD>(p, t.seq, kvh), t.n_kv, r.limit, begin + few_positions<E> * wave, end, q, a.scale, st);
+    attend_few<E, HD, few_step<E>>(p, pages_of<E, HD>(p, t.seq, kvh), t.n_kv, r.limit, begin + few_positions<E> * wave, end, q,
+                                   a.scale, st);
 
     // the four waves' positions together: every wave adds a quarter of the dimensions
     const float mine = add_groups(st.l);

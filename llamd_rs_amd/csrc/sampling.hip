@@ -23,9 +23,9 @@
 // Why bins and lists, not a sort: a row is read three times whatever the rule, and nothing but the lists is ever ordered.
 //
 // Bound and measured (one MI355X). Few rows: the launches, 2.6 us each, and the chain of steps in sample_draw (1 x 151936, top-k 50
-// and top-p 0.9: 14.9 us, of these 3.6 + 6.7 + 1.7 for the first three; 13 rows of 32001 with rules of their own 27.6). Many rows:
-// 64 x 151936 with top-p 62 us, 3 x 39 MB read: scan 9.0 us (4.3 TB/s), bins 25.8 and border 20.0 (both the 64-bit exponentials, about
-// 35 vector operations a token, and their prologue of dependent loads), draw 10.6.
+// and top-p 0.9: 14.6 us, of these 3.2 + 6.5 + 1.7 for the first three; 13 rows of 32001 with rules of their own 25 to 28). Many
+// rows: 64 x 151936 with top-p 56 us, 3 x 39 MB read: scan 8.4 us (4.7 TB/s, a large copy's rate), bins 20.7 (40 vector instructions
+// a logit, most of them of the 64-bit exponential; vector units busy 59%), border 18.5 (30, 52%), draw 10.9.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -73,7 +73,8 @@ __device__ __forceinline__ float of_rising(uint32_t r) { return __uint_as_float(
 // Position in the order: x falling, then index rising. (-0 is 0.)
 __device__ __forceinline__ u64 place(float x, uint32_t i) { return (u64)~rising(x + 0.0f) << 32 | i; }
 
-// s g + c. (Left to the compiler, c is copied first, one move for each of the polynomial's steps: 64 rows 59.8 us.)
+// s g + c. (Left to the compiler, c is copied first, one move for each of the polynomial's steps: 64 x 151936 with top-p
+// 59.8 us, so 56.6.)
 __device__ __forceinline__ double step(double s, double g, double c) {
     double x;
     asm("v_fma_f64 %0, %1, %2, %3" : "=v"(x) : "v"(s), "v"(g), "s"(c));
@@ -169,7 +170,7 @@ __device__ __forceinline__ Wanted wanted_of(const SampleArgs &a, int number) {
     r.k = how.top_k > 0 && how.top_k < a.n ? how.top_k : 0;
     r.p = how.top_p < 1.0f ? fmax((double)how.top_p, 0.0) : 1.0;  // (NaN: all)
     // (a bound of the k-th largest needs k groups; a quarter more leaves it some choice. By list and by bins, 151936 logits, top-k
-    // with top-p: 50 14.7 and 24.1 us, 600 22.7 and 24.5, 1000 25.1 and 24.7, in 64 rows 50 26.8 and 58.9, 1000 40.3 and 61.5)
+    // with top-p: 50 14.6 and 23.5 us, 600 22.4 and 24.0, 1000 24.5 and 23.8, in 64 rows 50 26.0 and 55.3, 1000 38.6 and 56.9)
     const bool few = r.k && r.k <= FEW && (a.n <= LIST || a.n / GROUP >= r.k + r.k / 4);
     r.mode = !(how.temperature > 0.0f) ? GREEDY : few ? SMALL : r.k || r.p < 1.0 ? BINNED : WHOLE;
     // How far the bins reach, in x: to the least value, or where weights end. Top-p alone: tokens beyond log2(n / (1 - p)) + 1
@@ -709,9 +710,9 @@ __device__ __forceinline__ void drawn(const SampleArgs &a, int number, u64 targe
 }
 
 // Listed tokens in order, by bins of their bits: a token's place is its bin's beginning and those in front of it in the bin.
-// CROWD: tokens of a cell from which on it is done by digits (last_place) instead. By cells and by digits: top-p alone, 1 row 26.7 and
-// 34.9 us, 64 rows 62.2 and 68.3; logits of 16 bits, whose border's cell holds hundreds of equal ones: with this limit 33.1 and 73.2,
-// with a limit of 1024 41.2 and 86.7, always by digits 36.7 and 72.5.
+// CROWD: tokens of a cell from which on it is done by digits (last_place) instead. By cells and by digits: top-p alone, 1 row 25.3 and
+// 27.1 us, 64 rows 55.8 and 61.2, top-k 1000 24.5 and 45.0; 64 rows of 16-bit logits, whose border's cell holds hundreds of equal
+// ones: with this limit 66.7, with a limit of 1024 78.4, always by digits 66.9.
 constexpr int CELLS = 2048, PER_CELL = CELLS / DRAW, CROWD = 64;
 struct Ordered {
     unsigned begin[CELLS + 1];  // the cells' first tokens
@@ -798,8 +799,9 @@ __device__ __forceinline__ bool order(Ordered &o, Token (&t)[HELD]) {
 }
 
 // A row whose small top-k has left few tokens: every token is compared with every other, by LANES lanes, first for its place in
-// the order, then for its place among the kept ones' ids. Few barriers (1 x 151936, top-k 10, 50 and 100 with top-p: 13.9,
-// 14.9 and 16.7 us, by order() 18.4, 19.7 and 20.2; up to 256 tokens with 4 lanes each: top-k 190 20.4 to 21.1, by order() 19.7).
+// the order, then for its place among the kept ones' ids. Few barriers (1 x 151936, top-k 10, 50 and 100 with top-p: 13.2,
+// 14.6 and 18.3 us, by order() 18.5, 19.6 and 19.7; 64 rows of 50 26.0 and 31.3; up to 256 tokens with 4 lanes each: top-k 190 20.4 to
+// 21.1, by order() 19.7).
 constexpr int LANES = 8, PAIRS = DRAW / LANES;
 struct Few {
     ulonglong2 token[PAIRS];  // (place, weight), then (id, kept weight)
@@ -1031,8 +1033,8 @@ template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleAr
 
 template <bool VEC> void launch(const SampleArgs &a, const Rows &rows, int n, hipStream_t st) {
     const dim3 block(THREADS);
-    // workgroups of a row: four for each CU in all, a piece for each wave at least (64 x 151936 with top-p 62.2 us, two for each CU
-    // 69.3; more cost their prologues, and the bins' atomics: sample_bins 25 us, with six 28, with eight 31)
+    // workgroups of a row: four for each CU in all, a piece for each wave at least (64 x 151936 with top-p 55.8 us, two for each CU
+    // 60.0, three 56.8, five 57.1)
     const int pieces = (a.n + PIECE - 1) / PIECE, parts = std::max(1, std::min((pieces + 3) / 4, 1024 / n));
     hipLaunchKernelGGL((sample_scan<VEC>), dim3(n * rows.chunks), block, 0, st, a, rows);
     hipLaunchKernelGGL((sample_bins<VEC>), dim3(n * parts), block, 0, st, a, rows, parts);
@@ -1060,7 +1062,8 @@ int launch_sample(const SampleArgs &a, int n, hipStream_t st) {
         x.ids += first;
         if (x.prob) x.prob += first;
         const int here = std::min(n - first, MOST_ROWS);
-        // (four logits to a load where all rows allow it: 64 x 151936 62.2 us, one at a time 64.0)
+        // (four logits to a load where all rows allow it: 64 x 151936 with top-p 55.8 us, without a border 28.7, one at a time 57.2 and
+        // 30.8)
         if (((uintptr_t)x.logits & 15) == 0 && a.ld % 4 == 0) launch<true>(x, rows, here, st);
         else launch<false>(x, rows, here, st);
     }
