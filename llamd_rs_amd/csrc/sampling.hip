@@ -341,7 +341,8 @@ struct Maxima {
 };
 
 // A bound that k groups' maxima, and so k tokens, reach: as few more as a short search finds. Four bounds are counted at a
-// time, one by each wave. 0: there are fewer than k.
+// time, one by each wave. 0: there are fewer than k, or more tokens
+// would reach it than a list holds.
 __device__ __forceinline__ uint32_t bound_of(const Maxima &m, float top, int k) {
     __shared__ int counts[4];
     constexpr int HELD = Maxima::HELD;
@@ -404,6 +405,12 @@ __device__ __forceinline__ uint32_t bound_of(const Maxima &m, float top, int k) 
         if (reached) lo = min(was + reached * step, hi);
         if (reached < 4) hi = min(was + (reached + 1) * step, hi);
     }
+    // How many tokens reach it: of `all` groups of tokens that are alike, `best` with one at least, -all log(1 - best / all).
+    // (Up to a sixteenth of the list's length fit even if no group is without one, all log(all) then.)
+    if (best > LIST / 16) {
+        const int all = count_of(none + 1);
+        if (best >= all || all * -log1pf(-(float)best / (float)all) > 0.9f * LIST) return 0;
+    }
     return lo;
 }
 
@@ -440,7 +447,14 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
     const int k = a.how[number].top_k;
     if (k > 0 && k <= FEW) maxima.load(rows.maxima(number), rows.chunks * GROUPS);
     int at;
-    const Rule r = rule_of(row, rows.chunks, at);
+    Rule r = rule_of(row, rows.chunks, at);
+    uint32_t bound = 0;
+    if (r.mode == SMALL && a.n > LIST) {
+        bound = bound_of(maxima, (float)r.m, r.k);
+        // (all workgroups of the row alike; a list that is too short would have sample_draw read the row instead: 16 x 80383, a third
+        // masked, top-k 1000, 38 us, so 276; the estimate costs other rows 0.3 to 0.8)
+        if (!bound) r.mode = BINNED;
+    }
     if (part == 0 && threadIdx.x == 0) row.rule = r, row.best = at;
     if (r.mode == GREEDY) return;
     if (r.mode == WHOLE) {
@@ -459,7 +473,6 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_bins(Sampl
     }
     if (r.mode == SMALL) {
         if (threadIdx.x == 0) listed = 0;
-        const uint32_t bound = a.n <= LIST ? 0 : bound_of(maxima, (float)r.m, r.k);
         const float least = bound ? of_rising(bound) : -INFINITY;
         __syncthreads();
         each_piece<VEC>(c, x, a.n, wave, waves, [&](const Piece<VEC> &c, int) {

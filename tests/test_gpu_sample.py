@@ -138,6 +138,21 @@ def test_flat_and_steep_rows(gpu, spread, temperature):
     check(gpu, x, rules, rng.random(len(rules)))
 
 
+@pytest.mark.parametrize("n,k", [(80_383, 1000), (80_383, 1004), (70_000, 600), (30_000, 374), (151_936, 1024)])
+def test_a_top_k_of_most_groups(gpu, n, k):
+    """The maxima of 64 values bound the k-th largest from far below, or there are fewer than k of them that are finite."""
+    rng = np.random.default_rng(23)
+    x = logits(rng, 6, n)
+    x[1, rng.random(n) < 0.3] = -np.inf
+    x[2, rng.random(n) < 0.97] = -np.inf
+    x[3, :n // 2], x[3, n // 2 + 5000:] = -np.inf, -np.inf   # 5000 in a row, 79 groups
+    x[4, 700:] = -np.inf
+    x[5] = np.round(x[5] * 4) / 4
+    rules = [(1, k, 1, 0), (0.8, k, 0.95, 0), (1.2, k, 1, 0.01), (1, k, 0.9, 0), (1, k, 1, 0), (0.7, k, 0.99, 0)]
+    for turn in range(3):
+        check(gpu, x, rules, rng.random(6), turn)
+
+
 def test_an_outlier_below(gpu):
     """One logit far below the others stretches the bins: most others fall into one."""
     rng = np.random.default_rng(9)
