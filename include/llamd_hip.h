@@ -554,7 +554,7 @@ int llamd_hip_paged8_decode(const llamd_hip_pages8 *c, const llamd_hip_batch *b,
  *   top_p: of these, with S the sum of their w, those whose predecessors sum to
  *     less than top_p * S
  *   min_p: of these, those with w >= min_p
- *   (the first is always kept)
+ *   (the first is always kept, alone if min_p is above 1)
  *   ids: the first id, in rising order, at which the running sum of kept w
  *     exceeds u times the sum of all kept w;  prob (may be NULL): its w / that sum
  *

@@ -166,13 +166,14 @@ __device__ __forceinline__ Wanted wanted_of(const SampleArgs &a, int number) {
     const SampleRule how = a.how[number];
     Wanted r;
     r.c = 1.4426950408889634074 / (double)how.temperature;
-    r.furthest = how.min_p > 0.0f ? fmax(-log2((double)how.min_p), 0.0) : INFINITY;
+    r.furthest = how.min_p > 0.0f ? -log2((double)how.min_p) : INFINITY;  // (negative above 1: GREEDY)
     r.k = how.top_k > 0 && how.top_k < a.n ? how.top_k : 0;
     r.p = how.top_p < 1.0f ? fmax((double)how.top_p, 0.0) : 1.0;  // (NaN: all)
     // (a bound of the k-th largest needs k groups; a quarter more leaves it some choice. By list and by bins, 151936 logits, top-k
     // with top-p: 50 14.6 and 23.5 us, 600 22.4 and 24.0, 1000 24.5 and 23.8, in 64 rows 50 26.0 and 55.3, 1000 38.6 and 56.9)
     const bool few = r.k && r.k <= FEW && (a.n <= LIST || a.n / GROUP >= r.k + r.k / 4);
-    r.mode = !(how.temperature > 0.0f) ? GREEDY : few ? SMALL : r.k || r.p < 1.0 ? BINNED : WHOLE;
+    // (no weight reaches a min-p above 1: the first token alone is kept, not all that are equal to it)
+    r.mode = !(how.temperature > 0.0f) || how.min_p > 1.0f ? GREEDY : few ? SMALL : r.k || r.p < 1.0 ? BINNED : WHOLE;
     // How far the bins reach, in x: to the least value, or where weights end. Top-p alone: tokens beyond log2(n / (1 - p)) + 1
     // sum to less than half of (1 - p) S, S >= 1, and are not needed to reach p S.
     const double reach = r.k || r.p == 1.0 ? RANGE : fmin(RANGE, log2(a.n / (1.0 - r.p)) + 1.0);

@@ -91,6 +91,24 @@ def test_equal_logits(gpu, n):
         check(gpu, np.full((len(rules), n), value, np.float32), rules, [0.3, 0.99, 0.7, 0.5, 0.999, 0.01], value)
 
 
+@pytest.mark.parametrize("least", [float(np.nextafter(np.float32(1), np.float32(2))), 1.5, 2.0, 3e38, np.inf])
+@pytest.mark.parametrize("n", [10, 2048, 2049, 40_000, 151_936])
+def test_a_min_p_that_no_weight_reaches(gpu, n, least):
+    """The first alone is kept, of equal maxima the one of the lowest id, whatever else the rule says."""
+    rng = np.random.default_rng(24)
+    rules = [(1, 0, 1, least), (0.5, 5, 1, least), (1, 0, 0.9, least), (2, n // 2, 0.3, least), (np.inf, 0, 1, least),
+             (1, 5, 1, least), (1, 0, 1, least)]
+    x = logits(rng, len(rules), n)
+    first = rng.integers(1, n // 2, len(rules))
+    for r in range(len(rules)):
+        x[r, first[r]] = x[r, [first[r] + 1, n - 1]] = x[r].max() + 1
+    x[5], first[5] = 0.25, 0
+    x[6, first[6]] = x[6, first[6] + 1] = np.inf
+    for u in (0.0, 0.4, 0.9, 1.0):
+        ids, prob = check(gpu, x, rules, np.full(len(rules), u), u)
+        assert np.array_equal(ids, first) and (prob == 1).all()
+
+
 @pytest.mark.parametrize("values", [(0.0, -0.0, 1.0), (2.0, 2.25, 1.75, -8.0), (5.0, -np.inf, 4.0), (7.0, LOWEST), (1.0, 1 + 2.0 ** -23)])
 @pytest.mark.parametrize("n", [500, 30_000])
 def test_few_values(gpu, values, n):
