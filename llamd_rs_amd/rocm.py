@@ -332,6 +332,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> tuple[n
     """A token per row of logits [n_seq, n] and the probability that it was drawn with (llamd_hip_sample): u uniform
     numbers in [0, 1), one per row; the rule's numbers for all rows or one per row."""
     x = np.atleast_2d(_f32(logits))
+    if x.ndim > 2:
+        raise ValueError("logits must be [n_seq, n]")
     if np.shape(u) not in ((), (len(x),)):
         raise ValueError("u: one number per row")
     rules = sampling_rules(len(x), temperature, top_k, top_p, min_p)
@@ -524,7 +526,7 @@ class LmHead:
         """A drawn token per sequence and its probability (sample), from logits that stay on the device."""
         x = np.atleast_2d(_f32(x))
         nseq = x.shape[0]
-        if x.shape[1] != self.blocks * QK_K or not 0 < nseq <= self.max_seq:
+        if x.ndim > 2 or x.shape[1] != self.blocks * QK_K or not 0 < nseq <= self.max_seq:
             raise ValueError("x must be [1 <= nseq <= max_seq, k]")
         if np.shape(u) not in ((), (nseq,)):
             raise ValueError("u: one number per sequence")

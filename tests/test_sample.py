@@ -42,6 +42,18 @@ def test_rules():
             rocm.sample(x, u)
 
 
+def test_logits_of_more_than_two_axes_are_refused():
+    """(Rows of what they hold would be drawn from: [2, 3, 100] as two rows of three logits.)"""
+    for x in (np.zeros((2, 3, 100)), np.zeros((1, 1, 1, 5))):
+        with pytest.raises(ValueError):
+            rocm.sample(x, 0.5)
+    head = rocm.LmHead.__new__(rocm.LmHead)  # (the check comes before the device)
+    head.rows, head.blocks, head.max_seq, head._h = 100, 1, 8, None
+    for x in (np.zeros((2, 256, 2)), np.zeros((1, 256, 1))):
+        with pytest.raises(ValueError):
+            head.sample(x, 0.5)
+
+
 def test_the_restatement():
     """By hand: weights 1, 1/2, 1/2, 1/4 at ids 2, 0, 3, 1."""
     x = np.log(np.array([0.5, 0.25, 1, 0.5]))
