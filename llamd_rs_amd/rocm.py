@@ -311,6 +311,10 @@ def sampling_rules(n_seq: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
     for name, x in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
         if np.ndim(x) > 1 or (np.ndim(x) == 1 and len(x) != n_seq):
             raise ValueError(f"{name}: one number, or one per sequence")
+        if name == "top_k":
+            k = np.asarray(x, np.float64)
+            if not ((k == np.rint(k)) & (np.abs(k + 0.5) < 2.0 ** 31)).all():
+                raise ValueError("top_k: whole numbers of 32 bits")
         r[name] = x
     return r
 

@@ -54,6 +54,21 @@ def test_logits_of_more_than_two_axes_are_refused():
             head.sample(x, 0.5)
 
 
+@pytest.mark.parametrize("top_k", [2.5, np.nan, np.inf, 1 << 31, -(1 << 31) - 1, [1, 2, (1 << 32) + 5], np.array([1, 2, 1 << 40]),
+                                   np.array([0.5, 1, 2]), 1 << 70])
+def test_a_top_k_that_is_no_whole_number_of_32_bits(top_k):
+    """(Wrapped or cut short it would be another rule: 2^32 + 5 the first five.)"""
+    with pytest.raises(ValueError):
+        rocm.sampling_rules(3, top_k=top_k)
+
+
+def test_a_top_k_of_any_number_type():
+    for top_k in (7, 7.0, np.float32(7), np.uint64(7), [7, 7.0, np.int8(7)]):
+        assert rocm.sampling_rules(3, top_k=top_k)["top_k"].tolist() == [7, 7, 7]
+    for top_k in ((1 << 31) - 1, -(1 << 31)):
+        assert rocm.sampling_rules(3, top_k=top_k)["top_k"].tolist() == [top_k] * 3
+
+
 def test_the_restatement():
     """By hand: weights 1, 1/2, 1/2, 1/4 at ids 2, 0, 3, 1."""
     x = np.log(np.array([0.5, 0.25, 1, 0.5]))
