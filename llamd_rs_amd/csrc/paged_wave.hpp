@@ -139,6 +139,27 @@ template <class E> __device__ __forceinline__ run4 to_run(const float *x) {
 // 2^LAZY, and O is rescaled only where a row's maximum climbs further, which after the first few tiles it hardly does.
 constexpr float LAZY = 8.0f;
 
+// A weight's exponent is one multiply-add, rounded once: for a row's largest score it is off from 0 by what the maximum was rounded
+// by. That is a factor of all the row's weights and goes out with their sum, but from a maximum of 2^26 on it is 2^2 and more: with
+// LAZY's 2^8 f16 weights overflow, and from 2^31 on the exponential does. There the maximum is taken off first, and the multiply-add
+// has nothing to take off. Which rows those are changes with the maximum only (kept; asked for again in every step, 8192 tokens of
+// bf16 take 2% longer, this way less than the 1% between runs).
+constexpr float FAR_SCORE = 0x1p26f;
+__device__ __forceinline__ unsigned long long far_rows(float m) {
+    return __ballot(__builtin_fabsf(m) >= FAR_SCORE && m != NEG_INF);
+}
+__device__ __forceinline__ float subtrahend(float m) { return __builtin_fabsf(m) < FAR_SCORE ? m : 0.0f; }
+// N vectors of L scores
+template <int L, int N, class V> __device__ __forceinline__ void take_off(V (&s)[N], float scale, float m, unsigned long long far) {
+    if (!far) return;
+    const bool mine = far >> (threadIdx.x & 63) & 1;
+    const float back = 1.0f / scale;
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int i = 0; i < L; ++i) s[b][i] = mine ? (s[b][i] * scale - m) * back : s[b][i];
+}
+
 // 32 rows' running softmax and O, over tiles of 32 * SUB positions.
 template <class E, int HD> struct RowState {
     static constexpr int DB = HD / 32;             // blocks of 32 dimensions
@@ -146,6 +167,7 @@ template <class E, int HD> struct RowState {
     static constexpr int PS = 32 / (2 * E::RUN);   // steps of the second, per 32 positions
     v16f o[DB];
     float m, l;  // what x is taken against, and this half's part of the sum
+    unsigned long long far;
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -154,6 +176,7 @@ template <class E, int HD> struct RowState {
             for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
         m = NEG_INF;
         l = 0.0f;
+        far = 0;
     }
 
     // The running maximum brought up to date with scores, and O and l with it.
@@ -167,6 +190,7 @@ template <class E, int HD> struct RowState {
         if (__any(top > m + LAZY)) {
             const float m1 = fmaxf(m, top), shrink = exp2_fast(m - against(m1));
             m = m1;
+            far = far_rows(m1);
             l *= shrink;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
@@ -177,7 +201,8 @@ template <class E, int HD> struct RowState {
 
     // Scores (kv_reg's order) to weights, which add to l.
     template <int SUB> __device__ __forceinline__ void weigh(v16f (&s)[SUB], float scale) {
-        const float ref = against(m);
+        take_off<16>(s, scale, m, far);
+        const float ref = subtrahend(m);
         float sum = 0.0f;
 #pragma unroll
         for (int b = 0; b < SUB; ++b)
@@ -252,12 +277,14 @@ template <class E, int HD> struct FewState {
     static constexpr int PS = 32 / (4 * E::RUN);  // steps of the second
     v4f o[DB];   // dimension 16 d + 4 group + i
     float m, l;  // what x is taken against, and this lane's part of the sum
+    unsigned long long far;
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         m = NEG_INF;
         l = 0.0f;
+        far = 0;
     }
 
     // (of 8-bit pages `scale` is the lane's: its positions' unit is in it)
@@ -271,11 +298,13 @@ template <class E, int HD> struct FewState {
         if (__any(top > m + LAZY)) {
             const float m1 = fmaxf(m, top), shrink = exp2_fast(m - against(m1));
             m = m1;
+            far = far_rows(m1);
             l *= shrink;
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= shrink;
         }
-        const float ref = against(m);
+        take_off<4>(s, scale, m, far);
+        const float ref = subtrahend(m);
 #pragma unroll
         for (int b = 0; b < N; ++b)
 #pragma unroll
