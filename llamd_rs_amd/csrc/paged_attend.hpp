@@ -347,7 +347,7 @@ __device__ __forceinline__ void attend_few8(const PagedArgs &p, const Pages<Elem
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
-                    s[b] = mul16<E>(widen(k[b][c][2 * h], k[b][c][2 * h + 1], 1.0f), q[2 * c + h], s[b]);
+                    s[b] = mul16<E>(widen(k[b][c][2 * h], k[b][c][2 * h + 1], 0x1p-8f), q[2 * c + h], s[b]);
         if constexpr (masked) {
 #pragma unroll
             for (int b = 0; b < 4; ++b)
@@ -359,8 +359,9 @@ __device__ __forceinline__ void attend_few8(const PagedArgs &p, const Pages<Elem
         }
         // (what lies in place of a scale that is none may be anything)
         const bool some = valid >> (SCALE_BLOCK * g) & 1;
-        // (inside f32's range: 0 scores, and masked ones, stay what they are)
-        st.softmax(s, fminf(fmaxf(scale * unit_of(some ? ek : 127u), 0x1p-126f), 0x1.fffffep127f));
+        // (K was taken 2^-8 of its numbers, 1.75 at most: as they are, up to 448, large q would pass f32's range before the unit
+        // is in. Inside that range: 0 scores, and masked ones, stay what they are)
+        st.softmax(s, fminf(fmaxf(scale * unit_of(some ? ek : 127u) * 0x1p8f, 0x1p-126f), 0x1.fffffep127f));
         const float unit = unit_of(some ? ev : 127u);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {

@@ -15,7 +15,7 @@ FAR = 8  # dimensions that make a far row's scores
 
 # powers of two: of a far row's q and of k, each within its type
 SIZES = [("bf16", 14, 14), ("bf16", 60, 60), ("bf16", 0, 110), ("bf16", 119, 1), ("f32", 14, 13), ("f32", 50, 70), ("f32", 119, 0),
-         ("f16", 14, 13), ("f16", 13, 14), ("8", 26, 1), ("8", 31, 0), ("8", 60, 60), ("8", 0, 115), ("8", 95, -60),
+         ("f16", 14, 13), ("f16", 13, 14), ("8", 26, 1), ("8", 31, 0), ("8", 60, 60), ("8", 0, 115), ("8", 120, 0), ("8", 95, -60),
          ("8", -60, 119)]
 
 
