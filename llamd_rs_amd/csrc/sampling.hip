@@ -864,7 +864,7 @@ __device__ __forceinline__ void draw_few(const SampleArgs &a, int number, const 
     if (keep && first == 0) drawn(a, number, target_of(u, total), upto, w, total, (int)(uint32_t)mine.x);
 }
 
-template <bool VEC> __global__ __launch_bounds__(DRAW) void sample_draw(SampleArgs a, Rows rows) {
+__global__ __launch_bounds__(DRAW) void sample_draw(SampleArgs a, Rows rows) {
     __shared__ u64 sums[MOST_PIECES], highest, of_k;
     __shared__ struct { int piece; u64 before; } hit;
     __shared__ unsigned in_front, near;
@@ -1053,7 +1053,7 @@ template <bool VEC> void launch(const SampleArgs &a, const Rows &rows, int n, hi
     hipLaunchKernelGGL((sample_scan<VEC>), dim3(n * rows.chunks), block, 0, st, a, rows);
     hipLaunchKernelGGL((sample_bins<VEC>), dim3(n * parts), block, 0, st, a, rows, parts);
     hipLaunchKernelGGL((sample_border<VEC>), dim3(n * parts), block, 0, st, a, rows, parts);
-    hipLaunchKernelGGL((sample_draw<VEC>), dim3(n), dim3(DRAW), 0, st, a, rows);
+    hipLaunchKernelGGL(sample_draw, dim3(n), dim3(DRAW), 0, st, a, rows);
 }
 
 }  // namespace
