@@ -511,14 +511,18 @@ int llamd_hip_paged_decode(const llamd_hip_pages *c, const llamd_hip_batch *b, c
  * and kv head, K and V apart.
  *
  * What is said above holds, with these differences. q and q_out are bf16, results
- * bf16 or f32; products and weights are those of a bf16 cache, which holds
- * every element exactly (of V, where E is 10 or more). paged8_store takes for 16 positions the least E with
- * which the new ones' largest finite value fits (448 * 2^(E - 127)), or the E
- * there where positions of the sequence before the new ones need more; where E
- * grows, those positions' numbers are rounded again (exactly but for values below
- * 2^-14 of the largest that fits). Each value is off by half a step: 2^-4 of itself,
- * or 2^-10 * 2^(E - 127). Infinities are stored as NaN. What lies in the 16
- * positions behind the new tokens is left as it was, in the E that there is now.
+ * bf16 or f32; products and weights are those of a bf16 cache (of f32 results
+ * too), which holds every element exactly where E is 10 or more and the element
+ * inside f32's range. paged8_store takes for 16 positions the least E with
+ * which the new ones' largest finite value fits (448 * 2^(E - 127), E 247 at
+ * most), but no less than the E there where the sequence has positions before the
+ * new ones (also an E that tokens needed which these replace); where E grows, those
+ * positions' numbers are rounded again (exactly but for values below 2^-14 of the
+ * largest that fits). A value is off by half a step: 2^-4 of itself or, where that is
+ * more, 2^-10 * 2^(E - 127), and 2^-9 * 2^(E - 127) once E has grown since. Values
+ * of up to 2^-10 * 2^(E - 127), about 2^-19 of the largest that fits, become 0.
+ * Infinities are stored as NaN. What lies in the 16 positions behind the new tokens
+ * is left as it was, in the E that there is now.
  * Two sequences of one call that store into the same 16 positions of a page leave
  * those undefined. */
 typedef struct {

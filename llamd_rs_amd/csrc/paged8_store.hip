@@ -6,8 +6,10 @@
 //   stored: e4m3(y * 2^(127 - E)), to nearest, ties to even: half a step, 2^-4 of a value, or 2^-10 of the unit
 //
 // Positions before the new ones stand where the block's E grows: their numbers are multiplied by 2^(old E - E), which is exact
-// down to e4m3's normal numbers: a block that fills token by token is as exact as one stored at once, but for values below
-// 2^-15 of the block's largest. Infinities and NaN are stored as NaN, and do not count for the unit.
+// down to e4m3's normal numbers, 2^-6 units: 2^-14 of the 448 units that fit. A block that fills token by token is as exact as one
+// stored at once, but below them, where the roundings add up to 2^-9 units at the most (2^-10 of the last, half as much of the one
+// before, and so on). E does not shrink while the block has positions before the new ones. Infinities and NaN are stored as NaN,
+// and do not count for the unit.
 //
 // Bound: memory, 4 (H + 2 Hkv) hd bytes read, 2 H hd + 2 Hkv hd written per token, and for a few tokens the chain of loads
 // from the length to the block's scale. One launch: queries as in paged_store.hip, a wave per token; and a workgroup per 16
@@ -16,7 +18,9 @@
 //
 // Measured (one MI355X): 8000 tokens of 32 query and 4 kv heads of 128, 238 MB, 52.1 us (4.6 TB/s, a large copy's rate is 4.7); 5
 // prompts of 16 and 8 heads, 52 MB, 14.1 us; one token 7.1 us, of which the kernel 5.2 (of a 16-bit cache
-// 4.0). The values' loads beside the page's number, and V's old bytes before the norm: 7.3, 14.6 and 53.2.
+// 4.0). The values' loads beside the page's number, and V's old bytes before the norm: 7.3, 14.6 and 53.2. With n_rot % 8 != 0
+// (pairs of single dimensions, bytes stored one by one) one token 7.6, 700 tokens 9.5 (runs 7.7), 8000 58 to 63 where the same
+// call in runs takes 40 (rows already in the caches).
 #include <algorithm>
 
 #include "paged_store.hpp"
