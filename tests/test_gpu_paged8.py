@@ -137,6 +137,35 @@ def test_positions_behind_the_new_ones_stay(gpu):
             assert same[[0, 2, 3]].all() and same[1, :, 1].all() and (b[1, :, 0] > a[1, :, 0]).all()
 
 
+def test_a_sequence_that_is_cut_and_goes_on(gpu):
+    """Inside 16 positions the unit of the tokens cut off stays and those before keep their bytes; from a multiple of 16 on the
+    unit is the new tokens'."""
+    rng = np.random.default_rng(28)
+    heads, kvh, hd, page = 2, 2, 64, 32
+    table = np.array([[1, 0]], np.int32)
+    c = gpu.PagedCache8(2, page, heads, kvh, hd)
+    x = [rng.standard_normal((40, h * hd)).astype(np.float32) for h in (heads, kvh, kvh)]
+    for a in x:
+        a[20:24] *= 2.0 ** 12
+    c.store(*x, table, [40], [0, 40])
+    before = c.read_bytes()
+    new = [rng.standard_normal((22, h * hd)).astype(np.float32) for h in (heads, kvh, kvh)]
+    c.store(*(a[:3] for a in new), table, [23], [0, 3])      # positions 20 .. 22 again
+    for i, turn in ((0, lambda b: b), (1, lambda b: b.swapaxes(2, 3))):
+        after = c.read_bytes()
+        assert np.array_equal(before[2 + i], after[2 + i])
+        was, now = turn(before[i]), turn(after[i])
+        assert np.array_equal(was[1, :, :20], now[1, :, :20]) and np.array_equal(was[1, :, 23:], now[1, :, 23:])
+        got = turn(c.read()[i])[1, :, 20:23].swapaxes(0, 1).reshape(3, -1)
+        unit = 2.0 ** (after[2 + i][1, :, 1].astype(float) - 127).repeat(hd)
+        assert (np.abs(got - new[1 + i][:3]) <= np.maximum(2.0 ** -4 * np.abs(new[1 + i][:3]), 2.0 ** -10 * unit)).all()
+    c.store(*new, table, [38], [0, 22])                      # positions 16 .. 37
+    after = c.read_bytes()
+    assert (after[2][1, :, 1] < before[2][1, :, 1]).all() and (after[3][1, :, 1] < before[3][1, :, 1]).all()
+    got = c.read()[0][1, :, 16:].swapaxes(0, 1).reshape(16, -1)
+    assert (np.abs(got - new[1][:16]) <= np.maximum(2.0 ** -4 * np.abs(new[1][:16]), 2.0 ** -10 * 2.0 ** -6)).all()
+
+
 def test_not_finite_values_are_nan_and_do_not_count(gpu):
     rng = np.random.default_rng(16)
     heads, kvh, hd, page, n = 2, 1, 64, 16, 20

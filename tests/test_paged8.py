@@ -115,3 +115,20 @@ def test_scale_bytes_on_the_host():
     assert e[0] == 127 and e[1] == 128 and e[2] == 120 and e[3] == 121 and (e[-3:] == 1).all()
     t = top[:6].astype(np.float64)
     assert (t <= 448 * 2.0 ** (e[:6] - 127)).all() and (t > 448 * 2.0 ** (e[:6] - 128)).all()
+
+
+def test_numbers_rounded_again_on_the_host():
+    """A unit that grows by steps: numbers that stay normal (2^-14 of 448 units or more) are those of one rounding, the others are
+    off by less than 2^-9 of the last unit; up to 2^-10 of it they are 0 in one rounding."""
+    rng = np.random.default_rng(1)
+    x = np.concatenate([np.exp2(rng.uniform(-24, 8.8, 20_000)), [448.0, 2.0 ** -10, 2.0 ** -9]]) * rng.choice([-1, 1], 20_003)
+    for steps in ([1], [3], [1, 1, 1, 1], [2, 5, 1], [1] * 9):
+        y, unit = rocm.from_e4m3(rocm.to_e4m3(x)).astype(np.float64), 1.0
+        for step in steps:
+            unit *= 2.0 ** step
+            y = rocm.from_e4m3(rocm.to_e4m3(y / 2.0 ** step)).astype(np.float64)
+        once = rocm.from_e4m3(rocm.to_e4m3(x / unit)).astype(np.float64)
+        large = np.abs(x / unit) >= 448 * 2.0 ** -14
+        assert np.array_equal(y[large], once[large])
+        assert (np.abs(y - x / unit) <= np.maximum(2.0 ** -4 * np.abs(x / unit), 2.0 ** -9)).all()
+        assert (once[np.abs(x / unit) <= 2.0 ** -10] == 0).all()
