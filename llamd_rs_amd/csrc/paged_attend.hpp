@@ -21,8 +21,8 @@
 // TFLOP/s of the causal half, where a library product of 8192^3 reaches 1349); f32 110 to 119 of 154. Pieces and packed
 // prompts: the steps of a CU's tiles, 1.1 us each, and 8 us to every workgroup's first product (512 tokens after 7000 81 us,
 // 9 prompts of 192 to 700 tokens 41). Decode: memory, then the chain length -> table -> keys and the second launch (1 x 4100
-// 12.8 us, 13 x 1000 in f32 20.4, 48 behind 4100 shared 25.8). 8-bit pages: 8192 tokens 562 to 594 us (925 to 978 TFLOP/s), 512
-// after 7000 83 to 86, 9 packed prompts 40.3; decode 1 x 4100 12.3, 61 x 500 to 2000 (79 MB) 28.3, of these 23 at 3.4 TB/s and
+// 12.8 us, 13 x 1000 in f32 20.4, 48 behind 4100 shared 25.8). 8-bit pages: 8192 tokens 562 to 603 us (912 to 978 TFLOP/s), 512
+// after 7000 83 to 88, 9 packed prompts 40.3; decode 1 x 4100 12.3, 61 x 500 to 2000 (79 MB) 28.3, of these 23 at 3.4 TB/s and
 // the join 5.4, 48 behind 4100 shared 25.4.
 #pragma once
 
@@ -1306,7 +1306,9 @@ int prompt_as(const PagedAttendArgs &a, hipStream_t st) {
     // 8-bit pages, whose 16-row steps are 64 positions: also where tiles would not be split and the 16-row ones are resident
     // at once with some to spare (256 tokens after 500 positions 15.8 us, in larger tiles 25.0; 9 x 40 after 900 18.6 and 30.6;
     // 16 query and 8 kv heads: 512 tokens 11.4 and 18.6; heads of 256: 9 x 100 after 900 38.9 and 55.7). Beyond: 9 x 100 after
-    // 900 of 16 and 8 heads, 584 tiles, 31.8 and 32.4; 400 tokens, 800 tiles, 19.2 and 17.1; 128 tokens after 1500 25.2 and 20.6
+    // 900 of 16 and 8 heads, 584 tiles, 31.8 and 32.4; 400 tokens, 800 tiles, 19.2 and 17.1; 128 tokens after 1500 25.2 and 20.6.
+    // Missed: sequences behind longer contexts (16 of up to 20 tokens after 2000, 38.8, in 16-row tiles 28.2), and any whose table
+    // is wider than they need, since the lengths are on the device (the first three with tables of 17 to 2048 pages: 27.3, 32.7, 21.0)
     if (bytes_of<E> && top <= tile_positions<E, HD>() * whole_steps<E>() && total * p.n_kv_head <= 16 * few_resident<HD>() * 3 / 4)
         return prompt_few<E, HD>(a, st);
     // eight waves where all CUs still have work (32 query heads on 4: 4096 tokens 175 us, four waves 195; 3000 110 and 101)

@@ -19,13 +19,16 @@
 //     added up by piece (gathered in LDS first: of a wave's 64 values few are in front, and their exponentials are what costs)
 //   sample_draw: one workgroup per row. A small top-k's tokens are sorted, cut, and sorted by index. Else the border is found
 //     among the listed tokens by digits of (x, index), then the piece that u falls into, and the token in it. Where a list is too
-//     short (most logits equal), the row is read in its place.
+//     short (each_listed), the row is read in its place.
 // Why bins and lists, not a sort: a row is read three times whatever the rule, and nothing but the lists is ever ordered.
 //
-// Bound and measured (one MI355X). Few rows: the launches, 2.6 us each, and the chain of steps in sample_draw (1 x 151936, top-k 50
-// and top-p 0.9: 14.6 us, of these 3.2 + 6.5 + 1.7 for the first three; 13 rows of 32001 with rules of their own 25 to 28). Many
-// rows: 64 x 151936 with top-p 56 us, 3 x 39 MB read: scan 8.4 us (4.7 TB/s, a large copy's rate), bins 20.7 (40 vector instructions
-// a logit, most of them of the 64-bit exponential; vector units busy 59%), border 18.5 (30, 52%), draw 10.9.
+// Bound and measured (one MI355X; calls back to back, and each launch alone under a trace, where clocks are lower and launches do not
+// follow each other closely: those do not add up to the call). Few rows: the launches, 2.6 us each, and the chain of steps in
+// sample_draw (1 x 151936, top-p 0.9 with top-k 20 14.1 us, 50 14.5, 200 20.9, 1000 23.8, without a top-k 24.0; traced at 50: scan
+// 3.2, bins 6.5, border 1.7, draw 6.1; 13 rows of 32001 with rules of their own 25 to 29; rows that fit a list are sorted whole, 500
+// logits with a top-k of 50 18.9). Many rows: 64 x 151936 with top-p 56 us, 3 x 39 MB read; traced: scan 8.4 us (4.7 TB/s, a large
+// copy's rate), bins 20.7 (40 vector instructions a logit, most of them of the 64-bit exponential; vector units busy 59%), border
+// 18.5 (30, 52%), draw 10.9. Without a border 29, min-p alone 25, greedy 15.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -323,7 +326,9 @@ template <bool VEC> __global__ __launch_bounds__(THREADS) void sample_scan(Sampl
     }
 }
 
-// A row's maxima of groups, as many as a wave holds: four groups in a number.
+// A row's maxima of groups, as many as a wave holds: four groups in a number. HELD: 163840 logits; of more, every round of bound_of
+// reads the others again, but registers for more cost every row (top-k 50 with top-p, 10 and 16 of them: 1 x 151936 14.4 and 15.0 us,
+// 201088 17.6 and 15.1, 262144 20.6 and 15.1; 64 rows 26.0 and 32.2, 34.8 and 36.2, 41.4 and 38.6).
 struct Maxima {
     static constexpr int HELD = 10;
     float4 v[HELD];
@@ -629,7 +634,10 @@ struct Listed {
     unsigned n;
 };
 
-// f(place, weight) for those of bins [lo, hi]: from the list, or where that is too short, from the row (then from all tokens).
+// f(place, weight) for those of bins [lo, hi]: from the list, or where that is too short, from the row (then from all tokens). It is
+// where the border's bins hold more than 2048 tokens: few different values, as 16-bit logits far from 0 have. One workgroup reads
+// the row then, once for each digit: 151936 16-bit logits around 24, 0.125 apart, spread 2.5, temperature 1.4, top-p 0.9: 236 us, 64
+// rows 398 (f32 logits alike 24 and 57; at temperature 1 the border lies among fewer: 42 and 69); all logits equal 660 to 830.
 template <class F>
 __device__ __forceinline__ void each_listed(const Listed &list, const Rule &r, const float *x, int n, int lo, int hi, F f) {
     if (list.n <= LIST) {
